@@ -1,0 +1,558 @@
+"""What lies between the q / k / v projections and the o projection of a decoder layer, as cases that can be timed: norms of
+queries and keys with the position rotation, writing new keys and values into a cache of 4-bit codes, reading them back, and
+attention over that cache.
+
+Every case has a plain form in elementary torch operations and the calls that a user makes of the public binding
+(ml-drift_amd/python/mldhip.py).  Tensors are the library's: [channels / 4][tokens][4], channel = head * head_dim + d, the tokens of
+all sequences one after the other.  What the paths of a layer share:
+
+  starts[s], starts[s + 1]   the rows of the tensors that belong to sequence s (rows from starts[sequences] on belong to none)
+  lengths[s]                 tokens of sequence s in the cache, the new ones included: row starts[s] + i is position
+                             lengths[s] - (starts[s + 1] - starts[s]) + i
+  page_table[s][p]           the page that holds positions p * page .. p * page + page - 1
+
+A group of `group` channels of one cached token is held as codes of 4 bits and one word of 16: value = scale * (code - zero),
+scale the smallest half of 7 significant bits with 15 * scale >= max(x, 0) - min(x, 0), zero = rint(-min(x, 0) / scale),
+code = min(max(rint(x / scale) + zero, 0), 15); the word is the half's bits with the zero point in its low 4.  Every value is a half.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+# ---------------------------------------------------------------------------------------------------
+# The cases
+# ---------------------------------------------------------------------------------------------------
+
+
+def listed():
+    return [
+        # One decode step of the layer that the decoder stack of this repository has (8 query heads of 256 on one key / value head),
+        # one sequence of a thousand tokens: the smallest call, where latency counts.
+        dict(name="attention_one_token", op="attention", sequences=1, heads=8, kv_heads=1, head_dim=256, group=32, page=64, longest=1000,
+             new=1, ragged=False, window=0, behind=0),
+        # A decode step of a serving batch, sequences of different lengths up to 4096, four query heads on a key / value head.
+        dict(name="attention_batch", op="attention", sequences=32, heads=32, kv_heads=8, head_dim=128, group=64, page=64, longest=4096,
+             new=1, ragged=True, window=0, behind=0),
+        # A decode step over long documents: the cache is all there is to read.
+        dict(name="attention_long", op="attention", sequences=4, heads=32, kv_heads=8, head_dim=128, group=64, page=64, longest=65536,
+             new=1, ragged=False, window=0, behind=0),
+        # Four speculated tokens of each sequence of a batch, a key / value head for every query head, small pages, a padded batch.
+        dict(name="attention_speculated", op="attention", sequences=16, heads=16, kv_heads=16, head_dim=64, group=32, page=16,
+             longest=2047, new=4, ragged=True, window=0, behind=3),
+        # A long prompt, the largest: matrix products bound it.
+        dict(name="attention_prompt", op="attention", sequences=1, heads=32, kv_heads=8, head_dim=128, group=64, page=64, longest=8192,
+             new=8192, ragged=False, window=0, behind=0),
+        # Chunks of prompts of different lengths behind what the cache holds already, heads of 256, a sliding window.
+        dict(name="attention_chunks", op="attention", sequences=5, heads=8, kv_heads=1, head_dim=256, group=32, page=16, longest=4001,
+             new=611, ragged=True, window=1024, behind=5),
+        # Norms and rotation of the decoder stack's layer at one token.
+        dict(name="norm_rope_one_token", op="norm_rope", tokens=1, heads=8, kv_heads=1, head_dim=256, rotary=256, norm=True, pairs=False,
+             f32=False, far=1000),
+        # The same for a prompt of 4096 tokens.
+        dict(name="norm_rope_prompt", op="norm_rope", tokens=4096, heads=32, kv_heads=8, head_dim=128, rotary=128, norm=True, pairs=False,
+             f32=False, far=4096),
+        # fp32 tensors, no norms, neighbouring channels as pairs, half of each head rotated, positions far into a long context.
+        dict(name="norm_rope_f32_far", op="norm_rope", tokens=777, heads=16, kv_heads=16, head_dim=64, rotary=32, norm=False, pairs=True,
+             f32=True, far=1000000),
+        # The new tokens of a decode step of 64 sequences into the cache, and back.
+        dict(name="append_one_token", op="append", sequences=64, kv_heads=8, head_dim=128, group=64, page=64, longest=1024, new=1,
+             ragged=True, f32=False, behind=0),
+        # Prompts of different lengths into the cache, fp32 tensors, one key / value head of 256.
+        dict(name="append_prompts", op="append", sequences=3, kv_heads=1, head_dim=256, group=32, page=16, longest=5003, new=4999,
+             ragged=True, f32=True, behind=7),
+        # The whole cache of several sequences as tensors, as a program does that hands them to another one.
+        dict(name="read_sequences", op="read", sequences=8, kv_heads=8, head_dim=128, group=64, page=64, longest=8192, new=8192,
+             ragged=False, f32=False, behind=0),
+    ]
+
+
+def _log(rng, lo, hi):
+    """A whole number of [lo, hi], spread over its logarithm."""
+    return max(lo, min(hi, int(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.999))))))
+
+
+def draw(rng):
+    op = rng.choice(["attention", "attention", "attention", "norm_rope", "append", "read"])
+    head_dim = rng.choice([64, 128, 128, 256])
+    kv_heads = rng.choice([1, 2, 4, 8])
+    group = rng.choice([32, 32, 64]) if head_dim == 64 else rng.choice([32, 64, 64, 128])
+    page = rng.choice([16, 32, 64, 64, 128])
+    if op == "norm_rope":
+        return dict(op=op, tokens=_log(rng, 1, 4096), heads=kv_heads * rng.choice([1, 2, 4]), kv_heads=kv_heads, head_dim=head_dim,
+                    rotary=rng.choice([head_dim, head_dim, head_dim // 2]), norm=rng.random() < 0.6, pairs=rng.random() < 0.4,
+                    f32=rng.random() < 0.3, far=_log(rng, 100, 2000000))
+    sequences = _log(rng, 1, 48)
+    if op == "append":
+        new = 1 if rng.random() < 0.5 else _log(rng, 2, 8192 // sequences)
+        longest = new + _log(rng, 1, 2000)
+        return dict(op=op, sequences=sequences, kv_heads=kv_heads, head_dim=head_dim, group=group, page=page, longest=longest, new=new,
+                    ragged=rng.random() < 0.7, f32=rng.random() < 0.3, behind=rng.choice([0, 0, 5]))
+    if op == "read":
+        new = _log(rng, 1, 16384 // sequences)
+        return dict(op=op, sequences=sequences, kv_heads=kv_heads, head_dim=head_dim, group=group, page=page,
+                    longest=new + rng.choice([0, _log(rng, 1, 1000)]), new=new, ragged=rng.random() < 0.5, f32=rng.random() < 0.3,
+                    behind=rng.choice([0, 0, 3]))
+    heads = kv_heads * rng.choice([1, 2, 4, 8])
+    kind = rng.choice(["one", "one", "few", "chunk"])
+    new = 1 if kind == "one" else _log(rng, 2, 16) if kind == "few" else _log(rng, 17, 2048 // min(sequences, 8))
+    if kind == "chunk":
+        sequences = min(sequences, 8)
+    longest = new + _log(rng, 1, max(64, (65536 if kind == "one" else 16384 if kind == "few" else 4096) // sequences))
+    return dict(op=op, sequences=sequences, heads=heads, kv_heads=kv_heads, head_dim=head_dim, group=group, page=page, longest=longest, new=new,
+                ragged=rng.random() < 0.6, window=rng.choice([0, 0, _log(rng, 16, 2048)]), behind=rng.choice([0, 0, 3]))
+
+
+# ---------------------------------------------------------------------------------------------------
+# Inputs
+# ---------------------------------------------------------------------------------------------------
+
+BASE, EPS = 10000.0, 1e-6
+
+
+def _block_bytes(case):
+    """Bytes of one page of one key / value head: codes of keys and of values, then their words."""
+    p, d, g = case["page"], case["head_dim"], case["group"]
+    return p * d + 4 * p * (d // g)
+
+
+def _quantized(x, group):
+    """(codes, words) of x [..., head_dim]: codes as whole numbers, words [..., head_dim / group] as 16-bit integers."""
+    v = torch.nan_to_num(x.double(), nan=0.0).clamp(-57344.0, 57344.0)
+    v = v.reshape(*x.shape[:-1], x.shape[-1] // group, group)
+    low, high = v.amin(-1).clamp(max=0.0), v.amax(-1).clamp(min=0.0)
+    span = high - low
+    # the smallest half of 7 significant bits with 15 * scale >= span: steps of 2^-20 below 2^-13, of 2^(e - 6) above
+    exponent = torch.floor(torch.log2((span / 15).clamp(min=2.0**-14)))
+    exponent = torch.where(torch.exp2(exponent) * 15 > span, (exponent - 1).clamp(min=-14.0), exponent)
+    exponent = torch.where(torch.exp2(exponent + 1) * 15 <= span, exponent + 1, exponent)
+    step = torch.exp2(exponent - 6)
+    count = torch.floor(span / (15 * step))
+    count = torch.where(count * step * 15 < span, count + 1, count)
+    scale = count * step
+    safe = torch.where(scale > 0, scale, torch.ones_like(scale))
+    zero = torch.round(-low / safe)
+    codes = (torch.round(v / safe[..., None]) + zero[..., None]).clamp(0, 15)
+    words = scale.half().view(torch.int16).to(torch.int32) | zero.to(torch.int32)
+    return codes.reshape(x.shape).to(torch.uint8), words.to(torch.int16)
+
+
+def _packed(case, k, v):
+    """Pages [pages][kv_heads][block] from keys and values [pages][kv_heads][page][head_dim]."""
+    p, d, g = case["page"], case["head_dim"], case["group"]
+    plane = min(d, 128)
+    n, h = k.shape[0], k.shape[1]
+    out = torch.empty((n, h, _block_bytes(case)), dtype=torch.uint8, device=k.device)
+    for x, is_value in ((k, False), (v, True)):
+        codes, words = _quantized(x, g)
+        if not is_value:  # [tile][plane][token][quarter][word][8 channels]: channel = 128 plane + 32 word + 8 quarter + e
+            c = codes.reshape(n, h, p // 16, 16, d // plane, plane // 32, 4, 8).permute(0, 1, 2, 4, 3, 6, 5, 7)
+        else:  # [tile][plane][4 token quads][16 cells][channels of a cell / 4][pair][token of the pair][4 channels]
+            c = codes.reshape(n, h, p // 16, 4, 2, 2, d // plane, 16, plane // 64, 4).permute(0, 1, 2, 6, 3, 7, 8, 4, 5, 9)
+        c = c.reshape(n, h, p * d // 2, 2)
+        at = p * d // 2 if is_value else 0
+        out[:, :, at:at + p * d // 2] = c[..., 0] | (c[..., 1] << 4)
+        w = words.reshape(n, h, p // 16, 16, d // g).transpose(3, 4).contiguous()  # [tile][group][token]
+        at = p * d + (2 * p * (d // g) if is_value else 0)
+        out[:, :, at:at + 2 * p * (d // g)] = w.view(torch.uint8).reshape(n, h, -1)
+    return out
+
+
+def _binding():
+    folder = os.path.join(os.getcwd(), "ml-drift_amd", "python")  # (the working folder is the repository's root)
+    if folder not in sys.path:
+        sys.path.insert(0, folder)
+    import mldhip
+    return mldhip
+
+
+def _counts(case):
+    """New tokens of every sequence, the same for every seed (they are the tensors' shapes): in a ragged batch the second of several
+    sequences is not there and the third has one new token."""
+    s, new = case["sequences"], case["new"]
+    if not case["ragged"]:
+        return torch.full((s,), new)
+    gen = torch.Generator().manual_seed(1000 * s + new)
+    counts = torch.randint((new + 1) // 2, new + 1, (s,), generator=gen)
+    counts[0] = new
+    if s > 2:
+        counts[1], counts[2] = 0, 1
+    return counts
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    host = torch.Generator().manual_seed(seed)
+    state = {"case": case}
+
+    def normal(shape, dtype):
+        return torch.randn(shape, device="cuda", generator=gen).to(dtype)
+
+    def whole(low, high, shape=(1,)):
+        return torch.randint(low, high + 1, shape, generator=host)
+
+    f32 = case.get("f32", False)
+    dtype = torch.float32 if f32 else torch.float16
+    d, hk = case["head_dim"], case["kv_heads"]
+    if case["op"] == "norm_rope":
+        t, h = case["tokens"], case["heads"]
+        state["q"], state["k"] = normal((h * d // 4, t, 4), dtype), normal((hk * d // 4, t, 4), dtype)
+        first = int(whole(0, max(0, case["far"] - t)))
+        state["positions"] = (first + torch.arange(t)).to(torch.int32).cuda()
+        state["q_weight"], state["k_weight"] = (0.2 * normal((d,), torch.float32)).to(dtype), (0.2 * normal((d,), torch.float32)).to(dtype)
+        state["out_q"], state["out_k"] = torch.zeros_like(state["q"]), torch.zeros_like(state["k"])
+        if own:
+            M = _binding()
+            op = M.qk_norm_rope_create(M.FLOAT32 if f32 else M.FLOAT16, h, hk, d, rotary_dim=case["rotary"], base=BASE, norm=case["norm"], eps=EPS,
+                                       weight_offset=1.0, interleaved=case["pairs"], max_tokens=t)
+            srcs = [state["q"], state["k"], state["positions"]] + ([state["q_weight"], state["k_weight"]] if case["norm"] else [])
+            op.bind(srcs, [state["out_q"], state["out_k"]])
+            op.set_shape(1, 1, t)
+            state["ops"] = [op]
+        return state
+
+    s, longest, new, page = case["sequences"], case["longest"], case["new"], case["page"]
+    counts = _counts(case)
+    if case["ragged"]:
+        lengths = torch.where(counts > 0, torch.maximum(counts, whole(max(1, longest // 3), longest, (s,))), 0)
+        lengths[0] = longest
+    else:
+        lengths = torch.full((s,), longest)
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
+    per = -(-longest // page)
+    pages = s * per + 3
+    t = int(starts[-1]) + case["behind"]
+    state["starts"], state["lengths"] = starts.to(torch.int32).cuda(), lengths.to(torch.int32).cuda()
+    state["table"] = torch.randperm(pages, generator=host)[:s * per].reshape(s, per).to(torch.int32).cuda()
+    state["tokens"], state["most_new"] = t, int(counts.max())
+    if case["op"] == "append":
+        state["cache"] = torch.zeros((pages, hk, _block_bytes(case)), dtype=torch.uint8, device="cuda")
+        state["k"], state["v"] = normal((hk * d // 4, t, 4), dtype), normal((hk * d // 4, t, 4), dtype)
+        state["k"] += 2 * normal((hk * d // 4, 1, 4), dtype) * (torch.rand((hk * d // 4, 1, 4), device="cuda", generator=gen) < 0.1)
+    else:
+        # keys with a few channels that lie far from zero in every token, as trained ones have, values without
+        state["cache"] = torch.empty((pages, hk, _block_bytes(case)), dtype=torch.uint8, device="cuda")
+        away = 2 * normal((hk, 1, d), torch.float32) * (torch.rand((hk, 1, d), device="cuda", generator=gen) < 0.05)
+        at = max(1, (1 << 25) // (hk * page * d))
+        for p in range(0, pages, at):
+            n = min(at, pages - p)
+            state["cache"][p:p + n] = _packed(case, normal((n, hk, page, d), torch.float32) + away, normal((n, hk, page, d), torch.float32))
+    if case["op"] == "attention":
+        state["q"] = 1.5 * normal((case["heads"] * d // 4, t, 4), dtype)
+        state["out"] = torch.zeros_like(state["q"])
+    else:
+        state["out_k"] = torch.zeros((hk * d // 4, t, 4), dtype=dtype, device="cuda")
+        state["out_v"] = torch.zeros_like(state["out_k"])
+    if own:
+        M = _binding()
+        cache = M.kv4_cache_desc(kv_heads=hk, head_dim=d, group_size=case["group"], page_size=page, pages=pages, sequences=s, pages_per_sequence=per)
+        where = [state["table"], state["lengths"], state["starts"]]
+        kind = M.FLOAT32 if f32 else M.FLOAT16
+        if case["op"] == "attention":
+            op = M.kv4_attention_create(cache, case["heads"], scale=d**-0.5, causal=True, window=case["window"], max_tokens=t, max_new_tokens=new)
+            op.bind([state["q"], state["cache"]] + where, [state["out"]])
+            state["ops"] = [op]
+        else:
+            state["ops"] = []
+            if case["op"] == "append":
+                op = M.kv4_append_create(cache, kind, max_tokens=t, max_new_tokens=new)
+                op.bind([state["k"], state["v"]] + where, [state["cache"]])
+                state["ops"].append(op)
+            op = M.kv4_read_create(cache, kind, max_tokens=t, max_new_tokens=new)
+            op.bind([state["cache"]] + where, [state["out_k"], state["out_v"]])
+            state["ops"].append(op)
+        for op in state["ops"]:
+            op.set_shape(1, 1, t)
+    return state
+
+
+# ---------------------------------------------------------------------------------------------------
+# A pass
+# ---------------------------------------------------------------------------------------------------
+
+
+def run(state):
+    case = state["case"]
+    if own:
+        stream = torch.cuda.current_stream().cuda_stream
+        for op in state["ops"]:
+            op.launch(stream)
+        if case["op"] == "norm_rope":
+            return {"q": state["out_q"], "k": state["out_k"]}
+        return {"out": state["out"]} if case["op"] == "attention" else {"k": state["out_k"], "v": state["out_v"]}
+    if case["op"] == "norm_rope":
+        return {"q": _norm_rope(state, state["q"], state["q_weight"]), "k": _norm_rope(state, state["k"], state["k_weight"])}
+    if case["op"] == "attention":
+        return {"out": _attention(state)}
+    if case["op"] == "append":
+        _append(state)
+    return _read(state)
+
+
+def _rows(x, heads):
+    """[channels / 4][tokens][4] -> [tokens][heads][head_dim]."""
+    return x.permute(1, 0, 2).reshape(x.shape[1], heads, -1)
+
+
+def _slices(x):
+    """[tokens][heads][head_dim] -> [channels / 4][tokens][4]."""
+    return x.reshape(x.shape[0], -1, 4).permute(1, 0, 2).contiguous()
+
+
+def _norm_rope(state, x, weight):
+    case = state["case"]
+    d, r = case["head_dim"], case["rotary"]
+    y = _rows(x, x.shape[0] * 4 // d).float()
+    if case["norm"]:
+        y = y * torch.rsqrt((y * y).mean(-1, keepdim=True) + EPS) * (1.0 + weight.float())
+    frequency = BASE ** (-2.0 * torch.arange(r // 2, device="cuda", dtype=torch.float64) / r)
+    angle = (state["positions"].double()[:, None] * frequency)[:, None]
+    cos, sin = torch.cos(angle).float(), torch.sin(angle).float()
+    if case["pairs"]:
+        a, b = y[..., 0:r:2], y[..., 1:r:2]
+        turned = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+    else:
+        a, b = y[..., :r // 2], y[..., r // 2:r]
+        turned = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    return _slices(torch.cat([turned, y[..., r:]], -1).to(x.dtype))
+
+
+def _where(state):
+    """(sequence, position) of every row of the tensors that belongs to a sequence."""
+    rows = torch.arange(state["tokens"], device="cuda")
+    starts = state["starts"].long()
+    s = torch.searchsorted(starts[1:].contiguous(), rows, right=True).clamp(max=starts.numel() - 2)
+    return s, state["lengths"].long()[s] - starts[s + 1] + rows, rows < starts[-1]
+
+
+def _values(codes, words, group):
+    """Values of codes [..., head_dim] with their words [..., head_dim / group]."""
+    words = words.to(torch.int32) & 0xFFFF
+    scale = (words & 0xFFF0).to(torch.int16).view(torch.float16).float()
+    return (codes.float().unflatten(-1, (-1, group)) - (words & 15).float()[..., None]).mul_(scale[..., None]).flatten(-2)
+
+
+def _unpacked(case, blocks):
+    """Keys and values [..., page, head_dim] of blocks [..., block]."""
+    p, d, g = case["page"], case["head_dim"], case["group"]
+    plane, lead = min(d, 128), blocks.shape[:-1]
+    found = []
+    for is_value in (False, True):
+        at = p * d // 2 if is_value else 0
+        c = blocks[..., at:at + p * d // 2].reshape(-1, p * d // 2)
+        c = torch.stack([c & 15, c >> 4], -1)
+        if not is_value:
+            c = c.reshape(-1, p // 16, d // plane, 16, 4, plane // 32, 8).permute(0, 1, 3, 2, 5, 4, 6)
+        else:
+            c = c.reshape(-1, p // 16, d // plane, 4, 16, plane // 64, 2, 2, 4).permute(0, 1, 3, 6, 7, 2, 4, 5, 8)
+        at = p * d + (2 * p * (d // g) if is_value else 0)
+        w = blocks[..., at:at + 2 * p * (d // g)].contiguous().view(torch.int16).reshape(-1, p // 16, d // g, 16).transpose(2, 3)
+        found.append(_values(c.reshape(*lead, p, d), w.reshape(*lead, p, d // g), g))
+    return found
+
+
+def _cached(state):
+    """Keys and values [sequences][kv_heads][positions][head_dim] of every page that the table names."""
+    case = state["case"]
+    blocks = state["cache"][state["table"].long()].transpose(1, 2)  # [sequence][kv head][page]
+    return [x.flatten(2, 3) for x in _unpacked(case, blocks)]
+
+
+def _append(state):
+    """The new rows' codes and words into their bytes of the cache."""
+    case = state["case"]
+    p, d, g, hk = case["page"], case["head_dim"], case["group"], case["kv_heads"]
+    plane = min(d, 128)
+    s, position, inside = _where(state)
+    rows = torch.nonzero(inside & (position >= 0)).flatten()
+    s, position = s[rows], position[rows]
+    page = state["table"].long()[s, position // p]
+    block = (page[:, None] * hk + torch.arange(hk, device="cuda")) * _block_bytes(case)  # [row][kv head]
+    tile, token = position % p // 16, position % 16
+    flat = state["cache"].view(-1)
+    channel = torch.arange(0, d, 2, device="cuda")  # the even channel of every byte
+    inner = channel % plane
+    for x, is_value in ((state["k"], False), (state["v"], True)):
+        codes, words = _quantized(_rows(x, hk)[rows], g)
+        if not is_value:
+            at = (tile[:, None] * (d // plane) + channel // plane) * (8 * plane) + token[:, None] * (plane // 2) + inner % 32 // 8 * (plane // 8) + inner // 32 * 4 + inner % 8 // 2
+        else:
+            cell = plane // 16
+            at = (tile[:, None] * (d // plane) + channel // plane) * (8 * plane) + (token[:, None] // 4 * 16 + inner // cell) * (2 * cell) + inner % cell // 4 * 8 + token[:, None] % 4 * 2 + inner % 4 // 2 + p * d // 2
+        flat[block[:, :, None] + at[:, None]] = codes[..., 0::2] | (codes[..., 1::2] << 4)
+        at = p * d + (2 * p * (d // g) if is_value else 0) + 2 * ((tile[:, None] * (d // g) + torch.arange(d // g, device="cuda")) * 16 + token[:, None])
+        flat.view(torch.int16)[(block[:, :, None] + at[:, None]) // 2] = words
+
+
+def _read(state):
+    case = state["case"]
+    s, position, inside = _where(state)
+    valid = (inside & (position >= 0))[:, None, None]
+    at = position.clamp(min=0)
+    found = []
+    for x, old in zip(_cached(state), (state["out_k"], state["out_v"])):
+        found.append(_slices(torch.where(valid, x[s, :, at], torch.zeros((), device="cuda")).to(old.dtype)))
+    return {"k": found[0], "v": found[1]}
+
+
+def _attention(state):
+    case = state["case"]
+    hk, d, n, seqs = case["kv_heads"], case["head_dim"], state["most_new"], case["sequences"]
+    k, v = _cached(state)
+    starts, lengths = state["starts"].long(), state["lengths"].long()
+    counts = starts[1:] - starts[:-1]
+    rows = starts[:-1, None] + torch.arange(n, device="cuda")
+    q = _rows(state["q"], case["heads"]).float()[rows.clamp(max=state["tokens"] - 1)]  # [sequence][new][head][head_dim]
+    q = q.reshape(seqs, n, hk, -1, d).permute(0, 2, 3, 1, 4)  # [sequence][kv head][head of it][new][head_dim]
+    scores = torch.matmul(q.reshape(seqs, hk, -1, d), k.transpose(2, 3).contiguous()).mul_(d**-0.5).unflatten(2, (-1, n))
+    position = (lengths - counts)[:, None] + torch.arange(n, device="cuda")
+    at = torch.arange(k.shape[2], device="cuda")
+    seen = (at <= position[..., None]) & (at < lengths[:, None, None])
+    if case["window"]:
+        seen &= at > position[..., None] - case["window"]
+    scores.masked_fill_(~seen[:, None, None], -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    weights = scores.sub_(torch.where(torch.isinf(top), torch.zeros_like(top), top)).exp_()
+    total = weights.sum(-1, keepdim=True)
+    out = torch.matmul(weights.flatten(2, 3), v).unflatten(2, (-1, n)) / torch.where(total > 0, total, torch.ones_like(total))
+    out = out.permute(0, 3, 1, 2, 4).reshape(seqs, n, -1)  # [sequence][new][channels]
+    s, _, inside = _where(state)
+    row = torch.arange(state["tokens"], device="cuda") - starts[s]
+    found = out[s, row.clamp(0, n - 1)]
+    return _slices(torch.where(inside[:, None], found, torch.zeros((), device="cuda")).to(state["q"].dtype).unflatten(-1, (-1, d)))
+
+
+# ---------------------------------------------------------------------------------------------------
+# What a pass cannot do without
+# ---------------------------------------------------------------------------------------------------
+
+
+def work(case):
+    d, hk = case["head_dim"], case["kv_heads"]
+    size = 4 if case.get("f32", False) else 2
+    if case["op"] == "norm_rope":
+        n = case["tokens"] * (case["heads"] + hk) * d
+        return {"bytes": 2 * size * n + 4 * case["tokens"], "flops": 10 * n}
+    s, longest, rows = case["sequences"], case["longest"], int(_counts(case).sum())
+    held = s * max(case["new"], 0.67 * longest) if case["ragged"] else s * longest  # (the middle of what prepare() draws)
+    token = hk * (d + 4 * (d // case["group"]))  # bytes of one cached token
+    if case["op"] == "append":
+        return {"bytes": 4 * size * rows * hk * d + rows * token, "flops": 20 * rows * hk * d}
+    if case["op"] == "read":
+        return {"bytes": 2 * size * rows * hk * d + rows * token, "flops": 4 * rows * hk * d}
+    window = case["window"] or longest
+    each = rows / s
+    seen = min(window, max(1.0, held / s - each / 2))  # keys that a row sees, about
+    touched = s * min(held / s, window + each)
+    return {"bytes": 2 * size * rows * case["heads"] * d + touched * token, "flops": 4 * d * case["heads"] * rows * seen}
+
+
+# ---------------------------------------------------------------------------------------------------
+# The definitions in 64 bits
+# ---------------------------------------------------------------------------------------------------
+
+
+def _exact_cached(case, flat, page, offset, is_value):
+    """Values [n][kv_heads][head_dim] of positions in pages (page[n], offset[n]), from where each nibble lies."""
+    p, d, g, hk = case["page"], case["head_dim"], case["group"], case["kv_heads"]
+    c = torch.arange(d, device="cuda")
+    width = 64 if d == 64 else 128
+    head = (page[:, None] * hk + torch.arange(hk, device="cuda")[None]) * (p * d + 4 * p * d // g)
+    sixteen, t = offset // 16, offset % 16
+    part, i = c // width, c % width
+    plane = sixteen[:, None] * (8 * d) + part[None] * (8 * width)
+    if is_value:
+        per = width // 16
+        nibble = plane * 2 + (t[:, None] // 4 * 16 + i // per) * (4 * per) + i % per // 4 * 16 + t[:, None] % 4 * 4 + i % 4 + p * d
+    else:
+        nibble = plane * 2 + t[:, None] * width + i % 32 // 8 * (width // 4) + i // 32 * 8 + i % 8
+    byte = flat[head[:, :, None] + nibble[:, None] // 2].to(torch.int64)
+    code = (byte >> (4 * (nibble[:, None] % 2))) & 15
+    word = p * d + (2 * p * d // g if is_value else 0) + 2 * ((sixteen[:, None] * (d // g) + c[None] // g) * 16 + t[:, None])
+    at = head[:, :, None] + word[:, None]
+    bits = flat[at].to(torch.int64) | (flat[at + 1].to(torch.int64) << 8)
+    power, digits = (bits >> 10) & 31, (bits & 0x3F0).double()
+    scale = torch.where(power > 0, (1024 + digits) * torch.exp2(power.double() - 25), digits * 2.0**-24)
+    return scale * (code - (bits & 15)).double()
+
+
+def _exact_kept(x, group):
+    """The values that a cache keeps of x [..., head_dim]."""
+    x = x.double().reshape(*x.shape[:-1], -1, group)
+    high, low = x.amax(-1, keepdim=True).clamp(min=0), x.amin(-1, keepdim=True).clamp(max=0)
+    # all scales there are, in order: 7 significant bits, multiples of 2^-20 at the small end
+    few = torch.arange(0, 64, device="cuda", dtype=torch.float64) * 2.0**-20
+    many = (torch.arange(64, 128, device="cuda", dtype=torch.float64)[None] * torch.exp2(torch.arange(-20.0, 10.0, device="cuda", dtype=torch.float64))[:, None]).flatten()
+    scales = torch.cat([few, many])
+    s = scales[torch.searchsorted(15 * scales, high - low)]
+    one = torch.where(s > 0, s, 1.0)
+    zero = torch.round(-low / one)
+    return (s * (torch.clamp(torch.round(x / one) + zero, 0, 15) - zero)).flatten(-2)
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    d, hk = case["head_dim"], case["kv_heads"]
+
+    def sliced(x):
+        return x.reshape(x.shape[0], -1, 4).transpose(0, 1).contiguous()
+
+    def rows_of(x):
+        return x.transpose(0, 1).reshape(x.shape[1], -1, d)
+
+    if case["op"] == "norm_rope":
+        found = {}
+        r = case["rotary"]
+        for name in ("q", "k"):
+            x = rows_of(state[name]).double()
+            if case["norm"]:
+                x = x / torch.sqrt(x.pow(2).sum(-1, keepdim=True) / d + EPS) * (1 + state[name + "_weight"].double())
+            i = torch.arange(r // 2, device="cuda")
+            first, second = (2 * i, 2 * i + 1) if case["pairs"] else (i, i + r // 2)
+            turn = torch.polar(torch.ones((), dtype=torch.float64, device="cuda"), state["positions"].double()[:, None] * torch.pow(torch.tensor(BASE, dtype=torch.float64, device="cuda"), -i.double() * 2 / r))
+            z = torch.complex(x[..., first], x[..., second]) * turn[:, None]
+            y = x.clone()
+            y[..., first], y[..., second] = z.real, z.imag
+            found[name] = sliced(y)
+        return found
+
+    starts, lengths, table = state["starts"].tolist(), state["lengths"].tolist(), state["table"].long()
+    flat, p = state["cache"].view(-1), case["page"]
+    if case["op"] == "append":
+        return {name: sliced(_exact_kept(rows_of(state[name])[:starts[-1]], case["group"]).new_zeros((state["tokens"], hk, d)).index_copy(
+            0, torch.arange(starts[-1], device="cuda"), _exact_kept(rows_of(state[name])[:starts[-1]], case["group"]))) for name in ("k", "v")}
+    if case["op"] == "read":
+        found = {}
+        for name in ("k", "v"):
+            x = torch.zeros((state["tokens"], hk, d), dtype=torch.float64, device="cuda")
+            for s in range(case["sequences"]):
+                for a in range(starts[s], starts[s + 1], 2048):
+                    b = min(a + 2048, starts[s + 1])
+                    at = lengths[s] - starts[s + 1] + torch.arange(a, b, device="cuda")
+                    x[a:b] = _exact_cached(case, flat, table[s][at // p], at % p, name == "v")
+            found[name] = sliced(x)
+        return found
+
+    out = torch.zeros((state["tokens"], case["heads"], d), dtype=torch.float64, device="cuda")
+    q = rows_of(state["q"]).double()
+    share = case["heads"] // hk
+    for s in range(case["sequences"]):
+        if starts[s + 1] == starts[s] or not lengths[s]:
+            continue
+        kept = []
+        for is_value in (False, True):
+            kept.append(torch.cat([_exact_cached(case, flat, table[s][at // p], at % p, is_value) for at in torch.arange(lengths[s], device="cuda").split(4096)]))
+        where = torch.arange(lengths[s], device="cuda")
+        for a in range(starts[s], starts[s + 1], 1024):
+            b = min(a + 1024, starts[s + 1])
+            position = lengths[s] - starts[s + 1] + torch.arange(a, b, device="cuda")[:, None]
+            hidden = where > position
+            if case["window"]:
+                hidden |= where <= position - case["window"]
+            for h in range(case["heads"]):
+                z = (q[a:b, h] @ kept[0][:, h // share].T.contiguous()) / math.sqrt(d)
+                out[a:b, h] = torch.softmax(z.masked_fill(hidden, -math.inf), -1) @ kept[1][:, h // share].contiguous()
+    return {"out": sliced(out)}
