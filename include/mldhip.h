@@ -422,6 +422,98 @@ typedef struct {
 
 int mldhip_conv_int8_create(const mldhip_conv_int8_desc* desc, mldhip_op** op);
 
+/* ------------------------------------------------------------------------------------ */
+/* Between the q / k / v projections and the o projection                                 */
+/* ------------------------------------------------------------------------------------ */
+
+/* No counterparts in the reference's FullyConnected path.  These ops take the tensors that the projections of a decoder layer write and
+ * the o projection reads, [channels / 4][tokens][4] with channel = head * head_dim + channel of the head, and follow the op contract
+ * above: objects bound by index, mldhip_op_set_shape(op, 1, 1, tokens), launches on the caller's stream that neither allocate nor
+ * synchronise and may be captured.  An op runs on the device that was current when it was created (FAILED_PRECONDITION with another one
+ * current); launches of one op that has a workspace must not overlap in time. */
+
+/* Norms of the query and key heads (left out where norm is 0) and the rotation by position, in one pass:
+ *   y = x / sqrt(mean over the head's channels of x^2 + eps) * (weight_offset + weight)
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * frequency_i, for the pairs of the first rotary_dim channels of a head:
+ *   channels (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved is set; frequency_i = base^(-2 i / rotary_dim), or
+ *   frequencies[i] (host memory, read by the create call) where that is given.  Channels behind rotary_dim are normed only.
+ * fp32 arithmetic, one rounding to the tensors' type; angles are exact to 2^-32 turns at every int32 position.
+ * src objects: 0 "src_q" [heads * head_dim / 4][tokens][4], 1 "src_k" [kv_heads * head_dim / 4][tokens][4], 2 "positions" int32 [tokens],
+ * and with norms 3 "q_norm_weight", 4 "k_norm_weight" [head_dim] of the tensors' type.  dst objects: 0 "dst_q", 1 "dst_k", as the sources;
+ * each may be its source's buffer itself.  head_dim and rotary_dim are multiples of 8, head_dim at most 256. */
+typedef struct {
+  int32_t src_type;  /* MLDHIP_FLOAT16 / MLDHIP_FLOAT32 */
+  int32_t heads, kv_heads, head_dim, rotary_dim;
+  double base;
+  const double* frequencies; /* rotary_dim / 2 radians per position, or null */
+  int32_t interleaved;
+  int32_t norm;
+  float eps, weight_offset;
+  int32_t max_tokens;
+} mldhip_qk_norm_rope_desc;
+
+int mldhip_qk_norm_rope_create(const mldhip_qk_norm_rope_desc* desc, mldhip_op** op);
+
+/* A key / value cache of 4-bit codes in pages.  A group of group_size channels of one head of one token is held as codes and one 16-bit
+ * word: value = scale * (code - zero), where scale is the smallest half of 7 significant bits with 15 * scale >= max(x, 0) - min(x, 0),
+ * zero = rint(-min(x, 0) / scale) and code = min(max(rint(x / scale) + zero, 0), 15), ties to even; x is held to +-57344 first, NaN
+ * counts as 0.  Every value is a half exactly.  4 + 16 / group_size bits a channel.
+ * The cache is one buffer of mldhip_kv4_cache_bytes: [pages][kv_heads][block], a block (page_size * (head_dim + 4 * head_dim / group_size)
+ * bytes) holding a page's codes of keys, codes of values, words of keys, words of values, all in tiles of 16 tokens; with
+ * P = min(head_dim, 128):
+ *   key codes    [tile][head_dim / P][token 16][4][P / 32][8 nibbles]            channel = P i1 + 32 i4 + 8 i3 + i5
+ *   value codes  [tile][head_dim / P][4][cell 16][P / 64][2][2][4 nibbles]       channel = P i1 + P / 16 i3 + 4 i4 + i7, token = 4 i2 + 2 i5 + i6
+ *   words        [tile][head_dim / group_size][token 16]                         the scale's bits (low 4 clear) | zero
+ * (low nibble first).  A page's bytes may be copied to another page, or to another cache of the same description.
+ *
+ * What the three ops below read on the device at each launch, as src objects in this order:
+ *   "page_table" int32 [sequences][pages_per_sequence]   the pages of a sequence, in order of its positions
+ *   "lengths"    int32 [sequences]                       tokens of a sequence in the cache, the new ones included
+ *   "starts"     int32 [sequences + 1]                   rows starts[s] .. starts[s + 1] - 1 of the tensors are sequence s: row
+ *                                                        starts[s] + i has position lengths[s] - (starts[s + 1] - starts[s]) + i
+ * Rows in front of starts[0] and from starts[sequences] on belong to no sequence and are left as they are.  Positions below 0, behind
+ * what the table has room for, or on a page that is not one of the cache's are held nowhere: appended nowhere, read as zeros, never
+ * attended.  starts must not decrease. */
+typedef struct {
+  int32_t kv_heads;
+  int32_t head_dim;   /* 64, 128 or 256 */
+  int32_t group_size; /* 32, 64 or 128, at most head_dim */
+  int32_t page_size;  /* tokens: a power of two, 16 .. 1024 */
+  int32_t pages;
+  int32_t sequences;  /* at most 65535 */
+  int32_t pages_per_sequence;
+} mldhip_kv4_cache_desc;
+
+int mldhip_kv4_cache_bytes(const mldhip_kv4_cache_desc* cache, size_t* bytes);
+
+/* New keys and values into the cache.  src objects: 0 "src_k", 1 "src_v" [kv_heads * head_dim / 4][tokens][4] (src_type FLOAT16 or
+ * FLOAT32), 2 "page_table", 3 "lengths", 4 "starts"; dst 0 "cache".  Nothing but the new tokens' codes and words is written.  A page that
+ * is written must belong to one sequence; positions that two rows of a launch share end with a mixture of both.
+ * max_new_tokens: rows of one sequence that a launch is sized for (more only take longer). */
+int mldhip_kv4_append_create(const mldhip_kv4_cache_desc* cache, int src_type, int max_tokens, int max_new_tokens, mldhip_op** op);
+
+/* Cached keys and values as tensors: the positions that the rows have.  src objects: 0 "cache", 1 "page_table", 2 "lengths", 3 "starts";
+ * dst objects 0 "dst_k", 1 "dst_v" [kv_heads * head_dim / 4][tokens][4] (dst_type FLOAT16 or FLOAT32, exact in both). */
+int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int max_tokens, int max_new_tokens, mldhip_op** op);
+
+/* Attention of the rows over what the cache holds of their sequence (their own positions appended before):
+ *   out_r = sum_t softmax_t(scale * q_r . k_t) v_t,  t < lengths[s]; causal: t <= position of r; window > 0: t > position of r - window.
+ * A row that sees no position is 0.  Query head h reads key / value head h / (heads / kv_heads).  src objects: 0 "src_q"
+ * [heads * head_dim / 4][tokens][4] halfs, 1 "cache", 2 "page_table", 3 "lengths", 4 "starts"; dst 0 "dst_tensor", as src_q (another buffer).
+ * fp16 tensors; scores, softmax and sums in fp32, the probabilities rounded to halfs for the second product.
+ * max_new_tokens chooses between the kernels for few and for many rows of a sequence; launches with more rows than that are served. */
+typedef struct {
+  mldhip_kv4_cache_desc cache;
+  int32_t heads; /* a multiple of cache.kv_heads */
+  float scale;   /* positive */
+  int32_t causal;
+  int32_t window; /* 0: none */
+  int32_t max_tokens;
+  int32_t max_new_tokens;
+} mldhip_kv4_attention_desc;
+
+int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* desc, mldhip_op** op);
+
 /* Introspection of the object lists, in registration order (GPUOperation::src_tensors_names_,
  * dst_tensors_names_, common/task/gpu_operation.h:97-274). */
 int mldhip_op_src_count(const mldhip_op* op);

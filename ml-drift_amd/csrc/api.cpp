@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <hip/hip_runtime_api.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -11,6 +12,7 @@
 
 #include "../../include/mldhip.h"
 #include "kernels.h"
+#include "kv4.h"
 #include "packer.h"
 
 using namespace mldhip;
@@ -85,7 +87,7 @@ int CheckDesc(const mldhip_weights_desc* d) {
 }  // namespace
 
 struct mldhip_op {
-  enum Kind { kFc, kQuant, kConvInt8 } kind = kFc;
+  enum Kind { kFc, kQuant, kConvInt8, kNormRope, kKv4Append, kKv4Read, kKv4Attention } kind = kFc;
   std::vector<std::string> src_names, dst_names;
   std::vector<const void*> src_ptr;
   std::vector<size_t> src_bytes;
@@ -96,6 +98,11 @@ struct mldhip_op {
   mldhip_fc_desc fc{};
   mldhip_quant_desc q{};
   mldhip_conv_int8_desc cv{};
+  mldhip_qk_norm_rope_desc nr{};
+  mldhip_kv4_attention_desc at{};  // (append, read: cache, max_new_tokens)
+  int tensor_type = 0;             // append, read
+  uint64_t* turns = nullptr;       // norms and rotation: turns per position, on the device
+  int device = -1;                 // the ops above and attention: current when the op was created; -1 without a GPU
   int idx_scale = -1, idx_zp = -1, idx_bias = -1;
   // FullyConnected with batched weights selected by a runtime tensor of ids
   int idx_weights = 1, idx_ids = -1;
@@ -594,6 +601,264 @@ int mldhip_conv_int8_create(const mldhip_conv_int8_desc* d, mldhip_op** out) {
   return MLDHIP_OK;
 }
 
+// ---------------------------------------------------------------------------------------
+// between the q / k / v projections and the o projection
+// ---------------------------------------------------------------------------------------
+
+// The device that an op's memory is allocated on; -1 on a host without a GPU, where ops can be created and inspected only.
+static int CurrentDevice() {
+  int devices = 0, device = -1;
+  if (hipGetDeviceCount(&devices) != hipSuccess || devices == 0 || hipGetDevice(&device) != hipSuccess) {
+    (void)hipGetLastError();
+    return -1;
+  }
+  return device;
+}
+
+int mldhip_qk_norm_rope_create(const mldhip_qk_norm_rope_desc* d, mldhip_op** out) {
+  if (!d || !out) return Fail(MLDHIP_INVALID_ARGUMENT, "null argument");
+  *out = nullptr;
+  if (d->src_type != MLDHIP_FLOAT16 && d->src_type != MLDHIP_FLOAT32)
+    return Fail(MLDHIP_INVALID_ARGUMENT, "tensors must be FLOAT16 or FLOAT32");
+  if (d->heads < 1 || d->kv_heads < 1 || d->max_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "bad shape");
+  if ((long long)d->heads + d->kv_heads > 65535) return Fail(MLDHIP_OUT_OF_RANGE, "more than 65535 heads");
+  if (d->head_dim < 8 || d->head_dim % 8 != 0) return Fail(MLDHIP_INVALID_ARGUMENT, "head_dim must be a multiple of 8");
+  if (d->head_dim > 256) return Fail(MLDHIP_UNIMPLEMENTED, "heads of more than 256 channels are not served");
+  if (d->rotary_dim < 0 || d->rotary_dim % 8 != 0 || d->rotary_dim > d->head_dim)
+    return Fail(MLDHIP_INVALID_ARGUMENT, "rotary_dim must be a multiple of 8, at most head_dim");
+  if ((d->interleaved != 0 && d->interleaved != 1) || (d->norm != 0 && d->norm != 1))
+    return Fail(MLDHIP_INVALID_ARGUMENT, "interleaved and norm must be 0 or 1");
+  if (d->norm && !(d->eps >= 0.0f && std::isfinite(d->eps) && std::isfinite(d->weight_offset)))
+    return Fail(MLDHIP_INVALID_ARGUMENT, "eps must not be negative, eps and weight_offset finite");
+  if (!d->frequencies && !(d->base > 0.0 && std::isfinite(d->base))) return Fail(MLDHIP_INVALID_ARGUMENT, "base must be positive");
+  uint64_t turns[128] = {};
+  for (int i = 0; i < d->rotary_dim / 2; ++i) {
+    const long double f = d->frequencies ? (long double)d->frequencies[i] : std::pow((long double)d->base, -2.0L * i / d->rotary_dim);
+    if (!std::isfinite(f)) return Fail(MLDHIP_INVALID_ARGUMENT, "frequencies must be finite");
+    long double t = f / 6.283185307179586476925286766559005768L;
+    t -= std::floor(t);
+    const long double whole = std::floor(std::ldexp(t, 64) + 0.5L);
+    turns[i] = whole >= 18446744073709551616.0L ? 0 : (uint64_t)whole;
+  }
+  mldhip_op* op = new (std::nothrow) mldhip_op();
+  if (!op) return Fail(MLDHIP_INTERNAL, "out of memory");
+  op->kind = mldhip_op::kNormRope;
+  op->nr = *d;
+  op->nr.frequencies = nullptr;
+  op->max_tokens = d->max_tokens;
+  op->AddSrc("src_q");
+  op->AddSrc("src_k");
+  op->AddSrc("positions");
+  if (d->norm) {
+    op->AddSrc("q_norm_weight");
+    op->AddSrc("k_norm_weight");
+  }
+  op->AddDst("dst_q");
+  op->AddDst("dst_k");
+  op->device = CurrentDevice();
+  if (op->device >= 0 && d->rotary_dim > 0) {
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&op->turns), sizeof(turns));
+    if (e == hipSuccess) e = hipMemcpy(op->turns, turns, sizeof(turns), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+      mldhip_op_destroy(op);
+      return HipFail(e, "table of frequencies");
+    }
+  }
+  UpdateRequiredSizes(op);
+  *out = op;
+  return MLDHIP_OK;
+}
+
+static int CheckKv4Cache(const mldhip_kv4_cache_desc* c) {
+  if (!c) return Fail(MLDHIP_INVALID_ARGUMENT, "null cache description");
+  if (c->kv_heads < 1 || c->pages < 1 || c->sequences < 1 || c->pages_per_sequence < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "bad cache shape");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return Fail(MLDHIP_UNIMPLEMENTED, "head_dim must be 64, 128 or 256");
+  if ((c->group_size != 32 && c->group_size != 64 && c->group_size != 128) || c->group_size > c->head_dim)
+    return Fail(MLDHIP_INVALID_ARGUMENT, "group_size must be 32, 64 or 128, at most head_dim");
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0)
+    return Fail(MLDHIP_INVALID_ARGUMENT, "page_size must be a power of two, 16 .. 1024");
+  if (c->kv_heads > 32767 || c->sequences > 65535) return Fail(MLDHIP_OUT_OF_RANGE, "at most 32767 key / value heads and 65535 sequences");
+  if ((long long)c->pages_per_sequence * c->page_size > 1 << 30) return Fail(MLDHIP_OUT_OF_RANGE, "more than 2^30 positions in a sequence");
+  return MLDHIP_OK;
+}
+
+static size_t Kv4CacheBytes(const mldhip_kv4_cache_desc& c) {
+  return (size_t)c.pages * c.kv_heads * Kv4BlockBytes(c.page_size, c.head_dim, c.head_dim / c.group_size);
+}
+
+int mldhip_kv4_cache_bytes(const mldhip_kv4_cache_desc* cache, size_t* bytes) {
+  if (!bytes) return Fail(MLDHIP_INVALID_ARGUMENT, "null output");
+  if (int rc = CheckKv4Cache(cache)) return rc;
+  *bytes = Kv4CacheBytes(*cache);
+  return MLDHIP_OK;
+}
+
+static int CreateKv4Move(const mldhip_kv4_cache_desc* cache, int type, int max_tokens, int max_new_tokens, bool read, mldhip_op** out) {
+  if (!out) return Fail(MLDHIP_INVALID_ARGUMENT, "null argument");
+  *out = nullptr;
+  if (int rc = CheckKv4Cache(cache)) return rc;
+  if (type != MLDHIP_FLOAT16 && type != MLDHIP_FLOAT32) return Fail(MLDHIP_INVALID_ARGUMENT, "tensors must be FLOAT16 or FLOAT32");
+  if (max_tokens < 1 || max_new_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "max_tokens and max_new_tokens must be positive");
+  mldhip_op* op = new (std::nothrow) mldhip_op();
+  if (!op) return Fail(MLDHIP_INTERNAL, "out of memory");
+  op->kind = read ? mldhip_op::kKv4Read : mldhip_op::kKv4Append;
+  op->at.cache = *cache;
+  op->at.max_new_tokens = max_new_tokens;
+  op->tensor_type = type;
+  op->max_tokens = max_tokens;
+  op->device = CurrentDevice();
+  if (read) {
+    op->AddSrc("cache");
+  } else {
+    op->AddSrc("src_k");
+    op->AddSrc("src_v");
+  }
+  op->AddSrc("page_table");
+  op->AddSrc("lengths");
+  op->AddSrc("starts");
+  if (read) {
+    op->AddDst("dst_k");
+    op->AddDst("dst_v");
+  } else {
+    op->AddDst("cache");
+  }
+  UpdateRequiredSizes(op);
+  *out = op;
+  return MLDHIP_OK;
+}
+
+int mldhip_kv4_append_create(const mldhip_kv4_cache_desc* cache, int src_type, int max_tokens, int max_new_tokens, mldhip_op** out) {
+  return CreateKv4Move(cache, src_type, max_tokens, max_new_tokens, false, out);
+}
+int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int max_tokens, int max_new_tokens, mldhip_op** out) {
+  return CreateKv4Move(cache, dst_type, max_tokens, max_new_tokens, true, out);
+}
+
+// The cache and the sequences as the kernels are told; the three device arrays are consecutive src objects.
+static Kv4Where Kv4WhereOf(const mldhip_op* op, int first_object) {
+  const mldhip_kv4_cache_desc& c = op->at.cache;
+  Kv4Where w;
+  w.table = static_cast<const int32_t*>(op->src_ptr[first_object]);
+  w.lengths = static_cast<const int32_t*>(op->src_ptr[first_object + 1]);
+  w.starts = static_cast<const int32_t*>(op->src_ptr[first_object + 2]);
+  w.kv_heads = c.kv_heads;
+  w.group_shift = c.group_size == 32 ? 5 : c.group_size == 64 ? 6 : 7;
+  while ((1 << w.page_shift) < c.page_size) ++w.page_shift;
+  w.pages = c.pages;
+  w.sequences = c.sequences;
+  w.pages_per_sequence = c.pages_per_sequence;
+  w.tokens = op->Tokens();
+  w.block_bytes = (uint32_t)Kv4BlockBytes(c.page_size, c.head_dim, c.head_dim / c.group_size);
+  return w;
+}
+
+static Kv4AttentionArgs Kv4AttentionArgsOf(mldhip_op* op) {
+  const mldhip_kv4_attention_desc& d = op->at;
+  Kv4AttentionArgs a;
+  a.where = Kv4WhereOf(op, 2);
+  a.q = op->src_ptr[0];
+  a.cache = static_cast<const uint8_t*>(op->src_ptr[1]);
+  a.out = op->dst_ptr[0];
+  a.partial = op->partial;
+  a.head_dim = d.cache.head_dim;
+  a.heads = d.heads;
+  a.max_new = d.max_new_tokens;
+  a.max_tokens = d.max_tokens;
+  a.causal = d.causal;
+  a.window = d.window;
+  a.scale = d.scale;
+  a.variant = &op->last_variant;
+  a.tiles = op->last_tiles;
+  return a;
+}
+
+int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* d, mldhip_op** out) {
+  if (!d || !out) return Fail(MLDHIP_INVALID_ARGUMENT, "null argument");
+  *out = nullptr;
+  if (int rc = CheckKv4Cache(&d->cache)) return rc;
+  if (d->heads < 1 || d->heads % d->cache.kv_heads != 0) return Fail(MLDHIP_INVALID_ARGUMENT, "heads must be a multiple of kv_heads");
+  if (d->max_tokens < 1 || d->max_new_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "max_tokens and max_new_tokens must be positive");
+  if ((long long)d->max_tokens * d->heads > 1 << 30) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens * heads exceeds 2^30");
+  if (!(d->scale > 0.0f && std::isfinite(d->scale))) return Fail(MLDHIP_INVALID_ARGUMENT, "scale must be positive");
+  if (d->causal != 0 && d->causal != 1) return Fail(MLDHIP_INVALID_ARGUMENT, "causal must be 0 or 1");
+  if (d->window < 0 || d->window > 1 << 30) return Fail(MLDHIP_INVALID_ARGUMENT, "window must be 0 .. 2^30");
+  mldhip_op* op = new (std::nothrow) mldhip_op();
+  if (!op) return Fail(MLDHIP_INTERNAL, "out of memory");
+  op->kind = mldhip_op::kKv4Attention;
+  op->at = *d;
+  op->max_tokens = d->max_tokens;
+  op->AddSrc("src_q");
+  op->AddSrc("cache");
+  op->AddSrc("page_table");
+  op->AddSrc("lengths");
+  op->AddSrc("starts");
+  op->AddDst("dst_tensor");
+  op->device = CurrentDevice();
+  op->partial_floats = Kv4AttentionWorkspaceFloats(Kv4AttentionArgsOf(op));
+  if (op->device >= 0 && op->partial_floats > 0) {
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&op->partial), op->partial_floats * sizeof(float));
+    if (e != hipSuccess) {
+      mldhip_op_destroy(op);
+      return HipFail(e, "hipMalloc(workspace)");
+    }
+  }
+  UpdateRequiredSizes(op);
+  *out = op;
+  return MLDHIP_OK;
+}
+
+// Launches of these ops.
+static int LaunchAroundAttention(mldhip_op* op, hipStream_t stream) {
+  int device = -1;
+  if (hipGetDevice(&device) != hipSuccess || device != op->device) {
+    (void)hipGetLastError();
+    return Fail(MLDHIP_FAILED_PRECONDITION, "the op was created with another device current");
+  }
+  op->last_variant = "";
+  std::fill_n(op->last_tiles, 3, 0);
+  hipError_t e = hipSuccess;
+  if (op->kind == mldhip_op::kNormRope) {
+    const mldhip_qk_norm_rope_desc& d = op->nr;
+    NormRopeArgs a;
+    a.src_q = op->src_ptr[0];
+    a.src_k = op->src_ptr[1];
+    a.positions = static_cast<const int32_t*>(op->src_ptr[2]);
+    if (d.norm) {
+      a.q_weight = op->src_ptr[3];
+      a.k_weight = op->src_ptr[4];
+    }
+    a.dst_q = op->dst_ptr[0];
+    a.dst_k = op->dst_ptr[1];
+    a.turns = op->turns;
+    a.tokens = op->Tokens();
+    a.heads = d.heads;
+    a.kv_heads = d.kv_heads;
+    a.head_dim = d.head_dim;
+    a.rotary_dim = d.rotary_dim;
+    a.eps = d.eps;
+    a.weight_offset = d.weight_offset;
+    a.f16 = d.src_type == MLDHIP_FLOAT16;
+    a.norm = d.norm != 0;
+    a.interleaved = d.interleaved != 0;
+    e = LaunchQkNormRope(a, stream, &op->last_kernel);
+  } else if (op->kind == mldhip_op::kKv4Attention) {
+    e = LaunchKv4Attention(Kv4AttentionArgsOf(op), stream, &op->last_kernel);
+  } else {
+    const bool read = op->kind == mldhip_op::kKv4Read;
+    Kv4MoveArgs a;
+    a.where = Kv4WhereOf(op, read ? 1 : 2);
+    a.k = read ? op->dst_ptr[0] : const_cast<void*>(op->src_ptr[0]);
+    a.v = read ? op->dst_ptr[1] : const_cast<void*>(op->src_ptr[1]);
+    a.cache = read ? const_cast<void*>(op->src_ptr[0]) : op->dst_ptr[0];
+    a.head_dim = op->at.cache.head_dim;
+    a.max_new = op->at.max_new_tokens;
+    a.f16 = op->tensor_type == MLDHIP_FLOAT16;
+    e = read ? LaunchKv4Read(a, stream, &op->last_kernel) : LaunchKv4Append(a, stream, &op->last_kernel);
+  }
+  if (e != hipSuccess) return HipFail(e, "kernel launch");
+  return MLDHIP_OK;
+}
+
 int mldhip_op_src_count(const mldhip_op* op) { return op ? (int)op->src_names.size() : 0; }
 int mldhip_op_dst_count(const mldhip_op* op) { return op ? (int)op->dst_names.size() : 0; }
 const char* mldhip_op_src_name(const mldhip_op* op, int index) {
@@ -679,6 +944,30 @@ static void RequiredSizes(const mldhip_op* op, std::vector<size_t>* src, std::ve
       default: (*dst)[0] = s * m * 4;
     }
     (*dst)[1] = m * 4 * sizeof(float);
+  } else if (op->kind == mldhip_op::kNormRope) {
+    const mldhip_qk_norm_rope_desc& d = op->nr;
+    const size_t tb = TypeBytes(d.src_type);
+    (*src)[0] = (*dst)[0] = m * d.heads * d.head_dim * tb;
+    (*src)[1] = (*dst)[1] = m * d.kv_heads * d.head_dim * tb;
+    (*src)[2] = m * sizeof(int32_t);
+    if (d.norm) (*src)[3] = (*src)[4] = d.head_dim * tb;
+  } else if (op->kind != mldhip_op::kConvInt8) {  // the ops over the cache of 4-bit codes
+    const mldhip_kv4_cache_desc& c = op->at.cache;
+    const size_t cache = Kv4CacheBytes(c), kv = m * c.kv_heads * c.head_dim * TypeBytes(op->tensor_type);
+    size_t next = 1;
+    if (op->kind == mldhip_op::kKv4Attention) {
+      (*src)[0] = (*dst)[0] = m * op->at.heads * c.head_dim * sizeof(uint16_t);
+      (*src)[next++] = cache;
+    } else if (op->kind == mldhip_op::kKv4Append) {
+      (*src)[0] = (*src)[next++] = kv;
+      (*dst)[0] = cache;
+    } else {
+      (*src)[0] = cache;
+      (*dst)[0] = (*dst)[1] = kv;
+    }
+    (*src)[next] = (size_t)c.sequences * c.pages_per_sequence * sizeof(int32_t);
+    (*src)[next + 1] = (size_t)c.sequences * sizeof(int32_t);
+    (*src)[next + 2] = ((size_t)c.sequences + 1) * sizeof(int32_t);
   } else {
     const mldhip_conv_int8_desc& d = op->cv;
     const size_t k16 = DivUp(d.i, 16), ns = DivUp(d.o, 4);
@@ -774,6 +1063,8 @@ int mldhip_op_launch(mldhip_op* op, void* stream_ptr) {
   if (int rc = CheckBindings(op)) return rc;
   hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
   hipError_t e = hipSuccess;
+  if (op->kind == mldhip_op::kNormRope || op->kind == mldhip_op::kKv4Append || op->kind == mldhip_op::kKv4Read || op->kind == mldhip_op::kKv4Attention)
+    return LaunchAroundAttention(op, stream);
   if (op->kind == mldhip_op::kFc) {
     const mldhip_fc_desc& d = op->fc;
     if (d.src_type == MLDHIP_INT8) {
@@ -1019,6 +1310,14 @@ int mldhip_op_cost(const mldhip_op* op, uint64_t* bytes, uint64_t* flops) {
     for (int idx : objects)
       if (idx >= 0) need_src[idx] = need_src[idx] / op->weights_batch * op->h;
   }
+  // the cache of 4-bit codes: the tokens that the launch has, or with attention all that the page table has room for
+  if (op->kind == mldhip_op::kKv4Append || op->kind == mldhip_op::kKv4Read || op->kind == mldhip_op::kKv4Attention) {
+    const mldhip_kv4_cache_desc& c = op->at.cache;
+    const uint64_t token = (uint64_t)c.kv_heads * (c.head_dim + 4 * (c.head_dim / c.group_size));
+    const uint64_t held = (uint64_t)c.sequences * c.pages_per_sequence * c.page_size;
+    (op->kind == mldhip_op::kKv4Append ? need_dst[0] : need_src[op->kind == mldhip_op::kKv4Read ? 0 : 1]) =
+        token * (op->kind == mldhip_op::kKv4Attention ? held : (uint64_t)op->Tokens());
+  }
   uint64_t total = 0;
   for (size_t v : need_src) total += v;
   for (size_t v : need_dst) total += v;
@@ -1029,6 +1328,12 @@ int mldhip_op_cost(const mldhip_op* op, uint64_t* bytes, uint64_t* flops) {
       *flops = 2 * m * (uint64_t)op->src_c * (uint64_t)op->dst_c;
     else if (op->kind == mldhip_op::kConvInt8)
       *flops = 2 * m * (uint64_t)op->cv.i * (uint64_t)op->cv.o;
+    else if (op->kind == mldhip_op::kNormRope)
+      *flops = 10 * m * (uint64_t)(op->nr.heads + op->nr.kv_heads) * op->nr.head_dim;
+    else if (op->kind == mldhip_op::kKv4Attention)
+      *flops = 4 * m * (uint64_t)op->at.heads * op->at.cache.head_dim * op->at.cache.pages_per_sequence * op->at.cache.page_size;
+    else if (op->kind != mldhip_op::kQuant)
+      *flops = (op->kind == mldhip_op::kKv4Append ? 20 : 4) * m * (uint64_t)op->at.cache.kv_heads * op->at.cache.head_dim;
     else
       *flops = 5 * m * (uint64_t)op->q.channels;
   }
@@ -1038,6 +1343,7 @@ int mldhip_op_cost(const mldhip_op* op, uint64_t* bytes, uint64_t* flops) {
 void mldhip_op_destroy(mldhip_op* op) {
   if (!op) return;
   if (op->partial) (void)hipFree(op->partial);
+  if (op->turns) (void)hipFree(op->turns);
   delete op;
 }
 

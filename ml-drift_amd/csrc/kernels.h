@@ -240,6 +240,57 @@ bool FcW4MfmaGatedSupported(const FcArgs& gate, const FcArgs& up);
 hipError_t LaunchFcW4MfmaGated(const FcArgs& gate, const FcArgs& up, int activation, void* dst, hipStream_t stream,
                                const char** kernel_name);
 
+// Norms of the query and key heads and the rotation by position (qk_norm_rope.hip).
+struct NormRopeArgs {
+  const void *src_q = nullptr, *src_k = nullptr;
+  const int32_t* positions = nullptr;  // [tokens]
+  const void *q_weight = nullptr, *k_weight = nullptr;  // [head_dim], read where norm is set
+  void *dst_q = nullptr, *dst_k = nullptr;
+  const uint64_t* turns = nullptr;  // [rotary_dim / 2]: turns per position as a 64-bit fraction
+  int tokens = 0, heads = 0, kv_heads = 0, head_dim = 0, rotary_dim = 0;
+  int heads_per_group = 1;  // heads that a work-group takes one after the other (set by the launch)
+  float eps = 0.0f, weight_offset = 0.0f;
+  bool f16 = true, norm = false, interleaved = false;
+};
+hipError_t LaunchQkNormRope(const NormRopeArgs& a, hipStream_t stream, const char** kernel_name);
+
+// What all kernels over the cache of 4-bit codes (kv4.h) are told about it and the sequences.
+struct Kv4Where {
+  const int32_t* table = nullptr;    // [sequences][pages_per_sequence]
+  const int32_t* lengths = nullptr;  // [sequences]
+  const int32_t* starts = nullptr;   // [sequences + 1]
+  int kv_heads = 0, group_shift = 0, page_shift = 0, pages = 0, sequences = 0, pages_per_sequence = 0;
+  int tokens = 0;  // rows of the tensors
+  uint32_t block_bytes = 0;
+};
+
+// New keys and values into the cache / cached ones into tensors (kv4_cache.hip).
+struct Kv4MoveArgs {
+  Kv4Where where;
+  void *k = nullptr, *v = nullptr;  // [kv_heads * head_dim / 4][tokens][4]
+  void* cache = nullptr;
+  int head_dim = 0, max_new = 0;
+  bool f16 = true;
+};
+hipError_t LaunchKv4Append(const Kv4MoveArgs& a, hipStream_t stream, const char** kernel_name);
+hipError_t LaunchKv4Read(const Kv4MoveArgs& a, hipStream_t stream, const char** kernel_name);
+
+// Attention over the cache (kv4_attention.hip).
+struct Kv4AttentionArgs {
+  Kv4Where where;
+  const void* q = nullptr;  // [heads * head_dim / 4][tokens][4], halfs
+  const uint8_t* cache = nullptr;
+  void* out = nullptr;  // as q
+  float* partial = nullptr;  // workspace of the op: Kv4AttentionWorkspaceFloats
+  int head_dim = 0, heads = 0, max_new = 0, max_tokens = 0;
+  int causal = 1, window = 0;
+  float scale = 1.0f;
+  const char** variant = nullptr;  // out: the form that was launched
+  int* tiles = nullptr;            // out: rows of a tile, waves, parts of a sequence's keys
+};
+size_t Kv4AttentionWorkspaceFloats(const Kv4AttentionArgs& a);
+hipError_t LaunchKv4Attention(const Kv4AttentionArgs& a, hipStream_t stream, const char** kernel_name);
+
 }  // namespace mldhip
 
 #endif  // MLDHIP_KERNELS_H_

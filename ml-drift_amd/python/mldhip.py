@@ -34,6 +34,7 @@ SYMBOLS = [
     "mldhip_checkpoint_fc_probe", "mldhip_checkpoint_fc_read", "mldhip_fc_launch_gated",
     "mldhip_scale_to_tensor_batched", "mldhip_fc_batch_ids_create",
     "mldhip_fc_int4_weights_desc_reference", "mldhip_fc_int4_weights_desc_decode", "mldhip_fc_int8_weights_desc_decode", "mldhip_set_tuning", "mldhip_fc_int4_decode_noalloc",
+    "mldhip_qk_norm_rope_create", "mldhip_kv4_cache_bytes", "mldhip_kv4_append_create", "mldhip_kv4_read_create", "mldhip_kv4_attention_create",
 ]
 
 
@@ -66,6 +67,22 @@ class ConvInt8Desc(C.Structure):
     _fields_ = [("src_packed_type", C.c_int32), ("dst_type", C.c_int32), ("o", C.c_int32),
                 ("i", C.c_int32), ("weights", WeightsDesc), ("has_zero_point", C.c_int32),
                 ("has_bias", C.c_int32), ("max_tokens", C.c_int32)]
+
+
+class NormRopeDesc(C.Structure):
+    _fields_ = [("src_type", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+                ("base", C.c_double), ("frequencies", C.POINTER(C.c_double)), ("interleaved", C.c_int32), ("norm", C.c_int32),
+                ("eps", C.c_float), ("weight_offset", C.c_float), ("max_tokens", C.c_int32)]
+
+
+class Kv4CacheDesc(C.Structure):
+    _fields_ = [("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("group_size", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
+                ("sequences", C.c_int32), ("pages_per_sequence", C.c_int32)]
+
+
+class Kv4AttentionDesc(C.Structure):
+    _fields_ = [("cache", Kv4CacheDesc), ("heads", C.c_int32), ("scale", C.c_float), ("causal", C.c_int32), ("window", C.c_int32),
+                ("max_tokens", C.c_int32), ("max_new_tokens", C.c_int32)]
 
 
 class CheckpointFc(C.Structure):
@@ -477,3 +494,52 @@ def fc_int4_decode_noalloc(src, weights, scale, bias, dst, o, i, scale_groups, o
     ptr = lambda t: None if t is None else C.c_void_p(t.data_ptr())
     check(lib().mldhip_fc_int4_decode_noalloc(ptr(src), ptr(weights), ptr(scale), ptr(bias), ptr(dst), o, i,
                                               scale_groups, output_group_size, tokens, C.c_void_p(stream)))
+
+
+# ---- between the q / k / v projections and the o projection ----
+def qk_norm_rope_create(src_type, heads, kv_heads, head_dim, rotary_dim=None, base=10000.0, frequencies=None, interleaved=False, norm=False,
+                        eps=1e-6, weight_offset=0.0, max_tokens=1):
+    """Norms of the query and key heads (with `norm`) and the rotation by position.  rotary_dim: head_dim unless given.  frequencies: radians
+    per position of every pair, instead of base ** (-2 i / rotary_dim)."""
+    rotary_dim = head_dim if rotary_dim is None else rotary_dim
+    table = None
+    if frequencies is not None:
+        table = np.ascontiguousarray(frequencies, np.float64)
+        if table.shape != (rotary_dim // 2,):
+            raise ValueError("frequencies: one for each of the rotary_dim / 2 pairs")
+    d = NormRopeDesc(src_type, heads, kv_heads, head_dim, rotary_dim, base,
+                     table.ctypes.data_as(C.POINTER(C.c_double)) if table is not None else None, int(interleaved), int(norm), eps, weight_offset,
+                     max_tokens)
+    h = C.c_void_p()
+    check(lib().mldhip_qk_norm_rope_create(C.byref(d), C.byref(h)))
+    return Op(h)
+
+
+def kv4_cache_desc(kv_heads, head_dim, group_size, page_size, pages, sequences, pages_per_sequence):
+    return Kv4CacheDesc(kv_heads, head_dim, group_size, page_size, pages, sequences, pages_per_sequence)
+
+
+def kv4_cache_bytes(cache):
+    n = C.c_size_t()
+    check(lib().mldhip_kv4_cache_bytes(C.byref(cache), C.byref(n)))
+    return n.value
+
+
+def kv4_append_create(cache, src_type, max_tokens, max_new_tokens=1):
+    h = C.c_void_p()
+    check(lib().mldhip_kv4_append_create(C.byref(cache), src_type, max_tokens, max_new_tokens, C.byref(h)))
+    return Op(h)
+
+
+def kv4_read_create(cache, dst_type, max_tokens, max_new_tokens=1):
+    h = C.c_void_p()
+    check(lib().mldhip_kv4_read_create(C.byref(cache), dst_type, max_tokens, max_new_tokens, C.byref(h)))
+    return Op(h)
+
+
+def kv4_attention_create(cache, heads, scale=None, causal=True, window=0, max_tokens=1, max_new_tokens=1):
+    """scale: head_dim ** -0.5 unless given."""
+    d = Kv4AttentionDesc(cache, heads, cache.head_dim ** -0.5 if scale is None else scale, int(causal), window, max_tokens, max_new_tokens)
+    h = C.c_void_p()
+    check(lib().mldhip_kv4_attention_create(C.byref(d), C.byref(h)))
+    return Op(h)

@@ -1,0 +1,390 @@
+"""The ops between the q / k / v projections and the o projection against plain arithmetic in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import mldhip as M
+import workloads as W
+from kv4math import Cache, attention, kept, norm_rope, slices, unslices
+
+torch = pytest.importorskip("torch")
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+# ---- norms and rotation ------------------------------------------------------------------------------------------------------
+
+def run_norm_rope(q, k, positions, rotary, interleaved, dtype, norm=None, base=10000.0, frequencies=None, eps=1e-6, offset=0.0, in_place=False):
+    """q, k: [tokens][heads][head_dim]; norm: (q weight, k weight) or None."""
+    t, h, d = q.shape
+    hk = k.shape[1]
+    sq, sk = dev(slices(q).astype(dtype)), dev(slices(k).astype(dtype))
+    oq, ok = (sq, sk) if in_place else (torch.full_like(sq, 7.0), torch.full_like(sk, 7.0))
+    op = M.qk_norm_rope_create(M.FLOAT16 if dtype == np.float16 else M.FLOAT32, h, hk, d, rotary_dim=rotary, base=base, frequencies=frequencies,
+                               interleaved=interleaved, norm=norm is not None, eps=eps, weight_offset=offset, max_tokens=t)
+    srcs = [sq, sk, dev(positions.astype(np.int32))]
+    if norm is not None:
+        srcs += [dev(norm[0].astype(dtype)), dev(norm[1].astype(dtype))]
+    op.bind(srcs, [oq, ok])
+    op.set_shape(1, 1, t)
+    print("norm_rope", t, h, hk, d, rotary, interleaved, dtype.__name__, norm is not None, flush=True)
+    op.launch(stream())
+    torch.cuda.synchronize()
+    assert op.kernel_name == "qk_norm_rope_kernel"
+    return unslices(oq.cpu().numpy(), d), unslices(ok.cpu().numpy(), d)
+
+
+# What the kernel may be off by, relative to the length of a pair (a rotation keeps it): the rounding of the result, half a step
+# (2^-11 / 2^-24 of it); the sine's and cosine's own error (hardware ones 2^-19 for halfs, 4 ulp of fp32 plus 2 pi 2^-26 of the angle
+# otherwise); with norms the sum of head_dim squares, the root, the reciprocal and three products, 12 roundings of 2^-24 at most where
+# the sum is of positive terms (its own error is at most 64 additions of a lane and 4 across, half of them by the root).
+def rope_tolerance(dtype, norm):
+    eps = 2.0**-11 + 2.0**-19 if dtype == np.float16 else 2.0**-24 + 8 * 2.0**-24 + 2 * math.pi * 2.0**-26
+    return eps + (12 + 34) * 2.0**-24 * (norm is not None) + 3 * 2.0**-24
+
+
+def check_rope(got, exact, tol, rotary, interleaved):
+    mag = np.abs(exact).copy()
+    r = rotary
+    a, b = (exact[..., 0:r:2], exact[..., 1:r:2]) if interleaved else (exact[..., :r // 2], exact[..., r // 2:r])
+    length = np.sqrt(a * a + b * b)
+    if interleaved:
+        mag[..., 0:r:2] = mag[..., 1:r:2] = length
+    else:
+        mag[..., :r // 2] = mag[..., r // 2:r] = length
+    err = np.abs(got.astype(np.float64) - exact)
+    bad = err > tol * mag + 2.0**-25  # (subnormal halves: half a step is 2^-25)
+    assert not bad.any(), (np.argwhere(bad)[:3], got[bad][:3], exact[bad][:3])
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,head_dim,rotary", [
+    (1, 8, 1, 256, 256), (3, 4, 2, 128, 128), (15, 2, 2, 64, 32), (16, 5, 1, 64, 64), (17, 3, 3, 128, 64), (63, 2, 1, 256, 128),
+    (65, 4, 4, 80, 80), (200, 6, 2, 96, 96), (513, 5, 2, 128, 128), (700, 3, 1, 8, 8), (530, 1, 1, 256, 0), (33, 2, 1, 24, 16)])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("with_norm", [False, True])
+def test_norm_rope(tokens, heads, kv_heads, head_dim, rotary, dtype, interleaved, with_norm):
+    rng = np.random.default_rng(tokens * 7 + heads)
+    q = rng.standard_normal((tokens, heads, head_dim)).astype(dtype)
+    k = rng.standard_normal((tokens, kv_heads, head_dim)).astype(dtype)
+    norm = tuple(rng.standard_normal(head_dim).astype(dtype) for _ in range(2)) if with_norm else None
+    positions = rng.integers(0, 5000, tokens)
+    got = run_norm_rope(q, k, positions, rotary, interleaved, dtype, norm, offset=1.0 if with_norm else 0.0)
+    for x, y, w in zip((q, k), got, norm or (None, None)):
+        exact = norm_rope(x, positions, rotary, interleaved, weight=w, offset=1.0)
+        # (what the norm multiplies by is at most |1 + w|: the same factor for error and value)
+        check_rope(y, exact, rope_tolerance(dtype, norm), rotary, interleaved)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_norm_rope_far_and_negative_positions(dtype):
+    rng = np.random.default_rng(5)
+    q, k = rng.standard_normal((40, 2, 64)).astype(dtype), rng.standard_normal((40, 1, 64)).astype(dtype)
+    positions = np.concatenate([[0, 1, -1, -77777, 2**31 - 1, -2**31, 2**24 + 1, 10**9], rng.integers(-2**31, 2**31, 32)])
+    # float64 angles lose 2^-53 of up to 2^31 radians: 2^-22; the reference takes whole turns out in extended precision
+    got = run_norm_rope(q, k, positions, 64, False, dtype)
+    for x, y in zip((q, k), got):
+        check_rope(y, norm_rope(x, positions, 64, False), rope_tolerance(dtype, None), 64, False)
+
+
+def test_norm_rope_given_frequencies_and_in_place():
+    rng = np.random.default_rng(6)
+    q, k = rng.standard_normal((70, 3, 128)).astype(np.float16), rng.standard_normal((70, 2, 128)).astype(np.float16)
+    positions = np.arange(70) + 1000
+    frequencies = rng.uniform(0, 9, 64)  # (above 2 pi too)
+    a = run_norm_rope(q, k, positions, 128, False, np.float16, frequencies=frequencies)
+    b = run_norm_rope(q, k, positions, 128, False, np.float16, frequencies=frequencies, in_place=True)
+    for x, y, z in zip((q, k), a, b):
+        check_rope(y, norm_rope(x, positions, 128, False, frequencies=frequencies), rope_tolerance(np.float16, None), 128, False)
+        assert np.array_equal(y, z)
+
+
+def test_norm_rope_zero_rows_and_neighbours_of_infinities():
+    x = np.zeros((20, 2, 64), np.float16)
+    x[1, 0, 60], x[2, 1, 61] = np.inf, np.nan  # behind the rotary channels: their neighbours keep their values
+    x[1, 0, :8] = 1
+    got, _ = run_norm_rope(x, x[:, :1], np.zeros(20, int), 32, False, np.float16)
+    assert np.array_equal(got, x, equal_nan=True)
+    w = np.ones(64, np.float16)
+    got, _ = run_norm_rope(np.zeros((20, 2, 64), np.float16), x[:, :1] * 0, np.arange(20), 64, False, np.float16, (w, w), eps=1e-6)
+    assert np.array_equal(got, np.zeros_like(got))
+
+
+# ---- the cache -----------------------------------------------------------------------------------------------------------------
+
+def batch(rng, counts, lengths, page, extra=2):
+    """starts, lengths, page_table (random distinct pages), pages."""
+    s = len(counts)
+    per = max(1, max((l + page - 1) // page for l in lengths))
+    pages = s * per + extra
+    table = rng.permutation(pages)[:s * per].reshape(s, per)
+    return np.concatenate([[0], np.cumsum(counts)]), np.array(lengths), table, pages
+
+
+class Device:
+    """A cache on the device with its sequences."""
+
+    def __init__(self, kv_heads, head_dim, group, page, pages, starts, lengths, table, tokens=None):
+        self.desc = M.kv4_cache_desc(kv_heads, head_dim, group, page, pages, len(lengths), table.shape[1])
+        self.host = Cache(kv_heads, head_dim, group, page, pages)
+        assert M.kv4_cache_bytes(self.desc) == self.host.bytes.size
+        self.cache = torch.full((self.host.bytes.size,), 0xFF, dtype=torch.uint8, device="cuda")  # words of NaN scales: what no test reads
+        self.starts, self.lengths, self.table = starts, lengths, table
+        self.tokens = tokens or int(starts[-1])
+        self.where = [dev(np.asarray(a).astype(np.int32)) for a in (table, lengths, starts)]
+        self.most = int(max(1, np.max(np.diff(starts))))
+
+    def fill(self, rng, scale=1.0):
+        """Every page of random keys and values, through the host's layout."""
+        k, v = [rng.standard_normal((self.host.pages, self.host.kv_heads, self.host.page, self.host.head_dim)) * scale for _ in range(2)]
+        self.host.set_all(k, v)
+        self.cache.copy_(torch.from_numpy(self.host.bytes))
+
+    def append(self, k, v, dtype, most=None):
+        op = M.kv4_append_create(self.desc, M.FLOAT16 if dtype == np.float16 else M.FLOAT32, self.tokens, most or self.most)
+        a = [dev(slices(x).astype(dtype)) for x in (k, v)]
+        op.bind(a + self.where, [self.cache])
+        op.set_shape(1, 1, self.tokens)
+        print("append", self.desc.kv_heads, self.desc.head_dim, self.desc.group_size, self.desc.page_size, self.tokens, dtype.__name__, flush=True)
+        op.launch(stream())
+        torch.cuda.synchronize()
+
+    def read(self, dtype, most=None, fill=5.0):
+        op = M.kv4_read_create(self.desc, M.FLOAT16 if dtype == np.float16 else M.FLOAT32, self.tokens, most or self.most)
+        c = self.desc.kv_heads * self.desc.head_dim
+        out = [torch.full((c // 4, self.tokens, 4), fill, dtype=torch.float16 if dtype == np.float16 else torch.float32, device="cuda") for _ in range(2)]
+        op.bind([self.cache] + self.where, out)
+        op.set_shape(1, 1, self.tokens)
+        print("read", self.desc.kv_heads, self.desc.head_dim, self.desc.group_size, self.desc.page_size, self.tokens, flush=True)
+        op.launch(stream())
+        torch.cuda.synchronize()
+        return [unslices(o.cpu().numpy(), self.desc.head_dim) for o in out]
+
+    def attend(self, q, heads, causal=True, window=0, scale=None, most=None, fill=5.0, launches=1):
+        op = M.kv4_attention_create(self.desc, heads, scale=scale, causal=causal, window=window, max_tokens=self.tokens, max_new_tokens=most or self.most)
+        src = dev(slices(q).astype(np.float16))
+        out = torch.full_like(src, fill)
+        op.bind([src, self.cache] + self.where, [out])
+        op.set_shape(1, 1, self.tokens)
+        print("attend", heads, self.desc.kv_heads, self.desc.head_dim, self.desc.group_size, self.desc.page_size, self.tokens, causal, window, most, flush=True)
+        for _ in range(launches):
+            op.launch(stream())
+        torch.cuda.synchronize()
+        self.op = op
+        return unslices(out.cpu().numpy(), self.desc.head_dim)
+
+
+def edges(rng, shape, dtype):
+    """Rows of every kind: zeros, one sign only, tiny, huge, ties, infinities and NaN."""
+    x = rng.standard_normal(shape)
+    flat = x.reshape(-1, shape[-1])
+    for i, row in enumerate(flat):
+        kind = i % 11
+        if kind == 1:
+            row[:] = 0
+        elif kind == 2:
+            row[:] = np.abs(row)
+        elif kind == 3:
+            row[:] = -np.abs(row)
+        elif kind == 4:
+            row *= 2.0**-22
+        elif kind == 5:
+            row *= 30000
+        elif kind == 6:  # ties: halves of the step of a span of 15
+            row[:] = rng.integers(-14, 15, row.shape) / 2.0
+            row[0::32], row[1::32] = 8.0, -7.0
+        elif kind == 7:
+            row[3], row[5], row[9] = np.inf, -np.inf, np.nan
+        elif kind == 8:
+            row[:] = 0.1
+        elif kind == 9:
+            row *= 10.0 ** rng.uniform(-8, 4, row.shape)
+    with np.errstate(over="ignore"):
+        return x.astype(dtype)
+
+
+SHAPES = [(1, 64, 32, 16), (2, 64, 64, 32), (1, 128, 32, 64), (3, 128, 64, 16), (1, 128, 128, 128), (1, 256, 32, 16), (2, 256, 64, 64), (1, 256, 128, 1024)]
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_append_writes_the_defined_bytes_and_no_others(kv_heads, head_dim, group, page, dtype):
+    rng = np.random.default_rng(head_dim + group + page)
+    # first tokens of a page, its last ones, a page border inside, single tokens, an empty sequence, more than one page
+    counts, lengths = [1, 0, 5, 37, 1, 16, 33], [1, 9, page, page + 20, 17, 16, 70]
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    tokens = int(starts[-1]) + 3  # (rows behind the last sequence)
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table, tokens)
+    k, v = edges(rng, (tokens, kv_heads, head_dim), dtype), edges(rng, (tokens, kv_heads, head_dim), dtype)
+    d.host.bytes[:] = 0xFF
+    for s, n in enumerate(counts):
+        for i in range(n):
+            p = lengths[s] - n + i
+            if p >= 0:
+                d.host.set_token(table[s][p // page], p % page, k[starts[s] + i], v[starts[s] + i])
+    d.append(k, v, dtype)
+    got = d.cache.cpu().numpy()
+    bad = np.nonzero(got != d.host.bytes)[0]
+    assert bad.size == 0, (bad.size, bad[:5], got[bad[:5]], d.host.bytes[bad[:5]])
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_read_gives_the_values(kv_heads, head_dim, group, page, dtype):
+    rng = np.random.default_rng(head_dim + group + page + 1)
+    counts, lengths = [1, 0, 5, 37, 1, 16, 33], [1, 9, page, page + 20, 17, 16, 70]
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    tokens = int(starts[-1]) + 3
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table, tokens)
+    d.fill(rng)
+    got = d.read(dtype)
+    ek, ev = d.host.values()
+    for x, y in zip(got, (ek, ev)):
+        want = np.full((tokens, kv_heads, head_dim), 5.0)
+        for s, n in enumerate(counts):
+            for i in range(n):
+                p = lengths[s] - n + i
+                want[starts[s] + i] = y[table[s][p // page], :, p % page] if p >= 0 else 0
+        assert np.array_equal(x.astype(np.float64), want)
+
+
+def test_append_and_read_of_rows_that_have_no_place():
+    """A length shorter than the new rows, one behind the table's room, pages that are not the cache's, a sequence of more rows than the
+    launch is sized for: the rows without a place are appended nowhere and read as zeros."""
+    rng = np.random.default_rng(3)
+    starts, lengths = np.array([0, 6, 10, 30, 230]), np.array([4, 40, 20, 200])
+    table = np.array([[0, 1], [2, 3], [4, 99], [5, 6]])
+    table = np.concatenate([table, np.full((4, 12), -1)], 1)
+    table[3, :14] = 7 + np.arange(14)
+    table[1, 2:] = 6  # (positions from 32 on: one page for many positions, written by no row of this test)
+    d = Device(2, 64, 32, 16, 21, starts, lengths, table)
+    d.cache.zero_()
+    k, v = [rng.standard_normal((230, 2, 64)).astype(np.float16) for _ in range(2)]
+    starts[1] = 6
+    # sequence 1: rows at 36 .. 39 on page 6; sequence 2: positions 0 .. 19, 16 .. 19 on page 99; sequence 3: 0 .. 199
+    d.append(k, v, np.float16, most=1)
+    got = d.read(np.float16, most=1)
+    for x, y in zip(got, (k, v)):
+        want = kept(y.astype(np.float64), 32)
+        want[0:2] = 0  # positions -2, -1
+        want[26:30] = 0
+        assert np.array_equal(x.astype(np.float64), want)
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------------------
+
+# The kernels' scores are fp32 sums of exact products (halfs by integers); of a score of magnitude S = scale * sum |q||k| they are off by
+# at most about 2^-16 S (sums of up to 256 terms, codes on a base of 1024), which scales a probability by as much.  Probabilities are
+# rounded to halfs (2^-11), their products summed in fp32, the result rounded to a half (2^-11).  An output is an average of the values
+# seen, so all of it is relative to the largest |v| seen: 2^-11 + 2 * 2^-16 S for the weights (numerator and sum), 2^-11 of the output.
+def check_attention(got, exact, largest, score):
+    tol = (2.0**-11 + 2 * 2.0**-16 * score + 2.0**-18) * largest + 2.0**-11 * np.abs(exact) + 2.0**-24
+    err = np.abs(got.astype(np.float64) - exact)
+    bad = ~(err <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:3], got[bad][:3], exact[bad][:3], (err / tol).max())
+
+
+def attention_case(kv_heads, share, head_dim, group, page, counts, lengths, causal=True, window=0, seed=0, behind=0, q_scale=1.0, most=None):
+    rng = np.random.default_rng(seed)
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    tokens = int(starts[-1]) + behind
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table, tokens)
+    d.fill(rng)
+    # what lies behind a sequence's last token is never looked at: NaN words there
+    d.host.spoil(table, lengths)
+    d.cache.copy_(torch.from_numpy(d.host.bytes))
+    q = (rng.standard_normal((tokens, kv_heads * share, head_dim)) * q_scale).astype(np.float16)
+    got = d.attend(q, kv_heads * share, causal, window, most=most)
+    exact, largest, score = attention(q, d.host, table, lengths, starts, head_dim**-0.5, causal, window, fill=5.0)
+    check_attention(got, exact, largest, score)
+    return d
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("share", [1, 4, 8])
+def test_attention_one_token(kv_heads, head_dim, group, page, share):
+    attention_case(kv_heads, share, head_dim, group, page, [1] * 9, [1, 2, 15, 16, 17, 63, 64, 65, 300], seed=share)
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("window", [0, 1, 40])
+def test_attention_few_tokens(kv_heads, head_dim, group, page, window):
+    attention_case(kv_heads, 3, head_dim, group, page, [4, 1, 0, 2, 3, 6], [4, 1, 0, 2, 100, 333], window=window, behind=2, seed=window)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("share", [1, 2, 7, 16, 20])
+def test_attention_row_tiles(causal, share):
+    attention_case(2, share, 64, 32, 16, [1, 5, 13, 21], [200, 5, 77, 129], causal=causal, window=0 if causal else 50, seed=share)
+
+
+def test_attention_of_nothing():
+    """No positions at all, a length shorter than the new rows, pages that are not the cache's."""
+    rng = np.random.default_rng(8)
+    starts, lengths = np.array([0, 2, 6, 9]), np.array([0, 2, 40])
+    table = np.array([[0, 1, 2], [3, 4, 5], [6, -1, 70]])
+    d = Device(1, 128, 64, 16, 8, starts, lengths, table)
+    d.fill(rng)
+    q = rng.standard_normal((9, 4, 128)).astype(np.float16)
+    got = d.attend(q, 4)
+    assert not got[:4].any()  # (sequence 1's first two rows have positions -2 and -1)
+    exact, largest, score = attention(q, d.host, table, lengths, starts, 128**-0.5, True, 0, fill=5.0)
+    check_attention(got, exact, largest, score)
+
+
+def test_attention_sharp_and_far_apart_scores():
+    """Scores of hundreds: one position takes all; and a long cache in which every position counts the same."""
+    attention_case(1, 8, 128, 64, 64, [1, 1], [1000, 4097], q_scale=60.0)
+    attention_case(1, 8, 128, 64, 64, [1, 1], [1000, 4097], q_scale=0.0)
+
+
+def test_attention_of_rows_that_are_not_finite():
+    rng = np.random.default_rng(9)
+    starts, lengths, table, pages = batch(rng, [3, 1], [90, 70], 16)
+    d = Device(1, 64, 32, 16, pages, starts, lengths, table)
+    d.fill(rng)
+    q = rng.standard_normal((4, 2, 64)).astype(np.float16)
+    q[1, 0, 5] = np.nan
+    got = d.attend(q, 2)
+    assert np.isnan(got[1, 0]).all()
+    q2 = q.copy()
+    q2[1, 0] = 0
+    rest = d.attend(q2, 2)
+    same = np.ones((4, 2), bool)
+    same[1, 0] = False
+    assert np.array_equal(got[same], rest[same])
+
+
+# ---- together --------------------------------------------------------------------------------------------------------------------
+
+def test_a_sequence_token_by_token_is_the_prompt_at_once():
+    """Appending and attending one token at a time gives what the prompt gives in one launch each, and both what the arithmetic gives."""
+    rng = np.random.default_rng(11)
+    heads, kv_heads, head_dim, group, page, n = 4, 2, 64, 32, 16, 45
+    q, k, v = [rng.standard_normal((n, h, head_dim)).astype(np.float16) for h in (heads, kv_heads, kv_heads)]
+    table = np.array([[3, 0, 2]])
+    whole = Device(kv_heads, head_dim, group, page, 4, np.array([0, n]), np.array([n]), table)
+    whole.append(k, v, np.float16)
+    at_once = whole.attend(q, heads)
+    for i in range(n):
+        d = Device(kv_heads, head_dim, group, page, 4, np.array([0, 1]), np.array([i + 1]), table)
+        if i:
+            d.cache.copy_(cache)
+        d.append(k[i:i + 1], v[i:i + 1], np.float16)
+        cache = d.cache
+        one = d.attend(q[i:i + 1], heads)
+        whole.host.set_token(table[0][i // page], i % page, k[i], v[i])
+        exact, largest, score = attention(q[i:i + 1], whole.host, table, np.array([i + 1]), np.array([0, 1]), head_dim**-0.5, True, 0)
+        check_attention(one, exact, largest, score)
+        check_attention(at_once[i:i + 1], exact, largest, score)
+    held = np.nonzero(cache.cpu().numpy() != whole.cache.cpu().numpy())[0]
+    assert held.size == 0
