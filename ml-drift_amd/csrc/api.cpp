@@ -101,6 +101,7 @@ struct mldhip_op {
   mldhip_qk_norm_rope_desc nr{};
   mldhip_kv4_attention_desc at{};  // (append, read: cache, max_new_tokens)
   int tensor_type = 0;             // append, read
+  Kv4AttentionPlan plan;           // attention
   uint64_t* turns = nullptr;       // norms and rotation: turns per position, on the device
   int device = -1;                 // the ops above and attention: current when the op was created; -1 without a GPU
   int idx_scale = -1, idx_zp = -1, idx_bias = -1;
@@ -196,7 +197,7 @@ int mldhip_set_tuning(const char* name, int value) {
       {"gemv_lpr", &t.gemv_lpr}, {"gemv_waves", &t.gemv_waves}, {"gemv_ksplit", &t.gemv_ksplit},
       {"gemv_narrow_max_mb", &t.gemv_narrow_max_mb}, {"gemm_fm", &t.gemm_fm}, {"gemm_ksplit", &t.gemm_ksplit},
       {"gemm_no_pair", &t.gemm_no_pair}, {"gemm_waves", &t.gemm_waves}, {"gemm_dual", &t.gemm_dual}, {"gemm_xcd_m", &t.gemm_xcd_m},
-      {"gemm_i8_fm", &t.gemm_i8_fm}, {"gemm_tiled", &t.gemm_tiled}};
+      {"gemm_i8_fm", &t.gemm_i8_fm}, {"gemm_tiled", &t.gemm_tiled}, {"kv4_many", &t.kv4_many}, {"kv4_parts", &t.kv4_parts}};
   for (const auto& k : knobs)
     if (std::strcmp(name, k.name) == 0) {
       *k.field = value;
@@ -760,6 +761,7 @@ static Kv4AttentionArgs Kv4AttentionArgsOf(mldhip_op* op) {
   a.cache = static_cast<const uint8_t*>(op->src_ptr[1]);
   a.out = op->dst_ptr[0];
   a.partial = op->partial;
+  a.plan = op->plan;
   a.head_dim = d.cache.head_dim;
   a.heads = d.heads;
   a.max_new = d.max_new_tokens;
@@ -794,7 +796,9 @@ int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* d, mldhip_op** 
   op->AddSrc("starts");
   op->AddDst("dst_tensor");
   op->device = CurrentDevice();
-  op->partial_floats = Kv4AttentionWorkspaceFloats(Kv4AttentionArgsOf(op));
+  op->plan = PlanKv4Attention(Kv4AttentionArgsOf(op));
+  const int parts = std::max(op->plan.few_parts, op->plan.many_parts);
+  op->partial_floats = parts > 1 ? (size_t)parts * d->max_tokens * d->heads * (d->cache.head_dim + 2) : 0;
   if (op->device >= 0 && op->partial_floats > 0) {
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&op->partial), op->partial_floats * sizeof(float));
     if (e != hipSuccess) {

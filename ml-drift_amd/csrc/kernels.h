@@ -193,6 +193,8 @@ struct Tuning {
   int gemm_fm = -1, gemm_waves = -1, gemm_ksplit = -1, gemm_xcd_m = -1;
   int gemm_no_pair = -1, gemm_dual = -1;  // (set: the direct kernel above 32 tokens; the forms that they chose between are gone)
   int gemm_i8_fm = -1;
+  int kv4_many = -1;            // 1 / 0: attention over the 4-bit cache always / never takes the kernel for many rows (read when an op is created)
+  int kv4_parts = -1;           // work-groups that it deals the keys of a sequence to (read when an op is created)
   int gemm_tiled = -1;          // 1 / 0: always / never take the LDS-tiled int4 GEMM where it can run
 };
 Tuning& GetTuning();
@@ -275,20 +277,26 @@ struct Kv4MoveArgs {
 hipError_t LaunchKv4Append(const Kv4MoveArgs& a, hipStream_t stream, const char** kernel_name);
 hipError_t LaunchKv4Read(const Kv4MoveArgs& a, hipStream_t stream, const char** kernel_name);
 
-// Attention over the cache (kv4_attention.hip).
+// Attention over the cache (kv4_attention.hip).  Which kernel serves which sequences, and in how many parts (work-groups) each deals the
+// keys of a sequence: chosen when an op is created.
+struct Kv4AttentionPlan {
+  int few_rows = 0;  // sequences of up to this many rows (new tokens x heads of a key head) go to the kernel for few rows
+  int few_parts = 1, many_parts = 1;
+};
 struct Kv4AttentionArgs {
   Kv4Where where;
   const void* q = nullptr;  // [heads * head_dim / 4][tokens][4], halfs
   const uint8_t* cache = nullptr;
   void* out = nullptr;  // as q
-  float* partial = nullptr;  // workspace of the op: Kv4AttentionWorkspaceFloats
+  float* partial = nullptr;  // workspace of the op: parts * max_tokens * heads * (head_dim + 2) floats where there are parts
+  Kv4AttentionPlan plan;
   int head_dim = 0, heads = 0, max_new = 0, max_tokens = 0;
   int causal = 1, window = 0;
   float scale = 1.0f;
   const char** variant = nullptr;  // out: the form that was launched
   int* tiles = nullptr;            // out: rows of a tile, waves, parts of a sequence's keys
 };
-size_t Kv4AttentionWorkspaceFloats(const Kv4AttentionArgs& a);
+Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a);
 hipError_t LaunchKv4Attention(const Kv4AttentionArgs& a, hipStream_t stream, const char** kernel_name);
 
 }  // namespace mldhip

@@ -19,6 +19,7 @@ namespace {
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -36,9 +37,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // their 11 bits down to 2^-28 of it.  The common factor leaves with the division by their sum, which is taken in fp32.
 constexpr float kLift = 14.0f;
 
-constexpr int kStep = 64;  // positions that a wave takes at a time
-
-struct FewParams {
+struct AttendParams {
   Kv4Where w;
   const __half* q;
   const uint8_t* cache;
@@ -50,32 +49,60 @@ struct FewParams {
   int rows_from, rows_to;  // sequences of rows_from .. rows_to rows are this kernel's
 };
 
+// Over the four lanes that share a row (lane & 15), by register exchanges.
 __device__ __forceinline__ float MaxAcrossQuarters(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float SumAcrossQuarters(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// The masks and bases in registers whose values the compiler does not see: as literals each and-or would be two instructions.
+struct Unpack {
+  uint32_t low_mask = kLowMask, high_mask = kHighMask, low_base = kLowBase, high_base = kHighBase, scale_mask = kScaleMask;
+  __device__ __forceinline__ Unpack() { asm volatile("" : "+v"(low_mask), "+v"(high_mask), "+s"(low_base), "+s"(high_base), "+s"(scale_mask)); }
+  __device__ __forceinline__ uint32_t Low(uint32_t w) const { return (w & low_mask) | low_base; }
+  __device__ __forceinline__ uint32_t High(uint32_t w) const { return (w & high_mask) | high_base; }
+};
 
 // Few rows for each key head (single tokens, speculated ones): the cache's bytes bound it, so the keys of a sequence are dealt to the
 // waves of `parts` work-groups, each wave with its own maximum, sum and output, joined at the end.
 //
-// A wave takes 64 positions at a time against RT tiles of 16 rows, by 16x16x32 products:
+// A wave takes 32 positions at a time against RT tiles of 16 rows, by 16x16x32 products:
 //   scores^T [16 positions][16 rows] = codes of keys x q^T     a lane has one row (lane & 15) and 4 positions (4 (lane >> 4) + i)
 //   out^T   [16 cells][16 rows]     += values^T x p^T          of 32 positions: those that the lanes hold are the operand's order, so the
 //                                                              probabilities go from one product to the next in registers
 // The first product runs on the codes as they are, exact small integers; their scale and zero point, which belong to (position, group),
 // are applied to its fp32 sums, one pair of multiply-adds per 32 .. 128 codes: sum q (code - zero) = sum q (base + code) - base sum q - zero
 // sum q.  The values are dequantized, exactly (kv4.h).
-template <int D, int GJ, int RT>
-__global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams p) {
-  constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16;
-  constexpr int kGroups = D / 32 / GJ;          // groups of a head
-  constexpr int kKeyRegs = kPlanes * kWords;    // 32-bit words of a lane's keys per tile (8 channels each)
-  constexpr int kValueRegs = kPlanes * kCell / 2;  // and of its values (4 channels of 2 positions each)
-  constexpr int kTiles = kStep / 16;
+template <int D, int GJ>
+struct FewShape {
+  static constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16;
+  static constexpr int kGroups = D / 32 / GJ;             // groups of a head
+  static constexpr int kKeyRegs = kPlanes * kWords;       // 32-bit words of a lane's keys per tile (8 channels each)
+  static constexpr int kValueRegs = kPlanes * kCell / 2;  // and of its values (4 channels of 2 positions each)
+  static constexpr int kStep = 32;                        // positions that a wave takes at a time: two steps are in registers
+  static constexpr int kTiles = kStep / 16;
+};
+
+// The cached bytes of one step, as a lane holds them.
+template <int D, int GJ>
+struct FewStep {
+  using S = FewShape<D, GJ>;
+  uint32_t keys[S::kTiles][S::kKeyRegs], values[S::kTiles][S::kValueRegs];
+  u32x2 key_words[S::kTiles][S::kGroups], value_words[S::kTiles][S::kPlanes];
+};
+
+template <int D, int GJ, int RT, bool BIG>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kernel(const AttendParams p) {
+  using S = FewShape<D, GJ>;
+  constexpr int P = S::P, kPlanes = S::kPlanes, kCell = S::kCell, kGroups = S::kGroups, kKeyRegs = S::kKeyRegs, kTiles = S::kTiles, kStep = S::kStep;
   const Kv4Where& w = p.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
@@ -85,20 +112,80 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
   if (rows < p.rows_from || rows > p.rows_to) return;
   const int part = blockIdx.x % p.parts;
   const int page_tokens = 1 << w.page_shift;
+  const int32_t* table = w.table + (size_t)s * w.pages_per_sequence;
   __shared__ float4 sum_lds[4][16][D / 4 + 1];
   __shared__ float2 ml_lds[4][16 * RT];
+  const Unpack unpack;
+  const uint32_t key_at = (n * 4 + quad) * (P / 8), value_at = (quad * 16 + n) * (2 * kCell);  // a lane's piece of a tile's codes
+  const uint32_t value_word_at = 32 * (n * kCell / (32 * GJ)) + 8 * quad;
 
   for (int row0 = (blockIdx.x / p.parts) * 16 * RT; row0 < rows; row0 += gridDim.x / p.parts * 16 * RT) {
-    // the positions that the tile's rows see: [lo, hi), in steps of 64 dealt to the parts and, one by one, to their waves
+    // the positions that the tile's rows see: [lo, hi), in steps dealt to the parts and, one by one, to their waves
     const int first_row = q.first + row0 / p.share, last_row = q.first + (min(rows, row0 + 16 * RT) - 1) / p.share;
     const int hi = p.causal ? min(q.held, last_row + 1) : q.held;
     const int lo = p.window > 0 ? max(0, first_row + 1 - p.window) : 0;
     const int step0 = lo / kStep, steps = hi > lo ? (hi - 1) / kStep + 1 - step0 : 0;
     const int each = (steps + p.parts - 1) / p.parts;
-    const int begin = step0 + min(steps, part * each), end = step0 + min(steps, (part + 1) * each);
+    const int begin = step0 + min(steps, part * each) + wave, end = step0 + min(steps, (part + 1) * each);
+
+    // The pages of a step are looked up one step ahead of its bytes, and these asked for one step ahead of their use: a wave always has a
+    // step's bytes in flight.  Pages of at least a step are one look-up and one address.  (Small pages: tiles behind the last held position
+    // read the last one again; what they hold is masked.)
+    constexpr int kIds = BIG ? 1 : kTiles;
+    struct Ids {
+      int id[kIds];
+    };
+    auto look_up = [&](int step) {
+      Ids r;
+#pragma unroll
+      for (int u = 0; u < kIds; ++u)
+        r.id[u] = table[BIG ? step * kStep >> w.page_shift : min(step * kTiles + u, (q.held - 1) >> 4) * 16 >> w.page_shift];
+      return r;
+    };
+    auto load = [&](int step, const Ids& ids, FewStep<D, GJ>& to) {
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u) {
+        const int id = ids.id[BIG ? 0 : u];
+        const bool there = id >= 0 && id < w.pages;
+        const uint8_t* block = p.cache + ((size_t)(there ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
+        const int in_page = (BIG ? step * kStep : min(step * kTiles + u, (q.held - 1) >> 4) * 16) & (page_tokens - 1);
+        const uint8_t* kc = block + in_page * (D / 2);
+        const uint8_t* vc = block + Kv4ValueCodes(page_tokens, D) + in_page * (D / 2);
+        const uint8_t* kw = block + Kv4KeyWords(page_tokens, D) + in_page * kGroups * 2;
+        const uint8_t* vw = block + Kv4ValueWords(page_tokens, D, kGroups) + in_page * kGroups * 2;
+        constexpr int kCodes = 8 * D, kWordBytes = 32 * kGroups;  // of a tile
+        const int t = BIG ? u : 0;
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl) {
+          if constexpr (P == 128) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(kc + key_at + t * kCodes + pl * 8 * P);
+            const u32x4 b = *reinterpret_cast<const u32x4*>(vc + value_at + t * kCodes + pl * 8 * P);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to.keys[u][4 * pl + e] = a[e], to.values[u][4 * pl + e] = b[e];
+          } else {
+            const u32x2 a = *reinterpret_cast<const u32x2*>(kc + key_at + t * kCodes), b = *reinterpret_cast<const u32x2*>(vc + value_at + t * kCodes);
+            to.keys[u][0] = a.x, to.keys[u][1] = a.y, to.values[u][0] = b.x, to.values[u][1] = b.y;
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) to.key_words[u][g] = *reinterpret_cast<const u32x2*>(kw + 8u * quad + t * kWordBytes + 32 * g);
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl)
+          to.value_words[u][pl] = *reinterpret_cast<const u32x2*>(vw + value_word_at + t * kWordBytes + 32 * (pl * P / (32 * GJ)));
+      }
+    };
+    FewStep<D, GJ> buffer[2];
+    Ids ids_now, ids_next;
+    if (begin < end) {
+      ids_now = look_up(begin);
+      load(begin, ids_now, buffer[0]);
+      ids_next = look_up(min(begin + 4, end - 1));
+    }
 
     u32x4 qa[RT][kKeyRegs];       // operands of the first product: channel s and channel s + 4 of 8 in each register
-    float qsum[RT][kGroups], qbase[RT][kGroups];  // sum of the row's q over a group; the same weighted by the codes' bases
+    // minus the sum of the row's q over a group; what the sums of products start from: minus the sum of q times the codes' bases, and the
+    // base of the zero points times the sum of q
+    float qsum[RT][kGroups], qbase[RT][kGroups];
     int row_lo[RT], row_hi[RT];   // what the lane's row sees
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -131,8 +218,8 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
       }
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        qsum[rt][g] = SumAcrossQuarters(qsum[rt][g]);
-        qbase[rt][g] = -SumAcrossQuarters(qbase[rt][g]);
+        qsum[rt][g] = -SumAcrossQuarters(qsum[rt][g]);
+        qbase[rt][g] = -SumAcrossQuarters(qbase[rt][g]) - kLowOffset * qsum[rt][g];
       }
     }
 
@@ -148,45 +235,7 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
         for (int j = 0; j < kCell; ++j) acc[rt][pl][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    for (int step = begin + wave; step < end; step += 4) {
-      uint32_t keys[kTiles][kKeyRegs], values[kTiles][kValueRegs];
-      u32x2 key_words[kTiles][kGroups], value_words[kTiles][kPlanes];
-      bool there[kTiles];
-      // a step inside what every row sees, on pages that there are, needs no masks
-      bool whole = step * kStep + kStep <= (p.causal ? min(q.held, first_row + 1) : q.held);
-      if (p.window > 0) whole = whole && step * kStep > last_row - p.window;
-      if (row0 + 16 * RT > rows) whole = whole && true;  // (rows that are not there have q = 0 and are not stored)
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u) {
-        // (tiles behind the last held position read the last one again: what they hold is masked)
-        const int tile = min(step * kTiles + u, (q.held - 1) >> 4);
-        const int id = w.table[(size_t)s * w.pages_per_sequence + (tile * 16 >> w.page_shift)];
-        there[u] = id >= 0 && id < w.pages;
-        whole = whole && there[u];
-        const uint8_t* block = p.cache + ((size_t)(there[u] ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
-        const int in_page = (tile * 16) & (page_tokens - 1);
-        const uint8_t* kc = block + (size_t)in_page * (D / 2) + (n * 4 + quad) * (P / 8);
-        const uint8_t* vc = block + Kv4ValueCodes(page_tokens, D) + (size_t)in_page * (D / 2) + (quad * 16 + n) * (2 * kCell);
-#pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl) {
-          if constexpr (P == 128) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(kc + pl * 8 * P), b = *reinterpret_cast<const u32x4*>(vc + pl * 8 * P);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) keys[u][4 * pl + e] = a[e], values[u][4 * pl + e] = b[e];
-          } else {
-            const u32x2 a = *reinterpret_cast<const u32x2*>(kc), b = *reinterpret_cast<const u32x2*>(vc);
-            keys[u][0] = a.x, keys[u][1] = a.y, values[u][0] = b.x, values[u][1] = b.y;
-          }
-        }
-        const uint16_t* kw = reinterpret_cast<const uint16_t*>(block + Kv4KeyWords(page_tokens, D)) + in_page * kGroups + 4 * quad;
-        const uint16_t* vw = reinterpret_cast<const uint16_t*>(block + Kv4ValueWords(page_tokens, D, kGroups)) + in_page * kGroups + 4 * quad;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) key_words[u][g] = *reinterpret_cast<const u32x2*>(kw + 16 * g);
-#pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl)
-          value_words[u][pl] = *reinterpret_cast<const u32x2*>(vw + 16 * ((pl * P + n * kCell) / (32 * GJ)));
-      }
-
+    auto attend = [&](int step, const Ids& ids, FewStep<D, GJ>& c) {
       // scores: score[rt][u][i] = q . k of row n and position 16 u + 4 quad + i
       float score[RT][kTiles][4];
 #pragma unroll
@@ -194,8 +243,8 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
         float4_t raw[RT][kGroups];
 #pragma unroll
         for (int k = 0; k < kKeyRegs; ++k) {
-          const uint32_t a = keys[u][k], b = a >> 8;
-          const u32x4 codes = {(a & kLowMask) | kLowBase, (a & kHighMask) | kHighBase, (b & kLowMask) | kLowBase, (b & kHighMask) | kHighBase};
+          const uint32_t a = c.keys[u][k], b = a >> 8;
+          const u32x4 codes = {unpack.Low(a), unpack.High(a), unpack.Low(b), unpack.High(b)};
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             const float o = qbase[rt][k / GJ];
@@ -212,31 +261,36 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
         for (int g = 0; g < kGroups; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t word = key_words[u][g][i / 2];
-            const float scale = (float)AsHalf2(word & kScaleMask)[i % 2];
-            const float zero = (float)((word >> (16 * (i % 2))) & 15u);
+            const uint32_t word = c.key_words[u][g][i / 2];
+            const float scale = (float)AsHalf2(word & unpack.scale_mask)[i % 2], zero = (float)AsHalf2(unpack.Low(word))[i % 2];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-              score[rt][u][i] = fmaf(scale, fmaf(-zero, qsum[rt][g], raw[rt][g][i]), score[rt][u][i]);
+              score[rt][u][i] = fmaf(scale, fmaf(zero, qsum[rt][g], raw[rt][g][i]), score[rt][u][i]);
           }
       }
+      // a step inside what every row sees, on pages that there are, needs no masks
+      bool whole = step * kStep + kStep <= (p.causal ? min(q.held, first_row + 1) : q.held);
+      if (p.window > 0) whole = whole && step * kStep > last_row - p.window;
+#pragma unroll
+      for (int u = 0; u < kIds; ++u) whole = whole && ids.id[u] >= 0 && ids.id[u] < w.pages;
       if (!whole) {
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) {
+          const int id = ids.id[BIG ? 0 : u];
+          const bool there = id >= 0 && id < w.pages;
           const int at = step * kStep + 16 * u + 4 * quad;
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (!there[u] || at + i >= row_hi[rt] || at + i < row_lo[rt]) score[rt][u][i] = -INFINITY;
+              if (!there || at + i >= row_hi[rt] || at + i < row_lo[rt]) score[rt][u][i] = -INFINITY;
           // what lies behind the held positions may be anything: as values it is 0 (0 * NaN would not be)
 #pragma unroll
           for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int two = at + 2 * i;
-              const uint32_t keep = !there[u] || two >= q.held ? 0u : two + 1 >= q.held ? 0x0000FFFFu : 0xFFFFFFFFu;
-              value_words[u][pl][i] &= keep;
+              c.value_words[u][pl][i] &= !there || two >= q.held ? 0u : two + 1 >= q.held ? 0x0000FFFFu : 0xFFFFFFFFu;
             }
         }
       }
@@ -252,7 +306,7 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
         best = MaxAcrossQuarters(best);
         if (__any(best > top[rt])) {
           const float now = fmaxf(top[rt], best);
-          const float down = top[rt] == now ? 1.0f : exp2f((top[rt] - now) * p.c);  // (-inf - finite: 0)
+          const float down = top[rt] == now ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - now) * p.c);  // (-inf - finite: 0)
           top[rt] = now;
           sum[rt] *= down;
 #pragma unroll
@@ -287,10 +341,10 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
           for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t word = value_words[u + v][pl][i];
-              scale[v][i] = AsHalf2(word & kScaleMask);
-              low_zero[v][i] = AsHalf2((word & kLowMask) | kLowBase);
-              high_zero[v][i] = AsHalf2(((word << 4) & kHighMask) | kHighBase);
+              const uint32_t word = c.value_words[u + v][pl][i];
+              scale[v][i] = AsHalf2(word & unpack.scale_mask);
+              low_zero[v][i] = AsHalf2(unpack.Low(word));
+              high_zero[v][i] = AsHalf2(unpack.High(word << 4));
             }
 #pragma unroll
           for (int h = 0; h < kCell / 4; ++h)
@@ -301,10 +355,9 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
               for (int v = 0; v < 2; ++v)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                  uint32_t word = values[u + v][(pl * (kCell / 4) + h) * 2 + i];
+                  uint32_t word = c.values[u + v][(pl * (kCell / 4) + h) * 2 + i];
                   if (e >= 2) word >>= 8;
-                  const half2_t x = (e & 1) ? AsHalf2((word & kHighMask) | kHighBase) - high_zero[v][i]
-                                            : AsHalf2((word & kLowMask) | kLowBase) - low_zero[v][i];
+                  const half2_t x = (e & 1) ? AsHalf2(unpack.High(word)) - high_zero[v][i] : AsHalf2(unpack.Low(word)) - low_zero[v][i];
                   op[2 * v + i] = AsU32(x * scale[v][i]);
                 }
 #pragma unroll
@@ -316,6 +369,28 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
             }
         }
       }
+    };
+
+    // (two steps a turn, so that the buffers are registers with names)
+    for (int step = begin; step < end; step += 8) {
+      Ids ids_after = ids_next;
+      if (step + 4 < end) {
+        load(step + 4, ids_next, buffer[1]);
+        ids_after = look_up(min(step + 8, end - 1));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      attend(step, ids_now, buffer[0]);
+      if (step + 4 >= end) break;
+      ids_now = ids_next;
+      ids_next = ids_after;
+      if (step + 8 < end) {
+        load(step + 8, ids_next, buffer[0]);
+        ids_after = look_up(min(step + 12, end - 1));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      attend(step + 4, ids_now, buffer[1]);
+      ids_now = ids_next;
+      ids_next = ids_after;
     }
 
     // the waves' outputs of each tile of rows, at the common maximum
@@ -333,9 +408,9 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const float2 ml = ml_lds[v][rt * 16 + n];
-        total += ml.y * (ml.x == best ? 1.0f : exp2f((ml.x - best) * p.c));
+        total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
       }
-      const float mine = top[rt] == best ? 1.0f : exp2f((top[rt] - best) * p.c);
+      const float mine = top[rt] == best ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - best) * p.c);
       const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl)
@@ -347,24 +422,24 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
                 make_float4(acc[rt][pl][4 * h][i] * factor, acc[rt][pl][4 * h + 1][i] * factor, acc[rt][pl][4 * h + 2][i] * factor,
                             acc[rt][pl][4 * h + 3][i] * factor);
       __syncthreads();
-      // 16 rows x D / 4 slices
-      for (int item = threadIdx.x; item < 16 * (D / 4); item += 256) {
-        const int r = item & 15, slice = item >> 4, row = row0 + rt * 16 + r;
-        if (row < rows) {
-          float4 v = sum_lds[0][r][slice];
+      // the rows that there are x D / 4 slices
+      const int mine_rows = min(16, rows - row0 - rt * 16);
+      for (int item = threadIdx.x; item < mine_rows * (D / 4); item += 256) {
+        const int r = p.parts > 1 ? item / (D / 4) : item % mine_rows, slice = p.parts > 1 ? item % (D / 4) : item / mine_rows;
+        const int row = row0 + rt * 16 + r;
+        float4 v = sum_lds[0][r][slice];
 #pragma unroll
-          for (int k = 1; k < 4; ++k) {
-            const float4 o = sum_lds[k][r][slice];
-            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-          }
-          const size_t token = q.start + row / p.share;
-          const int head = kv_head * p.share + row % p.share;
-          if (p.parts > 1) {
-            reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = v;
-          } else {
-            const half2_t a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
-            reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
-          }
+        for (int k = 1; k < 4; ++k) {
+          const float4 o = sum_lds[k][r][slice];
+          v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        }
+        const size_t token = q.start + row / p.share;
+        const int head = kv_head * p.share + row % p.share;
+        if (p.parts > 1) {
+          reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = v;
+        } else {
+          const half2_t a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
+          reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
         }
       }
       if (p.parts > 1 && wave == 0 && quad == 0) {
@@ -377,116 +452,456 @@ __global__ __launch_bounds__(256) void kv4_attention_few_kernel(const FewParams 
   }
 }
 
-// The parts of each row, joined: a wave per row, lanes over its slices.
+// Many rows for each key head (prompts and their chunks): matrix products bound it.  A work-group takes 128 RT rows of one key head, 32 RT to
+// a wave, and 64 positions at a time: each wave dequantizes 16 of them, exactly, into LDS, where all four read them as the operands of
+// 32x32x16 products (RT products for every operand that is read).
+//   scores^T [32 positions][32 rows] = keys x q^T      a lane has one row (lane & 31) and 16 positions: 8 (i / 4) + 4 (lane >> 5) + i % 4
+//   out^T [32 channels][32 rows]    += values^T x p^T   of 16 positions, those that the lanes hold: no exchange in between
+// In LDS: keys [head_dim / 8][position 64] pieces of 8 channels; values [16 positions][half][slot] pieces of 8 positions of one channel, the
+// positions that a lane of that half holds, the channels of a plane in the order (channel of the cell, cell): the writes of a wave and the
+// reads of a product are runs of neighbouring pieces.
+// The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.
+constexpr float kManyLift = 8.0f, kSlack = 6.0f;
+
+template <int D, int GJ, int RT>
+__global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const AttendParams p) {
+  constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16, kGroups = D / 32 / GJ;
+  constexpr int kKeyRegs = kPlanes * kWords, kValueRegs = kPlanes * kCell / 2;
+  constexpr int kStep = 64, kRows = 128 * RT, kQ = D / 16, kTilesD = D / 32;
+  const Kv4Where& w = p.w;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, quad = lane >> 4;        // of a 16-position tile, dequantizing
+  const int col = lane & 31, half = lane >> 5;      // of a product
+  const int kv_head = blockIdx.x, s = blockIdx.z, part = blockIdx.y % p.parts;
+  const Kv4Sequence q = Kv4SequenceOf(w, s);
+  const int rows = q.count * p.share;
+  if (rows < p.rows_from || rows > p.rows_to) return;
+  const int page_tokens = 1 << w.page_shift;
+  const int32_t* table = w.table + (size_t)s * w.pages_per_sequence;
+  constexpr int kPieces = kStep * D / 8;
+  __shared__ u32x4 lds[2 * 2 * kPieces];  // [2][keys, values]
+  __shared__ int there_lds[2][4];
+  const Unpack unpack;
+
+  const int row_tiles = (rows + kRows - 1) / kRows;
+  for (int turn = blockIdx.y / p.parts; turn < row_tiles; turn += gridDim.y / p.parts) {
+    const int row0 = (row_tiles - 1 - turn) * kRows;  // (the rows that see most first)
+    const int first_row = q.first + row0 / p.share, last_row = q.first + (min(rows, row0 + kRows) - 1) / p.share;
+    const int hi = p.causal ? min(q.held, last_row + 1) : q.held;
+    const int lo = p.window > 0 ? max(0, first_row + 1 - p.window) : 0;
+    const int step0 = lo / kStep, steps = hi > lo ? (hi - 1) / kStep + 1 - step0 : 0;
+    const int each = (steps + p.parts - 1) / p.parts;
+    const int begin = step0 + min(steps, part * each), end = step0 + min(steps, (part + 1) * each);
+
+    // 16 positions of each step are this wave's: their bytes one step ahead of the LDS, this one step ahead of the products
+    uint32_t keys[kKeyRegs], values[kValueRegs], key_words[kGroups];
+    u32x2 value_words[kPlanes];
+    bool there = false;
+    auto load = [&](int step) {
+      const int tile = min(step * 4 + wave, (q.held - 1) >> 4);
+      const int id = table[tile * 16 >> w.page_shift];
+      there = id >= 0 && id < w.pages;
+      const uint8_t* block = p.cache + ((size_t)(there ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
+      const int in_page = (tile * 16) & (page_tokens - 1);
+      const uint8_t* kc = block + in_page * (D / 2);
+      const uint8_t* vc = block + Kv4ValueCodes(page_tokens, D) + in_page * (D / 2);
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl) {
+        if constexpr (P == 128) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(kc + pl * 8 * P + (n * 4 + quad) * 16);
+          const u32x4 b = *reinterpret_cast<const u32x4*>(vc + pl * 8 * P + (quad * 16 + n) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) keys[4 * pl + e] = a[e], values[4 * pl + e] = b[e];
+        } else {
+          const u32x2 a = *reinterpret_cast<const u32x2*>(kc + (n * 4 + quad) * 8), b = *reinterpret_cast<const u32x2*>(vc + (quad * 16 + n) * 8);
+          keys[0] = a.x, keys[1] = a.y, values[0] = b.x, values[1] = b.y;
+        }
+      }
+      const uint16_t* kw = reinterpret_cast<const uint16_t*>(block + Kv4KeyWords(page_tokens, D)) + in_page * kGroups;
+      const uint16_t* vw = reinterpret_cast<const uint16_t*>(block + Kv4ValueWords(page_tokens, D, kGroups)) + in_page * kGroups;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) key_words[g] = kw[16 * g + n];
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl)
+        value_words[pl] = *reinterpret_cast<const u32x2*>(vw + 16 * ((pl * P + n * kCell) / (32 * GJ)) + 4 * quad);
+    };
+    auto dequantize = [&](int step, int buffer) {
+      u32x4* kb = lds + buffer * 2 * kPieces;
+      u32x4* vb = kb + kPieces;
+      if (lane == 0) there_lds[buffer][wave] = there;
+      if (step * kStep + wave * 16 + 16 > q.held || !there) {
+        // what lies behind the held positions may be anything: it is made 0 (0 * NaN would not be)
+        const int at = step * kStep + wave * 16;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          if (!there || at + n >= q.held) key_words[g] = 0;
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int two = at + 4 * quad + 2 * i;
+            value_words[pl][i] &= !there || two >= q.held ? 0u : two + 1 >= q.held ? 0x0000FFFFu : 0xFFFFFFFFu;
+          }
+      }
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const uint32_t word = key_words[g] | key_words[g] << 16;
+        const half2_t scale = AsHalf2(word & unpack.scale_mask), low_zero = AsHalf2(unpack.Low(word)), high_zero = AsHalf2(unpack.High(word << 4));
+#pragma unroll
+        for (int k = g * GJ; k < (g + 1) * GJ; ++k) {
+          const uint32_t a = keys[k], b = a >> 8;
+          const u32x4 piece = {AsU32((AsHalf2(unpack.Low(a)) - low_zero) * scale), AsU32((AsHalf2(unpack.High(a)) - high_zero) * scale),
+                               AsU32((AsHalf2(unpack.Low(b)) - low_zero) * scale), AsU32((AsHalf2(unpack.High(b)) - high_zero) * scale)};
+          kb[(4 * k + quad) * kStep + wave * 16 + n] = piece;
+        }
+      }
+      u32x2* v2 = reinterpret_cast<u32x2*>(vb + (wave * 2 + (quad & 1)) * D) + (quad >> 1);
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl) {
+        half2_t scale[2], low_zero[2], high_zero[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t word = value_words[pl][i];
+          scale[i] = AsHalf2(word & unpack.scale_mask);
+          low_zero[i] = AsHalf2(unpack.Low(word));
+          high_zero[i] = AsHalf2(unpack.High(word << 4));
+        }
+#pragma unroll
+        for (int h = 0; h < kCell / 4; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            u32x2 piece;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t word = values[(pl * (kCell / 4) + h) * 2 + i];
+              if (e >= 2) word >>= 8;
+              const half2_t x = (e & 1) ? AsHalf2(unpack.High(word)) - high_zero[i] : AsHalf2(unpack.Low(word)) - low_zero[i];
+              piece[i] = AsU32(x * scale[i]);
+            }
+            v2[2 * (pl * P + (4 * h + e) * 16 + n)] = piece;
+          }
+      }
+    };
+
+    if (begin < end) load(begin);
+
+    u32x4 qa[RT][kQ];
+    int row_lo[RT], row_hi[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = row0 + (wave * RT + rt) * 32 + col;
+      const bool is_row = row < rows;
+      const int token = (is_row ? row : 0) / p.share, head = kv_head * p.share + (is_row ? row : 0) % p.share;
+      const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + (size_t)head * (D / 4) * w.tokens + q.start + token;
+      const int position = q.first + token;
+      row_hi[rt] = is_row ? (p.causal ? min(q.held, position + 1) : q.held) : 0;
+      row_lo[rt] = p.window > 0 ? max(0, position + 1 - p.window) : 0;
+#pragma unroll
+      for (int k = 0; k < kQ; ++k) {
+        u32x2 a = {0u, 0u}, b = {0u, 0u};
+        if (is_row) {
+          a = src[(size_t)(4 * k + 2 * half) * w.tokens];
+          b = src[(size_t)(4 * k + 2 * half + 1) * w.tokens];
+        }
+        qa[rt][k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
+                          __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
+      }
+    }
+    // what all of the wave's rows see, and what any of them does
+    const int wave_row = row0 + wave * RT * 32, wave_first = q.first + min(wave_row, rows - 1) / p.share;
+    const int wave_last = q.first + min(wave_row + RT * 32 - 1, rows - 1) / p.share;
+    const int all_hi = p.causal ? min(q.held, wave_first + 1) : q.held, all_lo = p.window > 0 ? max(0, wave_last + 1 - p.window) : 0;
+    const int any_hi = wave_row >= rows ? 0 : p.causal ? min(q.held, wave_last + 1) : q.held, any_lo = p.window > 0 ? max(0, wave_first + 1 - p.window) : 0;
+
+    float16_t acc[RT][kTilesD];
+    float top[RT], sum[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      top[rt] = -INFINITY;
+      sum[rt] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kTilesD; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[rt][j][i] = 0.0f;
+    }
+
+    auto scores = [&](const u32x4* kb, int sub, float16_t* to) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[rt][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kQ; ++k) {
+        const half8_t a = __builtin_bit_cast(half8_t, kb[(2 * k + half) * kStep + sub * 32 + col]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) to[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, __builtin_bit_cast(half8_t, qa[rt][k]), to[rt], 0, 0, 0);
+      }
+    };
+    auto soften = [&](int at, bool whole, const int* tiles_there, float16_t* from, u32x4 (*prob)[2]) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float16_t& x = from[rt];
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int position = at + 8 * (i / 4) + 4 * half + i % 4;
+            if (!tiles_there[i / 8] || position >= row_hi[rt] || position < row_lo[rt]) x[i] = -INFINITY;
+          }
+        }
+        float best = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) best = fmaxf(best, x[i]);
+        const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
+        best = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        if (__any(best > top[rt] && !((best - top[rt]) * p.c <= kSlack))) {
+          const float now = fmaxf(top[rt], best);
+          const float down = top[rt] == now ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - now) * p.c);
+          top[rt] = now;
+          sum[rt] *= down;
+#pragma unroll
+          for (int j = 0; j < kTilesD; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[rt][j][i] *= down;
+        }
+        const float base = top[rt] == -INFINITY ? 0.0f : kManyLift - top[rt] * p.c;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float a = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, base)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], p.c, base));
+          sum[rt] += a + b;
+          prob[rt][i / 8][i % 8 / 2] = AsU32(half2_t{(_Float16)a, (_Float16)b});
+        }
+      }
+    };
+    auto gather = [&](const u32x4* vb, int sub, const u32x4 (*prob)[2]) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int j = 0; j < kTilesD; ++j) {
+          const half8_t v = __builtin_bit_cast(half8_t, vb[((sub * 2 + a) * 2 + half) * D + j * 32 + col]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            acc[rt][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8_t, prob[rt][a]), acc[rt][j], 0, 0, 0);
+        }
+    };
+
+    if (begin < end) {
+      dequantize(begin, 0);
+      if (begin + 1 < end) load(begin + 1);
+    }
+    __syncthreads();
+    for (int step = begin; step < end; ++step) {
+      const int buffer = (step - begin) & 1;
+      if (step + 1 < end) {
+        dequantize(step + 1, buffer ^ 1);
+        if (step + 2 < end) load(step + 2);
+      }
+      const u32x4* kb = lds + buffer * 2 * kPieces;
+      const u32x4* vb = kb + kPieces;
+      const int at = step * kStep;
+      if (at < any_hi && at + kStep > any_lo) {
+        int tiles_there[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) tiles_there[u] = __builtin_amdgcn_readfirstlane(there_lds[buffer][u]);
+        const bool whole = at >= all_lo && at + kStep <= all_hi && tiles_there[0] && tiles_there[1] && tiles_there[2] && tiles_there[3];
+        float16_t x0[RT], x1[RT];
+        u32x4 prob[RT][2];
+        scores(kb, 0, x0);
+        scores(kb, 1, x1);
+        soften(at, whole, tiles_there, x0, prob);
+        gather(vb, 0, prob);
+        soften(at + 32, whole, tiles_there + 2, x1, prob);
+        gather(vb, 1, prob);
+      }
+      __syncthreads();
+    }
+
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[rt]), __float_as_uint(sum[rt]), false, false);
+      const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+      const int row = row0 + (wave * RT + rt) * 32 + col;
+      if (row >= rows) continue;
+      const size_t token = q.start + row / p.share;
+      const int head = kv_head * p.share + row % p.share;
+      const float factor = p.parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl)
+#pragma unroll
+        for (int m = 0; m < 8; ++m)  // cells 8 (m / 4) + 4 half + m % 4
+#pragma unroll
+          for (int h = 0; h < kCell / 4; ++h) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[rt][pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
+            const int slice = (pl * P + (8 * (m / 4) + 4 * half + m % 4) * kCell) / 4 + h;
+            if (p.parts > 1) {
+              reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+              const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
+              reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
+            }
+          }
+      if (p.parts > 1 && half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top[rt], total);
+    }
+  }
+}
+
+// The parts of each row, joined: a work-group per row, its threads over the row's slices and, in turn, the parts.
 struct JoinParams {
   Kv4Where w;
   const float* part_o;
   const float2* part_ml;
   __half* out;
-  int heads, parts;
+  int heads, share;
   float c;
-  int share, rows_from, rows_to;  // of the sequences that were dealt in parts
+  int few_rows, few_parts, many_parts;  // sequences of up to few_rows rows were dealt in few_parts parts, the others in many_parts
 };
+constexpr int kMostParts = 256;
+constexpr int kFewRows = 32;  // rows of a sequence up to which the kernel for few rows serves it where there are more in a batch
 template <int D>
 __global__ __launch_bounds__(256) void kv4_attention_join_kernel(const JoinParams p) {
+  constexpr int kSlices = D / 4, kTurns = 256 / kSlices;
   const Kv4Where& w = p.w;
-  const int lane = threadIdx.x & 63;
+  const int slice = threadIdx.x % kSlices, turn = threadIdx.x / kSlices;
+  __shared__ float factors[kMostParts];
+  __shared__ float4 sums[kTurns][kSlices];
+  __shared__ float wave_best[4], wave_total[4];
   const Kv4Sequence q = Kv4SequenceOf(w, blockIdx.y);
-  if (q.count * p.share < p.rows_from || q.count * p.share > p.rows_to) return;
+  const int parts = q.count * p.share <= p.few_rows ? p.few_parts : p.many_parts;
+  if (parts == 1) return;
   const int rows = q.count * p.heads;
-  for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4) {
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const size_t token = q.start + row / p.heads;
     const int head = row % p.heads;
     const size_t at = token * p.heads + head, step = (size_t)w.tokens * p.heads;
-    float best = -INFINITY;
-    for (int k = lane; k < p.parts; k += 64) best = fmaxf(best, p.part_ml[k * step + at].x);
+    // each part's factor: a thread per part
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if ((int)threadIdx.x < parts) ml = p.part_ml[threadIdx.x * step + at];
+    float best = ml.x;
 #pragma unroll
     for (int off = 1; off < 64; off *= 2) best = fmaxf(best, __shfl_xor(best, off));
+    if ((threadIdx.x & 63) == 0) wave_best[threadIdx.x >> 6] = best;
+    __syncthreads();
+    best = fmaxf(fmaxf(wave_best[0], wave_best[1]), fmaxf(wave_best[2], wave_best[3]));
+    const float f = ml.y == 0.0f ? 0.0f : ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c);  // (0: a part that saw nothing)
+    factors[threadIdx.x] = f;
+    float total = ml.y * f;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) total += __shfl_xor(total, off);
+    if ((threadIdx.x & 63) == 0) wave_total[threadIdx.x >> 6] = total;
+    __syncthreads();
+    total = (wave_total[0] + wave_total[1]) + (wave_total[2] + wave_total[3]);
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float total = 0.0f;
-    for (int k = 0; k < p.parts; ++k) {
-      const float2 ml = p.part_ml[k * step + at];
-      if (ml.y == 0.0f) continue;  // (a part that saw nothing)
-      const float f = ml.x == best ? 1.0f : exp2f((ml.x - best) * p.c);
-      total += ml.y * f;
-      if (lane < D / 4) {
-        const float4 o = reinterpret_cast<const float4*>(p.part_o)[(k * step + at) * (D / 4) + lane];
-        v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+    for (int k = turn; k < parts; k += kTurns) {
+      const float g = factors[k];
+      if (g == 0.0f) continue;  // (nothing there, or nothing left of it)
+      const float4 o = reinterpret_cast<const float4*>(p.part_o)[(k * step + at) * kSlices + slice];
+      v.x += o.x * g, v.y += o.y * g, v.z += o.z * g, v.w += o.w * g;
+    }
+    sums[turn][slice] = v;
+    __syncthreads();
+    if (turn == 0) {
+#pragma unroll
+      for (int k = 1; k < kTurns; ++k) {
+        const float4 o = sums[k][slice];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
       }
+      const float g = total == 0.0f ? 0.0f : 1.0f / total;
+      const half2_t a = {(_Float16)(v.x * g), (_Float16)(v.y * g)}, b = {(_Float16)(v.z * g), (_Float16)(v.w * g)};
+      reinterpret_cast<u32x2*>(p.out)[((size_t)head * kSlices + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
     }
-    const float f = total == 0.0f ? 0.0f : 1.0f / total;
-    if (lane < D / 4) {
-      const half2_t a = {(_Float16)(v.x * f), (_Float16)(v.y * f)}, b = {(_Float16)(v.z * f), (_Float16)(v.w * f)};
-      reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + lane) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
-    }
+    __syncthreads();
   }
 }
 
-// How many work-groups a sequence's keys are dealt to.
-int Parts(const Kv4AttentionArgs& a) {
-  const int share = a.heads / a.where.kv_heads;
-  const long long groups = (long long)a.where.sequences * a.where.kv_heads * DivUp(std::min(a.max_new, a.max_tokens) * share, 16);
-  const long long keys = (long long)a.where.pages_per_sequence << a.where.page_shift;
-  const long long wanted = (1024 + groups - 1) / groups;
-  const long long most = (keys + 4 * kStep - 1) / (4 * kStep);
-  return (int)std::max(1LL, std::min(std::min(wanted, most), 512LL));
-}
-
 template <int D, int GJ>
-void LaunchFew(const Kv4AttentionArgs& a, hipStream_t stream) {
-  FewParams p;
+void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
+  const Kv4AttentionPlan& plan = a.plan;
+  const int share = a.heads / a.where.kv_heads, most_new = std::min(a.max_new, a.where.tokens);
+  AttendParams p;
   p.w = a.where;
   p.q = static_cast<const __half*>(a.q);
   p.cache = a.cache;
   p.out = static_cast<__half*>(a.out);
   p.heads = a.heads;
-  p.share = a.heads / a.where.kv_heads;
-  p.parts = Parts(a);
+  p.share = share;
   p.causal = a.causal;
   p.window = a.window;
   p.c = a.scale * kLog2e;
-  p.rows_from = 1;
-  p.rows_to = INT32_MAX;
   p.part_o = a.partial;
-  p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)p.parts * a.max_tokens * a.heads * D);
-  const int row_tiles = DivUp(std::min(a.max_new, a.where.tokens) * p.share, 16);
-  const dim3 grid(p.parts * row_tiles, a.where.kv_heads, a.where.sequences);
-  SetTiles(a.tiles, 16, 4, p.parts);
-  SetVariant(a.variant, "few");
-  kv4_attention_few_kernel<D, GJ, 1><<<grid, 256, 0, stream>>>(p);
-  if (p.parts > 1) {
+  p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)std::max(plan.few_parts, plan.many_parts) * a.max_tokens * a.heads * D);
+  if (plan.few_rows > 0) {
+    p.parts = plan.few_parts;
+    p.rows_from = 1;
+    p.rows_to = plan.few_rows;
+    const int row_tiles = DivUp(std::min(most_new * share, plan.few_rows), 16);
+    const dim3 grid(p.parts * row_tiles, a.where.kv_heads, a.where.sequences);
+    if (a.where.page_shift >= 5)
+      kv4_attention_few_kernel<D, GJ, 1, true><<<grid, 256, 0, stream>>>(p);
+    else
+      kv4_attention_few_kernel<D, GJ, 1, false><<<grid, 256, 0, stream>>>(p);
+  }
+  if (plan.few_rows < INT32_MAX) {
+    constexpr int kRowTiles = D == 256 ? 1 : 2;
+    p.parts = plan.many_parts;
+    p.rows_from = plan.few_rows + 1;
+    p.rows_to = INT32_MAX;
+    const dim3 grid(a.where.kv_heads, std::min(p.parts * DivUp(most_new * share, 128 * kRowTiles), 65535 / p.parts * p.parts), a.where.sequences);
+    kv4_attention_many_kernel<D, GJ, kRowTiles><<<grid, 256, 0, stream>>>(p);
+  }
+  if (plan.few_parts > 1 || plan.many_parts > 1) {
     JoinParams j;
     j.w = a.where;
     j.part_o = p.part_o;
     j.part_ml = p.part_ml;
     j.out = p.out;
     j.heads = a.heads;
-    j.parts = p.parts;
+    j.share = share;
     j.c = p.c;
-    j.share = p.share;
-    j.rows_from = p.rows_from;
-    j.rows_to = p.rows_to;
-    const dim3 join(DivUp(std::min(a.max_new, a.where.tokens) * a.heads, 4), a.where.sequences);
-    kv4_attention_join_kernel<D><<<join, 256, 0, stream>>>(j);
+    j.few_rows = plan.few_rows;
+    j.few_parts = plan.few_parts;
+    j.many_parts = plan.many_parts;
+    kv4_attention_join_kernel<D><<<dim3(most_new * a.heads, a.where.sequences), 256, 0, stream>>>(j);
   }
 }
 
 }  // namespace
 
-size_t Kv4AttentionWorkspaceFloats(const Kv4AttentionArgs& a) {
-  const int parts = Parts(a);
-  return parts > 1 ? (size_t)parts * a.max_tokens * a.heads * (a.head_dim + 2) : 0;
+Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
+  const Tuning& t = GetTuning();
+  Kv4AttentionPlan plan;
+  const int share = a.heads / a.where.kv_heads, most_new = std::min(a.max_new, a.max_tokens);
+  const long long rows = (long long)most_new * share, heads = (long long)a.where.sequences * a.where.kv_heads;
+  const long long keys = (long long)a.where.pages_per_sequence << a.where.page_shift;
+  const bool many = t.kv4_many >= 0 ? t.kv4_many > 0 : rows > kFewRows;
+  // (in a ragged batch sequences of few rows stay with the kernel for few)
+  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 ? kFewRows : 0;
+  // work-groups that are on the chip at once, and parts of at least a step for each wave
+  const long long few_groups = heads * (many ? kFewRows / 16 : (rows + 15) / 16), slots = a.head_dim == 64 ? 768 : a.head_dim == 128 ? 512 : 256;
+  const long long many_rows = a.head_dim == 256 ? 128 : 256, many_groups = heads * ((rows + many_rows - 1) / many_rows);
+  long long few = plan.few_rows > 0 ? std::min(slots / few_groups, (keys + 127) / 128) : 1;
+  long long each = many ? std::min(512 / many_groups, (keys + 511) / 512) : 1;
+  if (t.kv4_parts > 0) few = each = std::min<long long>(t.kv4_parts, (keys + 127) / 128);
+  // the parts' outputs: at most 256 MB
+  const long long room = ((long long)256 << 20) / ((long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4);
+  const auto parts = [&](long long v) { return (int)std::max(1LL, std::min(std::min(v, room), (long long)kMostParts)); };
+  plan.few_parts = plan.few_rows > 0 ? parts(few) : 1;
+  plan.many_parts = many ? parts(each) : 1;
+  return plan;
 }
 
 hipError_t LaunchKv4Attention(const Kv4AttentionArgs& a, hipStream_t stream, const char** kernel_name) {
-  *kernel_name = "kv4_attention_few_kernel";
+  const bool many = a.plan.few_rows < INT32_MAX;
+  *kernel_name = many ? "kv4_attention_many_kernel" : "kv4_attention_few_kernel";
+  SetVariant(a.variant, !many ? "few" : a.plan.few_rows > 0 ? "many, few" : "many");
+  SetTiles(a.tiles, many ? (a.head_dim == 256 ? 128 : 256) : 16, 4, many ? a.plan.many_parts : a.plan.few_parts);
   const int gj = 1 << (a.where.group_shift - 5);
   if (a.head_dim == 64)
-    gj == 1 ? LaunchFew<64, 1>(a, stream) : LaunchFew<64, 2>(a, stream);
+    gj == 1 ? Launch<64, 1>(a, stream) : Launch<64, 2>(a, stream);
   else if (a.head_dim == 128)
-    gj == 1 ? LaunchFew<128, 1>(a, stream) : gj == 2 ? LaunchFew<128, 2>(a, stream) : LaunchFew<128, 4>(a, stream);
+    gj == 1 ? Launch<128, 1>(a, stream) : gj == 2 ? Launch<128, 2>(a, stream) : Launch<128, 4>(a, stream);
   else
-    gj == 1 ? LaunchFew<256, 1>(a, stream) : gj == 2 ? LaunchFew<256, 2>(a, stream) : LaunchFew<256, 4>(a, stream);
+    gj == 1 ? Launch<256, 1>(a, stream) : gj == 2 ? Launch<256, 2>(a, stream) : Launch<256, 4>(a, stream);
   return hipGetLastError();
 }
 

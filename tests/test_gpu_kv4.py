@@ -327,6 +327,51 @@ def test_attention_row_tiles(causal, share):
     attention_case(2, share, 64, 32, 16, [1, 5, 13, 21], [200, 5, 77, 129], causal=causal, window=0 if causal else 50, seed=share)
 
 
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("share,causal,window", [(1, True, 0), (4, True, 0), (3, True, 40), (2, False, 0), (2, False, 70)])
+def test_attention_many_tokens(kv_heads, head_dim, group, page, share, causal, window):
+    d = attention_case(kv_heads, share, head_dim, group, page, [70, 1, 0, 130, 33, 16], [70, 90, 3, 200, 95, 400], causal, window, behind=2, seed=share)
+    assert d.op.kernel_name == "kv4_attention_many_kernel" and d.op.kernel_variant == "many, few"
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("many", [0, 1])
+@pytest.mark.parametrize("parts", [1, 2, 3, 7])
+def test_attention_in_parts(kv_heads, head_dim, group, page, many, parts):
+    """Both kernels with the keys in any number of parts, some of which see nothing."""
+    with M.tuning(kv4_many=many, kv4_parts=parts):
+        d = attention_case(kv_heads, 3, head_dim, group, page, [1, 40, 5, 90], [700, 333, 5, 1024], window=500 if parts == 3 else 0, seed=parts)
+        assert d.op.kernel_variant == ("many, few" if many else "few") and d.op.kernel_tiles[2] == parts
+        d = attention_case(kv_heads, 2, head_dim, group, page, [300], [900], seed=parts)
+        assert d.op.kernel_variant == ("many" if many else "few")
+
+
+def test_attention_of_more_rows_than_it_is_sized_for():
+    attention_case(1, 4, 64, 32, 16, [90, 200], [90, 230], most=1)
+    attention_case(1, 4, 64, 32, 16, [90, 700], [90, 730], most=20)
+
+
+def test_attention_of_pages_that_are_not_there():
+    """Pages in the middle that are not the cache's, for every kernel."""
+    rng = np.random.default_rng(12)
+    starts, lengths = np.array([0, 3, 80]), np.array([200, 160])
+    for page, head_dim in ((16, 128), (64, 64), (32, 256)):
+        per = -(-200 // page)
+        table = np.arange(2 * per).reshape(2, per)
+        table[0, 1], table[1, 0], table[1, 2] = -5, 10**6, 2 * per + 1
+        d = Device(2, head_dim, 32, page, 2 * per + 1, starts, lengths, table)
+        d.fill(rng)
+        d.host.spoil(table, lengths)
+        d.cache.copy_(torch.from_numpy(d.host.bytes))
+        q = rng.standard_normal((80, 4, head_dim)).astype(np.float16)
+        for many in (0, 1):
+            for window in (0, 30):
+                with M.tuning(kv4_many=many):
+                    got = d.attend(q, 4, window=window)
+                exact, largest, score = attention(q, d.host, table, lengths, starts, head_dim**-0.5, True, window, fill=5.0)
+                check_attention(got, exact, largest, score)
+
+
 def test_attention_of_nothing():
     """No positions at all, a length shorter than the new rows, pages that are not the cache's."""
     rng = np.random.default_rng(8)
@@ -343,8 +388,9 @@ def test_attention_of_nothing():
 
 def test_attention_sharp_and_far_apart_scores():
     """Scores of hundreds: one position takes all; and a long cache in which every position counts the same."""
-    attention_case(1, 8, 128, 64, 64, [1, 1], [1000, 4097], q_scale=60.0)
-    attention_case(1, 8, 128, 64, 64, [1, 1], [1000, 4097], q_scale=0.0)
+    for q_scale in (60.0, 0.0):
+        attention_case(1, 8, 128, 64, 64, [1, 1], [1000, 4097], q_scale=q_scale)
+        attention_case(1, 2, 128, 64, 64, [65, 100], [1000, 100], q_scale=q_scale)
 
 
 def test_attention_of_rows_that_are_not_finite():
@@ -358,10 +404,12 @@ def test_attention_of_rows_that_are_not_finite():
     assert np.isnan(got[1, 0]).all()
     q2 = q.copy()
     q2[1, 0] = 0
-    rest = d.attend(q2, 2)
     same = np.ones((4, 2), bool)
     same[1, 0] = False
-    assert np.array_equal(got[same], rest[same])
+    for many in (0, 1):
+        with M.tuning(kv4_many=many):
+            got, rest = d.attend(q, 2), d.attend(q2, 2)
+        assert np.isnan(got[1, 0]).all() and np.array_equal(got[same], rest[same])
 
 
 # ---- together --------------------------------------------------------------------------------------------------------------------
