@@ -452,9 +452,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
   }
 }
 
-// Many rows for each key head (prompts and their chunks): matrix products bound it.  A work-group takes 128 RT rows of one key head, 32 RT to
-// a wave, and 64 positions at a time: each wave dequantizes 16 of them, exactly, into LDS, where all four read them as the operands of
-// 32x32x16 products (RT products for every operand that is read).
+// Many rows for each key head (prompts and their chunks): matrix products bound it.  A work-group takes 32 rows of one key head to
+// a wave, 8 waves (4 where head_dim is 256), and 16 positions for each wave at a time: it dequantizes them, exactly, into LDS, where all waves
+// read all of them as operands of 32x32x16 products.
 //   scores^T [32 positions][32 rows] = keys x q^T      a lane has one row (lane & 31) and 16 positions: 8 (i / 4) + 4 (lane >> 5) + i % 4
 //   out^T [32 channels][32 rows]    += values^T x p^T   of 16 positions, those that the lanes hold: no exchange in between
 // In LDS: keys [head_dim / 8][position 64] pieces of 8 channels; values [16 positions][half][slot] pieces of 8 positions of one channel, the
@@ -462,12 +462,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
 // reads of a product are runs of neighbouring pieces.
 // The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.
 constexpr float kManyLift = 8.0f, kSlack = 6.0f;
+constexpr int ManyWaves(int head_dim) { return head_dim == 256 ? 4 : 8; }
 
-template <int D, int GJ, int RT>
-__global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const AttendParams p) {
+template <int D, int GJ>
+__global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_attention_many_kernel(const AttendParams p) {
   constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16, kGroups = D / 32 / GJ;
   constexpr int kKeyRegs = kPlanes * kWords, kValueRegs = kPlanes * kCell / 2;
-  constexpr int kStep = 64, kRows = 128 * RT, kQ = D / 16, kTilesD = D / 32;
+  constexpr int kWaves = ManyWaves(D), kStep = 16 * kWaves, kRows = 32 * kWaves, kQ = D / 16, kTilesD = D / 32;
   const Kv4Where& w = p.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;        // of a 16-position tile, dequantizing
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
   const int32_t* table = w.table + (size_t)s * w.pages_per_sequence;
   constexpr int kPieces = kStep * D / 8;
   __shared__ u32x4 lds[2 * 2 * kPieces];  // [2][keys, values]
-  __shared__ int there_lds[2][4];
+  __shared__ int there_lds[2][kWaves];
   const Unpack unpack;
 
   const int row_tiles = (rows + kRows - 1) / kRows;
@@ -493,12 +494,12 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
     const int each = (steps + p.parts - 1) / p.parts;
     const int begin = step0 + min(steps, part * each), end = step0 + min(steps, (part + 1) * each);
 
-    // 16 positions of each step are this wave's: their bytes one step ahead of the LDS, this one step ahead of the products
+    // the bytes of a step are asked for one step ahead of the LDS, this is filled one step ahead of the products
     uint32_t keys[kKeyRegs], values[kValueRegs], key_words[kGroups];
     u32x2 value_words[kPlanes];
     bool there = false;
     auto load = [&](int step) {
-      const int tile = min(step * 4 + wave, (q.held - 1) >> 4);
+      const int tile = min(step * kWaves + wave, (q.held - 1) >> 4);
       const int id = table[tile * 16 >> w.page_shift];
       there = id >= 0 && id < w.pages;
       const uint8_t* block = p.cache + ((size_t)(there ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
@@ -528,24 +529,13 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
     auto dequantize = [&](int step, int buffer) {
       u32x4* kb = lds + buffer * 2 * kPieces;
       u32x4* vb = kb + kPieces;
+      const int at = step * kStep + wave * 16;
       if (lane == 0) there_lds[buffer][wave] = there;
-      if (step * kStep + wave * 16 + 16 > q.held || !there) {
-        // what lies behind the held positions may be anything: it is made 0 (0 * NaN would not be)
-        const int at = step * kStep + wave * 16;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-          if (!there || at + n >= q.held) key_words[g] = 0;
-#pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int two = at + 4 * quad + 2 * i;
-            value_words[pl][i] &= !there || two >= q.held ? 0u : two + 1 >= q.held ? 0x0000FFFFu : 0xFFFFFFFFu;
-          }
-      }
+      // what lies behind the held positions may be anything: it is made 0 (0 * NaN would not be)
+      const int valid = there ? q.held - at : 0;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
-        const uint32_t word = key_words[g] | key_words[g] << 16;
+        const uint32_t word = n < valid ? key_words[g] | key_words[g] << 16 : 0;
         const half2_t scale = AsHalf2(word & unpack.scale_mask), low_zero = AsHalf2(unpack.Low(word)), high_zero = AsHalf2(unpack.High(word << 4));
 #pragma unroll
         for (int k = g * GJ; k < (g + 1) * GJ; ++k) {
@@ -561,7 +551,8 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
         half2_t scale[2], low_zero[2], high_zero[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t word = value_words[pl][i];
+          const int two = 4 * quad + 2 * i;
+          const uint32_t word = value_words[pl][i] & (two >= valid ? 0u : two + 1 >= valid ? 0x0000FFFFu : 0xFFFFFFFFu);
           scale[i] = AsHalf2(word & unpack.scale_mask);
           low_zero[i] = AsHalf2(unpack.Low(word));
           high_zero[i] = AsHalf2(unpack.High(word << 4));
@@ -585,103 +576,144 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
 
     if (begin < end) load(begin);
 
-    u32x4 qa[RT][kQ];
-    int row_lo[RT], row_hi[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int row = row0 + (wave * RT + rt) * 32 + col;
-      const bool is_row = row < rows;
-      const int token = (is_row ? row : 0) / p.share, head = kv_head * p.share + (is_row ? row : 0) % p.share;
-      const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + (size_t)head * (D / 4) * w.tokens + q.start + token;
-      const int position = q.first + token;
-      row_hi[rt] = is_row ? (p.causal ? min(q.held, position + 1) : q.held) : 0;
-      row_lo[rt] = p.window > 0 ? max(0, position + 1 - p.window) : 0;
+    const int wave_row = row0 + wave * 32, row = wave_row + col;
+    const bool is_row = row < rows;
+    const int token = q.start + (is_row ? row : 0) / p.share, head = kv_head * p.share + (is_row ? row : 0) % p.share;
+    const int position = q.first + (is_row ? row : 0) / p.share;
+    const int row_hi = is_row ? (p.causal ? min(q.held, position + 1) : q.held) : 0, row_lo = p.window > 0 ? max(0, position + 1 - p.window) : 0;
+    u32x4 qa[kQ];
+    {
+      // (one address of the lane and uniform strides: the lanes' own products would be hoisted out of the loops, two registers each)
+      const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + ((size_t)head * (D / 4) + 2 * half) * w.tokens + token;
 #pragma unroll
       for (int k = 0; k < kQ; ++k) {
         u32x2 a = {0u, 0u}, b = {0u, 0u};
         if (is_row) {
-          a = src[(size_t)(4 * k + 2 * half) * w.tokens];
-          b = src[(size_t)(4 * k + 2 * half + 1) * w.tokens];
+          a = src[(size_t)(4 * k) * w.tokens];
+          b = src[(size_t)(4 * k + 1) * w.tokens];
         }
-        qa[rt][k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
-                          __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
+        qa[k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
+                      __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
       }
     }
     // what all of the wave's rows see, and what any of them does
-    const int wave_row = row0 + wave * RT * 32, wave_first = q.first + min(wave_row, rows - 1) / p.share;
-    const int wave_last = q.first + min(wave_row + RT * 32 - 1, rows - 1) / p.share;
+    const int wave_first = q.first + min(wave_row, rows - 1) / p.share, wave_last = q.first + min(wave_row + 31, rows - 1) / p.share;
     const int all_hi = p.causal ? min(q.held, wave_first + 1) : q.held, all_lo = p.window > 0 ? max(0, wave_last + 1 - p.window) : 0;
     const int any_hi = wave_row >= rows ? 0 : p.causal ? min(q.held, wave_last + 1) : q.held, any_lo = p.window > 0 ? max(0, wave_first + 1 - p.window) : 0;
 
-    float16_t acc[RT][kTilesD];
-    float top[RT], sum[RT];
+    float16_t acc[kTilesD];
+    float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      top[rt] = -INFINITY;
-      sum[rt] = 0.0f;
+    for (int j = 0; j < kTilesD; ++j)
 #pragma unroll
-      for (int j = 0; j < kTilesD; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[rt][j][i] = 0.0f;
-    }
+      for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
 
-    auto scores = [&](const u32x4* kb, int sub, float16_t* to) {
+    // A step against the wave's rows, 32 positions at a time: the products of the next 32 positions' scores run under the exponentials of
+    // these, and every chunk of products has its operands asked for a chunk ahead.
+    constexpr int kAhead = 4, kSubs = kStep / 32;
+    float16_t bias;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+    for (int i = 0; i < 16; ++i) bias[i] = 0.0f;
+    // heads of 256: the outputs stay in accumulation registers, from which products are added up directly; the rare scaling down moves them
+    // out and back (the compiler by itself keeps them where that is quick, and moves all of them around every product)
+    auto settle = [&] {
+      if constexpr (D == 256) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) to[rt][i] = 0.0f;
+        for (int j = 0; j < kTilesD; ++j) asm volatile("" : "+a"(acc[j]));
 #pragma unroll
-      for (int k = 0; k < kQ; ++k) {
-        const half8_t a = __builtin_bit_cast(half8_t, kb[(2 * k + half) * kStep + sub * 32 + col]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) to[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, __builtin_bit_cast(half8_t, qa[rt][k]), to[rt], 0, 0, 0);
+        for (int k = 0; k < kQ; ++k) asm volatile("" : "+a"(qa[k]));
       }
     };
-    auto soften = [&](int at, bool whole, const int* tiles_there, float16_t* from, u32x4 (*prob)[2]) {
+    auto attend = [&](int step, int buffer, bool whole) {
+      const u32x4* kb = lds + buffer * 2 * kPieces + half * kStep + col;
+      const u32x4* vb = lds + buffer * 2 * kPieces + kPieces + half * D + col;
+      // operand number k of the scores of all the step's positions, number t of its values' products
+      auto key_piece = [&](int k) { return kb[2 * (k % kQ) * kStep + k / kQ * 32]; };
+      auto value_piece = [&](int t) { return vb[t / kTilesD * 2 * D + t % kTilesD * 32]; };
+      u32x4 kf[kAhead], vf[kAhead];
+      float16_t x[2];
+      // in steps that not every row sees whole: what the sums of products start from, 0 or -inf where the row does not see the position
+      auto start = [&](int sub) {
+        if (whole) return;
+        const int at = step * kStep + sub * 32 + 4 * half;
+        const int from = row_lo - at;
+        const int to[2] = {there_lds[buffer][sub * 2] ? row_hi - at : -1, there_lds[buffer][sub * 2 + 1] ? row_hi - at : -1};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float16_t& x = from[rt];
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int position = at + 8 * (i / 4) + 4 * half + i % 4;
-            if (!tiles_there[i / 8] || position >= row_hi[rt] || position < row_lo[rt]) x[i] = -INFINITY;
-          }
+        for (int i = 0; i < 16; ++i) {
+          const int k = 8 * (i / 4) + i % 4;
+          bias[i] = k < to[i / 8] && k >= from ? 0.0f : -INFINITY;
         }
-        float best = x[0];
+      };
+      auto key_product = [&](int sub, int k, float16_t& v) {
+        v = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, kf[k % kAhead]), __builtin_bit_cast(half8_t, qa[k]), k == 0 ? bias : v, 0, 0, 0);
+        if (sub * kQ + k + kAhead < kSubs * kQ) kf[k % kAhead] = key_piece(sub * kQ + k + kAhead);
+      };
 #pragma unroll
-        for (int i = 1; i < 16; ++i) best = fmaxf(best, x[i]);
+      for (int f = 0; f < kAhead; ++f) kf[f] = key_piece(f);
+#pragma unroll
+      for (int f = 0; f < kAhead; ++f) vf[f] = value_piece(f);
+      start(0);
+#pragma unroll
+      for (int k = 0; k < kQ; ++k) {
+        key_product(0, k, x[0]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
+        float16_t &now = x[sub & 1], &next = x[(sub & 1) ^ 1];
+        float best = now[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) best = fmaxf(best, now[i]);
         const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(best), __float_as_uint(best), false, false);
         best = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-        if (__any(best > top[rt] && !((best - top[rt]) * p.c <= kSlack))) {
-          const float now = fmaxf(top[rt], best);
-          const float down = top[rt] == now ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - now) * p.c);
-          top[rt] = now;
-          sum[rt] *= down;
+        settle();
+        if (__any(best > top && !((best - top) * p.c <= kSlack))) {
+          const float higher = fmaxf(top, best);
+          const float down = top == higher ? 1.0f : __builtin_amdgcn_exp2f((top - higher) * p.c);
+          top = higher;
+          sum *= down;
 #pragma unroll
           for (int j = 0; j < kTilesD; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[rt][j][i] *= down;
+            for (int i = 0; i < 16; ++i) acc[j][i] *= down;
         }
-        const float base = top[rt] == -INFINITY ? 0.0f : kManyLift - top[rt] * p.c;
+        settle();
+        const float base = top == -INFINITY ? 0.0f : kManyLift - top * p.c;
+        if (sub + 1 < kSubs) start(sub + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 prob[2];
+        if (sub + 1 < kSubs) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float a = __builtin_amdgcn_exp2f(fmaf(x[i], p.c, base)), b = __builtin_amdgcn_exp2f(fmaf(x[i + 1], p.c, base));
-          sum[rt] += a + b;
-          prob[rt][i / 8][i % 8 / 2] = AsU32(half2_t{(_Float16)a, (_Float16)b});
+          for (int k = 0; k < kQ; ++k) key_product(sub + 1, k, next);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = __builtin_amdgcn_exp2f(fmaf(now[2 * i], p.c, base)), v = __builtin_amdgcn_exp2f(fmaf(now[2 * i + 1], p.c, base));
+          const half2_t two = {(_Float16)u, (_Float16)v};
+          sum = __builtin_amdgcn_fdot2(two, half2_t{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+          prob[i / 4][i % 4] = AsU32(two);
+        }
+        if (sub + 1 < kSubs) {  // a product, the operand of a later one, and what of the exponentials the product hides
+#pragma unroll
+          for (int k = 0; k < kQ; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 48 / kQ, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 2 * kTilesD; ++t) {
+          acc[t % kTilesD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, vf[t % kAhead]), __builtin_bit_cast(half8_t, prob[t / kTilesD]),
+                                                                  acc[t % kTilesD], 0, 0, 0);
+          if (sub * 2 * kTilesD + t + kAhead < kSubs * 2 * kTilesD) vf[t % kAhead] = value_piece(sub * 2 * kTilesD + t + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-    };
-    auto gather = [&](const u32x4* vb, int sub, const u32x4 (*prob)[2]) {
+      if (!whole) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int j = 0; j < kTilesD; ++j) {
-          const half8_t v = __builtin_bit_cast(half8_t, vb[((sub * 2 + a) * 2 + half) * D + j * 32 + col]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            acc[rt][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8_t, prob[rt][a]), acc[rt][j], 0, 0, 0);
-        }
+        for (int i = 0; i < 16; ++i) bias[i] = 0.0f;
+      }
     };
 
     if (begin < end) {
@@ -690,40 +722,34 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
     }
     __syncthreads();
     for (int step = begin; step < end; ++step) {
-      const int buffer = (step - begin) & 1;
-      if (step + 1 < end) {
-        dequantize(step + 1, buffer ^ 1);
-        if (step + 2 < end) load(step + 2);
-      }
-      const u32x4* kb = lds + buffer * 2 * kPieces;
-      const u32x4* vb = kb + kPieces;
-      const int at = step * kStep;
+      const int buffer = (step - begin) & 1, at = step * kStep;
+      // the two waves of a SIMD fill the other buffer at different ends of the step, so that one's products meet the other's vector work
+      const auto fill = [&] {
+        if (step + 1 < end) {
+          dequantize(step + 1, buffer ^ 1);
+          if (step + 2 < end) load(step + 2);
+        }
+      };
+      settle();
+      if (kWaves == 4 || wave >= 4) fill();
       if (at < any_hi && at + kStep > any_lo) {
-        int tiles_there[4];
+        const bool whole = at >= all_lo && at + kStep <= all_hi;
+        int all_there = 1;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) tiles_there[u] = __builtin_amdgcn_readfirstlane(there_lds[buffer][u]);
-        const bool whole = at >= all_lo && at + kStep <= all_hi && tiles_there[0] && tiles_there[1] && tiles_there[2] && tiles_there[3];
-        float16_t x0[RT], x1[RT];
-        u32x4 prob[RT][2];
-        scores(kb, 0, x0);
-        scores(kb, 1, x1);
-        soften(at, whole, tiles_there, x0, prob);
-        gather(vb, 0, prob);
-        soften(at + 32, whole, tiles_there + 2, x1, prob);
-        gather(vb, 1, prob);
+        for (int u = 0; u < kWaves; ++u) all_there &= there_lds[buffer][u];
+        attend(step, buffer, whole && __builtin_amdgcn_readfirstlane(all_there));
       }
+      settle();
+      if (kWaves == 8 && wave < 4) fill();
       __syncthreads();
     }
 
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[rt]), __float_as_uint(sum[rt]), false, false);
-      const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-      const int row = row0 + (wave * RT + rt) * 32 + col;
-      if (row >= rows) continue;
-      const size_t token = q.start + row / p.share;
-      const int head = kv_head * p.share + row % p.share;
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    if (is_row) {
       const float factor = p.parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+      u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
+      float4* part_to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + half * kCell;
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
@@ -732,16 +758,16 @@ __global__ __launch_bounds__(256, 1) void kv4_attention_many_kernel(const Attend
           for (int h = 0; h < kCell / 4; ++h) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[rt][pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
-            const int slice = (pl * P + (8 * (m / 4) + 4 * half + m % 4) * kCell) / 4 + h;
+            for (int e = 0; e < 4; ++e) v[e] = acc[pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
+            const int slice = (pl * P + (8 * (m / 4) + m % 4) * kCell) / 4 + h;  // behind the half's own first
             if (p.parts > 1) {
-              reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = make_float4(v[0], v[1], v[2], v[3]);
+              part_to[slice] = make_float4(v[0], v[1], v[2], v[3]);
             } else {
               const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
-              reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
+              to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
             }
           }
-      if (p.parts > 1 && half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top[rt], total);
+      if (p.parts > 1 && half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
     }
   }
 }
@@ -842,12 +868,11 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
       kv4_attention_few_kernel<D, GJ, 1, false><<<grid, 256, 0, stream>>>(p);
   }
   if (plan.few_rows < INT32_MAX) {
-    constexpr int kRowTiles = D == 256 ? 1 : 2;
     p.parts = plan.many_parts;
     p.rows_from = plan.few_rows + 1;
     p.rows_to = INT32_MAX;
-    const dim3 grid(a.where.kv_heads, std::min(p.parts * DivUp(most_new * share, 128 * kRowTiles), 65535 / p.parts * p.parts), a.where.sequences);
-    kv4_attention_many_kernel<D, GJ, kRowTiles><<<grid, 256, 0, stream>>>(p);
+    const dim3 grid(a.where.kv_heads, std::min(p.parts * DivUp(most_new * share, 32 * ManyWaves(D)), 65535 / p.parts * p.parts), a.where.sequences);
+    kv4_attention_many_kernel<D, GJ><<<grid, 64 * ManyWaves(D), 0, stream>>>(p);
   }
   if (plan.few_parts > 1 || plan.many_parts > 1) {
     JoinParams j;
@@ -878,9 +903,9 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 ? kFewRows : 0;
   // work-groups that are on the chip at once, and parts of at least a step for each wave
   const long long few_groups = heads * (many ? kFewRows / 16 : (rows + 15) / 16), slots = a.head_dim == 64 ? 768 : a.head_dim == 128 ? 512 : 256;
-  const long long many_rows = a.head_dim == 256 ? 128 : 256, many_groups = heads * ((rows + many_rows - 1) / many_rows);
+  const long long many_rows = 32 * ManyWaves(a.head_dim), many_groups = heads * ((rows + many_rows - 1) / many_rows);
   long long few = plan.few_rows > 0 ? std::min(slots / few_groups, (keys + 127) / 128) : 1;
-  long long each = many ? std::min(512 / many_groups, (keys + 511) / 512) : 1;
+  long long each = many ? std::min(256 / many_groups, (keys + 511) / 512) : 1;
   if (t.kv4_parts > 0) few = each = std::min<long long>(t.kv4_parts, (keys + 127) / 128);
   // the parts' outputs: at most 256 MB
   const long long room = ((long long)256 << 20) / ((long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4);
@@ -894,7 +919,7 @@ hipError_t LaunchKv4Attention(const Kv4AttentionArgs& a, hipStream_t stream, con
   const bool many = a.plan.few_rows < INT32_MAX;
   *kernel_name = many ? "kv4_attention_many_kernel" : "kv4_attention_few_kernel";
   SetVariant(a.variant, !many ? "few" : a.plan.few_rows > 0 ? "many, few" : "many");
-  SetTiles(a.tiles, many ? (a.head_dim == 256 ? 128 : 256) : 16, 4, many ? a.plan.many_parts : a.plan.few_parts);
+  SetTiles(a.tiles, many ? 32 * ManyWaves(a.head_dim) : 16, many ? ManyWaves(a.head_dim) : 4, many ? a.plan.many_parts : a.plan.few_parts);
   const int gj = 1 << (a.where.group_shift - 5);
   if (a.head_dim == 64)
     gj == 1 ? Launch<64, 1>(a, stream) : Launch<64, 2>(a, stream);
