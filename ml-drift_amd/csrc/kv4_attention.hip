@@ -526,16 +526,29 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
       for (int pl = 0; pl < kPlanes; ++pl)
         value_words[pl] = *reinterpret_cast<const u32x2*>(vw + 16 * ((pl * P + n * kCell) / (32 * GJ)) + 4 * quad);
     };
-    auto dequantize = [&](int step, int buffer) {
-      u32x4* kb = lds + buffer * 2 * kPieces;
-      u32x4* vb = kb + kPieces;
-      const int at = step * kStep + wave * 16;
+    // what lies behind the held positions may be anything: it is made 0 (0 * NaN would not be)
+    auto clear = [&](int step, int buffer) {
       if (lane == 0) there_lds[buffer][wave] = there;
-      // what lies behind the held positions may be anything: it is made 0 (0 * NaN would not be)
-      const int valid = there ? q.held - at : 0;
+      const int valid = there ? q.held - (step * kStep + wave * 16) : 0;
+      if (valid < 16) {
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const uint32_t word = n < valid ? key_words[g] | key_words[g] << 16 : 0;
+        for (int g = 0; g < kGroups; ++g)
+          if (n >= valid) key_words[g] = 0;
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int two = 4 * quad + 2 * i;
+            value_words[pl][i] &= two >= valid ? 0u : two + 1 >= valid ? 0x0000FFFFu : 0xFFFFFFFFu;
+          }
+      }
+    };
+    // into LDS, a plane of channels at a time
+    auto dequantize = [&](int buffer, int pl) {
+      u32x4* kb = lds + buffer * 2 * kPieces;
+#pragma unroll
+      for (int g = pl * (P / 32 / GJ); g < (pl + 1) * (P / 32 / GJ); ++g) {
+        const uint32_t word = key_words[g] | key_words[g] << 16;
         const half2_t scale = AsHalf2(word & unpack.scale_mask), low_zero = AsHalf2(unpack.Low(word)), high_zero = AsHalf2(unpack.High(word << 4));
 #pragma unroll
         for (int k = g * GJ; k < (g + 1) * GJ; ++k) {
@@ -545,33 +558,29 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           kb[(4 * k + quad) * kStep + wave * 16 + n] = piece;
         }
       }
-      u32x2* v2 = reinterpret_cast<u32x2*>(vb + (wave * 2 + (quad & 1)) * D) + (quad >> 1);
+      u32x2* v2 = reinterpret_cast<u32x2*>(kb + kPieces + (wave * 2 + (quad & 1)) * D) + (quad >> 1);
+      half2_t scale[2], low_zero[2], high_zero[2];
 #pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl) {
-        half2_t scale[2], low_zero[2], high_zero[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int two = 4 * quad + 2 * i;
-          const uint32_t word = value_words[pl][i] & (two >= valid ? 0u : two + 1 >= valid ? 0x0000FFFFu : 0xFFFFFFFFu);
-          scale[i] = AsHalf2(word & unpack.scale_mask);
-          low_zero[i] = AsHalf2(unpack.Low(word));
-          high_zero[i] = AsHalf2(unpack.High(word << 4));
-        }
-#pragma unroll
-        for (int h = 0; h < kCell / 4; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u32x2 piece;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t word = values[(pl * (kCell / 4) + h) * 2 + i];
-              if (e >= 2) word >>= 8;
-              const half2_t x = (e & 1) ? AsHalf2(unpack.High(word)) - high_zero[i] : AsHalf2(unpack.Low(word)) - low_zero[i];
-              piece[i] = AsU32(x * scale[i]);
-            }
-            v2[2 * (pl * P + (4 * h + e) * 16 + n)] = piece;
-          }
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t word = value_words[pl][i];
+        scale[i] = AsHalf2(word & unpack.scale_mask);
+        low_zero[i] = AsHalf2(unpack.Low(word));
+        high_zero[i] = AsHalf2(unpack.High(word << 4));
       }
+#pragma unroll
+      for (int h = 0; h < kCell / 4; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u32x2 piece;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t word = values[(pl * (kCell / 4) + h) * 2 + i];
+            if (e >= 2) word >>= 8;
+            const half2_t x = (e & 1) ? AsHalf2(unpack.High(word)) - high_zero[i] : AsHalf2(unpack.Low(word)) - low_zero[i];
+            piece[i] = AsU32(x * scale[i]);
+          }
+          v2[2 * (pl * P + (4 * h + e) * 16 + n)] = piece;
+        }
     };
 
     if (begin < end) load(begin);
@@ -707,6 +716,20 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           acc[t % kTilesD] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, vf[t % kAhead]), __builtin_bit_cast(half8_t, prob[t / kTilesD]),
                                                                   acc[t % kTilesD], 0, 0, 0);
           if (sub * 2 * kTilesD + t + kAhead < kSubs * 2 * kTilesD) vf[t % kAhead] = value_piece(sub * 2 * kTilesD + t + kAhead);
+          if (D != 256) __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (D == 256) {
+          // one wave on a SIMD: its share of filling the other buffer goes under these products (behind the last step it is filled with what
+          // is at hand and not looked at)
+          static_assert(kSubs == kPlanes || D != 256);
+          dequantize(buffer ^ 1, sub);
+#pragma unroll
+          for (int t = 0; t < 2 * kTilesD; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 10, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -716,31 +739,36 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
       }
     };
 
+    const auto fill = [&](int step) {  // the buffer of a step that there is
+      clear(step, (step - begin) & 1);
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl) dequantize((step - begin) & 1, pl);
+    };
     if (begin < end) {
-      dequantize(begin, 0);
+      fill(begin);
       if (begin + 1 < end) load(begin + 1);
     }
     __syncthreads();
     for (int step = begin; step < end; ++step) {
       const int buffer = (step - begin) & 1, at = step * kStep;
-      // the two waves of a SIMD fill the other buffer at different ends of the step, so that one's products meet the other's vector work
-      const auto fill = [&] {
-        if (step + 1 < end) {
-          dequantize(step + 1, buffer ^ 1);
-          if (step + 2 < end) load(step + 2);
-        }
-      };
+      const bool more = step + 1 < end, sees = at < any_hi && at + kStep > any_lo;
       settle();
-      if (kWaves == 4 || wave >= 4) fill();
-      if (at < any_hi && at + kStep > any_lo) {
+      // eight waves: the two of a SIMD fill the other buffer at different ends of the step, so that one's products meet the other's vector work
+      if (kWaves == 8 && wave >= 4 && more) {
+        fill(step + 1);
+        if (step + 2 < end) load(step + 2);
+      }
+      if (sees) {
         const bool whole = at >= all_lo && at + kStep <= all_hi;
         int all_there = 1;
 #pragma unroll
         for (int u = 0; u < kWaves; ++u) all_there &= there_lds[buffer][u];
+        if (kWaves == 4 && more) clear(step + 1, buffer ^ 1);
         attend(step, buffer, whole && __builtin_amdgcn_readfirstlane(all_there));
       }
       settle();
-      if (kWaves == 8 && wave < 4) fill();
+      if ((kWaves == 4 ? !sees : wave < 4) && more) fill(step + 1);
+      if ((kWaves == 4 || wave < 4) && step + 2 < end) load(step + 2);
       __syncthreads();
     }
 
@@ -899,8 +927,10 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   const long long rows = (long long)most_new * share, heads = (long long)a.where.sequences * a.where.kv_heads;
   const long long keys = (long long)a.where.pages_per_sequence << a.where.page_shift;
   const bool many = t.kv4_many >= 0 ? t.kv4_many > 0 : rows > kFewRows;
-  // (in a ragged batch sequences of few rows stay with the kernel for few)
-  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 ? kFewRows : 0;
+  // In a ragged batch sequences of few rows go to the kernel for few where they could be many, or see more than the prompts' own work-groups
+  // take anyway; else a work-group of the other kernel each, beside the prompts', costs less than one more launch.
+  const long long seen = a.window > 0 ? std::min<long long>(keys, a.window) : keys;
+  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && (heads >= 64 || seen > 4096) ? kFewRows : 0;
   // work-groups that are on the chip at once, and parts of at least a step for each wave
   const long long few_groups = heads * (many ? kFewRows / 16 : (rows + 15) / 16), slots = a.head_dim == 64 ? 768 : a.head_dim == 128 ? 512 : 256;
   const long long many_rows = 32 * ManyWaves(a.head_dim), many_groups = heads * ((rows + many_rows - 1) / many_rows);

@@ -7,10 +7,11 @@
 // codes do not depend on how a division rounds.  Inputs are held to +-57344 and NaN counts as 0: a cached value is always a finite half,
 // and a masked position can never turn a product into NaN.
 //
-// A wave is 16 tokens (one tile of the cache, so that a tile's bytes are written by one wave) x 4 lanes that share a head of a token, each
-// with head_dim / 4 neighbouring channels.  Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.56.
+// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.56.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "kernels.h"
 #include "kv4.h"
@@ -76,171 +77,206 @@ __device__ __forceinline__ void Store4(uint2* p, const float v[4]) {  // (every 
 }
 __device__ __forceinline__ void Store4(float4* p, const float v[4]) { *p = make_float4(v[0], v[1], v[2], v[3]); }
 
-// Byte offsets inside a tile's codes: of the word of 8 key channels from `channel` on, of the 2 bytes of 4 value channels.
+// Byte offsets inside a tile's codes: of the 2 bytes of 4 channels from `channel` on.
 template <int D>
-__device__ __forceinline__ int KeyWordAt(int token, int channel) {
+__device__ __forceinline__ int KeyCodesAt(int token, int channel) {
   constexpr int P = Kv4Plane(D);
   const int i = channel % P;
-  return channel / P * (8 * P) + (token * 4 + i % 32 / 8) * (P / 8) + i / 32 * 4;
+  return channel / P * (8 * P) + (token * 4 + i % 32 / 8) * (P / 8) + i / 32 * 4 + i % 8 / 2;
 }
 template <int D>
-__device__ __forceinline__ int ValuePairAt(int token, int channel) {
+__device__ __forceinline__ int ValueCodesAt(int token, int channel) {
   constexpr int P = Kv4Plane(D), kCell = P / 16;
   const int i = channel % P;
   return channel / P * (8 * P) + (token / 4 * 16 + i / kCell) * (2 * kCell) + i % kCell / 4 * 8 + token % 4 * 2;
 }
 
-// What a wave works on: 16 positions of a sequence and one head of the keys or the values.
-struct Tile {
-  bool inside;     // the lane's token is one of the sequence's new rows, at a position of a page that there is
-  bool row_only;   // it is a row, but its position is on no page
-  int row;         // of the tensors
-  int in_page;     // first token of the tile in its page
-  uint8_t* block;  // the page's block of this head
-};
-__device__ __forceinline__ Tile TileOf(const Kv4Where& w, const Kv4Sequence& q, int s, int tile, int head, int token, const uint8_t* cache) {
-  Tile r;
-  const int position = tile * kKv4Tile + token;
-  const int i = position - q.first;
-  const bool is_row = i >= 0 && i < q.count;
-  r.row = q.start + i;
-  int page = -1;
-  if (tile >= 0 && tile * kKv4Tile < q.held) page = w.table[(size_t)s * w.pages_per_sequence + (tile * kKv4Tile >> w.page_shift)];
-  const bool there = page >= 0 && page < w.pages && position < q.held;
-  r.inside = is_row && there;
-  r.row_only = is_row && !there;
-  r.in_page = (tile * kKv4Tile) & ((1 << w.page_shift) - 1);
-  r.block = const_cast<uint8_t*>(cache) + ((size_t)(there ? page : 0) * w.kv_heads + head) * w.block_bytes;
-  return r;
-}
-
-// Grid: tiles of a sequence's new rows x (head, keys or values) x sequences; a work-group of 4 waves takes 4 tiles, then those
-// 4 * gridDim.x on (more rows than the op was made for only take longer).
-template <typename T, int D, bool READ>
+// Grid: runs of a sequence's new rows x (head, keys or values) x sequences.  A wave takes kRows neighbouring rows of one head, a row shared
+// by the D / CH lanes that have CH neighbouring channels each (rows run along the lanes, so that loads and stores of the tensors are runs of
+// 8 or 16 bytes times kRows).  More rows than the launch was sized for only take longer.
+template <typename T, int D, int CH, bool READ>
 __global__ __launch_bounds__(256) void kv4_move_kernel(const Kv4MoveArgs p) {
   using Raw = typename Slice<T>::type;
-  constexpr int kMine = D / 4;  // channels of a lane
+  constexpr int kRows = 64 * CH / D;
   const Kv4Where& w = p.where;
-  const int lane = threadIdx.x & 63, token = lane & 15, quarter = lane >> 4;
+  const int lane = threadIdx.x & 63;
   const bool is_value = blockIdx.y & 1;
   const int head = blockIdx.y >> 1, s = blockIdx.z;
   const Kv4Sequence q = Kv4SequenceOf(w, s);
-  if (q.count == 0) return;
   const int page_tokens = 1 << w.page_shift, groups = D >> w.group_shift, group = 1 << w.group_shift;
   const int codes_at = is_value ? Kv4ValueCodes(page_tokens, D) : 0;
   const int words_at = is_value ? Kv4ValueWords(page_tokens, D, groups) : Kv4KeyWords(page_tokens, D);
-  const int tile_begin = q.first >> 4, tile_end = (q.first + q.count + 15) >> 4;  // (first may be negative: rows without a position)
-  Raw* tensor = static_cast<Raw*>(is_value ? p.v : p.k) + (size_t)(head * D + quarter * kMine) / 4 * w.tokens;
-  for (int tile = tile_begin + (int)(blockIdx.x * 4 + (threadIdx.x >> 6)); tile < tile_end; tile += gridDim.x * 4) {
-    const Tile at = TileOf(w, q, s, tile, head, token, static_cast<const uint8_t*>(p.cache));
-    uint8_t* codes = at.block + codes_at + (size_t)at.in_page * (D / 2);
-    uint16_t* words = reinterpret_cast<uint16_t*>(at.block + words_at) + at.in_page * groups + token;  // [group][16]
+  const int channel0 = lane / kRows * CH;  // the lane's first
+  Raw* tensor = static_cast<Raw*>(is_value ? p.v : p.k) + (size_t)(head * D + channel0) / 4 * w.tokens + q.start;
+  for (int first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows; first < q.count; first += gridDim.x * 4 * kRows) {
+    const int i = first + lane % kRows, position = q.first + i;
+    const bool is_row = i < q.count;
+    int page = -1;
+    if (is_row && position >= 0 && position < q.held) page = w.table[(size_t)s * w.pages_per_sequence + (position >> w.page_shift)];
+    const bool there = page >= 0 && page < w.pages;
+    uint8_t* block = static_cast<uint8_t*>(p.cache) + ((size_t)(there ? page : 0) * w.kv_heads + head) * w.block_bytes;
+    const int token = position & 15, in_page = position & (page_tokens - 1) & ~15;
+    uint8_t* codes = block + codes_at + in_page * (D / 2);
+    uint16_t* words = reinterpret_cast<uint16_t*>(block + words_at) + in_page * groups + token;  // [group][16]
     if constexpr (READ) {
-      if (!at.inside && !at.row_only) continue;
+      if (!is_row) continue;
 #pragma unroll
-      for (int c = 0; c < kMine; c += 8) {
-        const int channel = quarter * kMine + c;
-        float v[2][4] = {};
-        if (at.inside) {
+      for (int c = 0; c < CH; c += 4) {
+        const int channel = channel0 + c;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (there) {
           const uint32_t word = words[(channel >> w.group_shift) * 16];
           const float scale = __half2float(__ushort_as_half((unsigned short)(word & 0xFFF0u)));
           const int zero = (int)(word & 15u);
-          uint32_t nibbles;
-          if (is_value) {
-            nibbles = *reinterpret_cast<const uint16_t*>(codes + ValuePairAt<D>(token, channel));
-            nibbles |= (uint32_t)*reinterpret_cast<const uint16_t*>(codes + ValuePairAt<D>(token, channel + 4)) << 16;
-          } else {
-            nibbles = *reinterpret_cast<const uint32_t*>(codes + KeyWordAt<D>(token, channel));
-          }
+          const uint32_t nibbles = *reinterpret_cast<const uint16_t*>(codes + (is_value ? ValueCodesAt<D>(token, channel) : KeyCodesAt<D>(token, channel)));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e / 4][e % 4] = scale * (float)((int)((nibbles >> (4 * e)) & 15u) - zero);
+          for (int e = 0; e < 4; ++e) v[e] = scale * (float)((int)((nibbles >> (4 * e)) & 15u) - zero);
         }
-        Store4(tensor + (size_t)(c / 4) * w.tokens + at.row, v[0]);
-        Store4(tensor + (size_t)(c / 4 + 1) * w.tokens + at.row, v[1]);
+        Store4(tensor + (size_t)(c / 4) * w.tokens + i, v);
       }
     } else {
-      // (lanes without a token take part in the reductions with zeros)
-      float x[kMine];
+      // (lanes without a place take part in the reductions with zeros)
+      float x[CH];
 #pragma unroll
-      for (int c = 0; c < kMine; c += 4) {
+      for (int c = 0; c < CH; c += 4) {
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (at.inside) Load4(tensor[(size_t)(c / 4) * w.tokens + at.row], v);
+        if (is_row) Load4(tensor[(size_t)(c / 4) * w.tokens + i], v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[c + e] = Held(v[e]);
       }
-      // lowest and highest of blocks of 16 channels, then of the groups: inside a lane, then across the lanes that share one
-      constexpr int kBlocks = kMine / 16;
-      float low[kBlocks], high[kBlocks];
+      float low = 0.0f, high = 0.0f;
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        low[b] = high[b] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          low[b] = fminf(low[b], x[16 * b + e]);
-          high[b] = fmaxf(high[b], x[16 * b + e]);
-        }
+      for (int c = 0; c < CH; ++c) {
+        low = fminf(low, x[c]);
+        high = fmaxf(high, x[c]);
       }
-#pragma unroll
-      for (int width = 2; width <= 8; width *= 2) {  // blocks of a group so far
-        if (width * 16 > group) break;
-        if (width <= kBlocks) {
-#pragma unroll
-          for (int b = 0; b < kBlocks; b += width)
-#pragma unroll
-            for (int e = 0; e < width / 2 && b + e + width / 2 < kBlocks; ++e) {
-              low[b + e] = low[b + e + width / 2] = fminf(low[b + e], low[b + e + width / 2]);
-              high[b + e] = high[b + e + width / 2] = fmaxf(high[b + e], high[b + e + width / 2]);
-            }
-        } else {
-          const int across = width / kBlocks * 8;  // 16 or 32: the lane of the neighbouring run of channels
-          low[0] = fminf(low[0], __shfl_xor(low[0], across));
-          high[0] = fmaxf(high[0], __shfl_xor(high[0], across));
-          if (kBlocks > 1) {
-#pragma unroll
-            for (int b = 1; b < kBlocks; ++b) low[b] = low[0], high[b] = high[0];
-          }
-        }
+      for (int lanes = kRows; lanes * CH < group * kRows; lanes *= 2) {  // the lanes that share the group
+        low = fminf(low, __shfl_xor(low, lanes));
+        high = fmaxf(high, __shfl_xor(high, lanes));
       }
-      if (!at.inside) continue;
+      if (!there) continue;
+      const uint32_t bits = ScaleBits((double)high - (double)low);
+      const float scale = __half2float(__ushort_as_half((unsigned short)bits));
+      const float inv = bits ? 1.0f / scale : 0.0f;
+      const float zero = bits ? RoundedQuotient(-low, scale, inv) : 0.0f;
+      if ((channel0 & (group - 1)) == 0) words[(channel0 >> w.group_shift) * 16] = (uint16_t)(bits | (uint32_t)zero);
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const int channel0 = quarter * kMine + 16 * b;
-        const uint32_t bits = ScaleBits((double)high[b] - (double)low[b]);
-        const float scale = __half2float(__ushort_as_half((unsigned short)bits));
-        const float inv = bits ? 1.0f / scale : 0.0f;
-        const float zero = bits ? RoundedQuotient(-low[b], scale, inv) : 0.0f;
-        if ((channel0 & (group - 1)) == 0) words[(channel0 >> w.group_shift) * 16] = (uint16_t)(bits | (uint32_t)zero);
+      for (int c = 0; c < CH; c += 4) {
+        uint32_t nibbles = 0;
 #pragma unroll
-        for (int c = 0; c < 16; c += 8) {
-          uint32_t nibbles = 0;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float code = bits ? RoundedQuotient(x[16 * b + c + e], scale, inv) + zero : 0.0f;
-            nibbles |= (uint32_t)fminf(fmaxf(code, 0.0f), 15.0f) << (4 * e);
-          }
-          if (is_value) {
-            *reinterpret_cast<uint16_t*>(codes + ValuePairAt<D>(token, channel0 + c)) = (uint16_t)nibbles;
-            *reinterpret_cast<uint16_t*>(codes + ValuePairAt<D>(token, channel0 + c + 4)) = (uint16_t)(nibbles >> 16);
-          } else {
-            *reinterpret_cast<uint32_t*>(codes + KeyWordAt<D>(token, channel0 + c)) = nibbles;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float code = bits ? RoundedQuotient(x[c + e], scale, inv) + zero : 0.0f;
+          nibbles |= (uint32_t)fminf(fmaxf(code, 0.0f), 15.0f) << (4 * e);
         }
+        *reinterpret_cast<uint16_t*>(codes + (is_value ? ValueCodesAt<D>(token, channel0 + c) : KeyCodesAt<D>(token, channel0 + c))) = (uint16_t)nibbles;
       }
     }
   }
 }
 
+// Reading many rows: a wave takes one tile of the cache, whose codes it reads as a lane of attention's products does, 8 or 16 bytes at a time
+// (kv4.h); tokens run along the lanes of the stores, so that these are runs of 16 tokens.
+// Grid: tiles of a sequence's rows x (head, keys or values) x sequences.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv4_read_tiles_kernel(const Kv4MoveArgs p) {
+  using Raw = typename Slice<T>::type;
+  constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16;
+  const Kv4Where& w = p.where;
+  const int lane = threadIdx.x & 63, n = lane & 15, quad = lane >> 4;
+  const bool is_value = blockIdx.y & 1;
+  const int head = blockIdx.y >> 1, s = blockIdx.z;
+  const Kv4Sequence q = Kv4SequenceOf(w, s);
+  const int page_tokens = 1 << w.page_shift, groups = D >> w.group_shift;
+  __shared__ uint32_t exchange[4][kPlanes * 64 * kWords];
+  const int tile_begin = q.first >> 4, tile_end = (q.first + q.count + 15) >> 4;  // (first may be negative: rows without a position)
+  // row i of the sequence, slice c of the head: tensor[c * tokens + i]
+  Raw* tensor = static_cast<Raw*>(is_value ? p.v : p.k) + (size_t)head * (D / 4) * w.tokens + q.start;
+  for (int tile = tile_begin + (int)(blockIdx.x * 4 + (threadIdx.x >> 6)); tile < tile_end; tile += gridDim.x * 4) {
+    int page = -1;
+    if (tile >= 0 && tile * kKv4Tile < q.held) page = w.table[(size_t)s * w.pages_per_sequence + (tile * kKv4Tile >> w.page_shift)];
+    const bool there = page >= 0 && page < w.pages;
+    const uint8_t* block = static_cast<const uint8_t*>(p.cache) + ((size_t)(there ? page : 0) * w.kv_heads + head) * w.block_bytes;
+    const int in_page = (tile * kKv4Tile) & (page_tokens - 1);
+    const uint8_t* codes = block + (is_value ? Kv4ValueCodes(page_tokens, D) : 0) + in_page * (D / 2) + (is_value ? quad * 16 + n : n * 4 + quad) * (P / 8);
+    const uint16_t* words = reinterpret_cast<const uint16_t*>(block + (is_value ? Kv4ValueWords(page_tokens, D, groups) : Kv4KeyWords(page_tokens, D))) + in_page * groups;
+    uint32_t piece[kPlanes][kWords];
+#pragma unroll
+    for (int pl = 0; pl < kPlanes; ++pl) {
+      if constexpr (P == 128) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(codes + pl * 8 * P);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) piece[pl][k] = a[k];
+      } else {
+        const u32x2 a = *reinterpret_cast<const u32x2*>(codes);
+        piece[0][0] = a.x, piece[0][1] = a.y;
+      }
+    }
+    // the lane's token, and its place among the tensors' rows
+    const int position = tile * kKv4Tile + n, row = position - q.first;
+    const bool is_row = row >= 0 && row < q.count, held = there && position < q.held;
+    if (is_value) {  // a lane has the values of four tokens: through LDS to the lanes of these
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl)
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) exchange[threadIdx.x >> 6][(pl * 64 + quad * 16 + n) * kWords + k] = piece[pl][k];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    const uint16_t* mine = reinterpret_cast<const uint16_t*>(exchange[threadIdx.x >> 6]);
+#pragma unroll
+    for (int pl = 0; pl < kPlanes; ++pl)
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) {
+        // 8 channels: of a word of the keys; of the values those of two (four) cells, 8 (4) channels each
+        const int channel = is_value ? pl * P + quad * (P / 4) + 8 * k : pl * P + 32 * k + 8 * quad;
+        uint32_t nibbles = piece[pl][k];
+        if (is_value) {
+          const int i = channel % P, j = i + 4;  // (of 4 channels each)
+          const int at = (pl * 64 + n / 4 * 16) * 2 * kWords + n % 4;
+          nibbles = mine[at + i / kCell * 2 * kWords + i % kCell / 4 * 4] | (uint32_t)mine[at + j / kCell * 2 * kWords + j % kCell / 4 * 4] << 16;
+        }
+        const uint32_t word = held ? words[(channel >> w.group_shift) * 16 + n] : 0;  // (scale 0: zeros)
+        const float scale = __half2float(__ushort_as_half((unsigned short)(word & 0xFFF0u)));
+        float v[2][4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e / 4][e % 4] = scale * (float)((int)((nibbles >> (4 * e)) & 15u) - (int)(word & 15u));
+        if (is_row) {
+          Store4(tensor + (size_t)(channel / 4) * w.tokens + row, v[0]);
+          Store4(tensor + (size_t)(channel / 4 + 1) * w.tokens + row, v[1]);
+        }
+      }
+    __builtin_amdgcn_wave_barrier();  // (the exchange is written again)
+  }
+}
+
+template <typename T, int D, int CH, bool READ>
+void LaunchForm(const Kv4MoveArgs& p, hipStream_t stream) {
+  const dim3 grid(DivUp(std::min(p.max_new, p.where.tokens), 4 * (64 * CH / D)), 2 * p.where.kv_heads, p.where.sequences);
+  kv4_move_kernel<T, D, CH, READ><<<grid, 256, 0, stream>>>(p);
+}
+template <typename T, int D, bool READ>
+void LaunchHead(const Kv4MoveArgs& p, hipStream_t stream) {
+  // few rows: a lane has one slice, so that a row is spread over as many lanes as it can; else 16 channels (reading: a tile for each wave)
+  if (p.max_new <= 8) {
+    LaunchForm<T, D, 4, READ>(p, stream);
+  } else if constexpr (READ) {
+    const int tiles = DivUp(std::min(p.max_new, p.where.tokens), kKv4Tile) + 1;
+    kv4_read_tiles_kernel<T, D><<<dim3(DivUp(tiles, 4), 2 * p.where.kv_heads, p.where.sequences), 256, 0, stream>>>(p);
+  } else {
+    LaunchForm<T, D, 16, false>(p, stream);
+  }
+}
 template <typename T, bool READ>
 void LaunchTyped(const Kv4MoveArgs& p, hipStream_t stream) {
-  // tiles that max_new rows can touch, 4 to a work-group
-  const int tiles = DivUp(p.max_new, kKv4Tile) + 1;
-  const dim3 grid(DivUp(tiles, 4), 2 * p.where.kv_heads, p.where.sequences);
   if (p.head_dim == 64)
-    kv4_move_kernel<T, 64, READ><<<grid, 256, 0, stream>>>(p);
+    LaunchHead<T, 64, READ>(p, stream);
   else if (p.head_dim == 128)
-    kv4_move_kernel<T, 128, READ><<<grid, 256, 0, stream>>>(p);
+    LaunchHead<T, 128, READ>(p, stream);
   else
-    kv4_move_kernel<T, 256, READ><<<grid, 256, 0, stream>>>(p);
+    LaunchHead<T, 256, READ>(p, stream);
 }
 
 }  // namespace

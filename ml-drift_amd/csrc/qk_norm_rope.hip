@@ -182,7 +182,9 @@ void LaunchTyped(NormRopeArgs p, hipStream_t stream) {
     Launch<T, 16, 2>(p, dim3(DivUp(p.tokens, 16), heads), stream);
     return;
   }
-  if (p.tokens >= 512) p.heads_per_group = 4;
+  // heads that share sines and cosines: as many as leave two waves for every SIMD
+  const long long waves = (long long)DivUp(p.tokens, 16) * heads;
+  p.heads_per_group = waves >= 4 * 2048 ? 4 : waves >= 2 * 2048 ? 2 : 1;
   const dim3 grid(DivUp(p.tokens, 64), DivUp(heads, p.heads_per_group));
   if (p.head_dim <= 64)
     Launch<T, 4, 2>(p, grid, stream);

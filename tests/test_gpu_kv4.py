@@ -331,6 +331,15 @@ def test_attention_row_tiles(causal, share):
 @pytest.mark.parametrize("share,causal,window", [(1, True, 0), (4, True, 0), (3, True, 40), (2, False, 0), (2, False, 70)])
 def test_attention_many_tokens(kv_heads, head_dim, group, page, share, causal, window):
     d = attention_case(kv_heads, share, head_dim, group, page, [70, 1, 0, 130, 33, 16], [70, 90, 3, 200, 95, 400], causal, window, behind=2, seed=share)
+    assert d.op.kernel_name == "kv4_attention_many_kernel" and d.op.kernel_variant == "many"
+
+
+@pytest.mark.parametrize("head_dim,group", [(64, 32), (128, 64), (256, 128)])
+@pytest.mark.parametrize("parts", [-1, 3])
+def test_attention_of_prompts_and_single_tokens_together(head_dim, group, parts):
+    counts, lengths = [1, 70, 16, 0, 2, 33, 1, 20, 1, 1], [90, 90, 16, 3, 333, 200, 1, 400, 64, 77]
+    with M.tuning(kv4_parts=parts):
+        d = attention_case(8, 2, head_dim, group, 32, counts, lengths, behind=1)
     assert d.op.kernel_name == "kv4_attention_many_kernel" and d.op.kernel_variant == "many, few"
 
 
@@ -341,7 +350,7 @@ def test_attention_in_parts(kv_heads, head_dim, group, page, many, parts):
     """Both kernels with the keys in any number of parts, some of which see nothing."""
     with M.tuning(kv4_many=many, kv4_parts=parts):
         d = attention_case(kv_heads, 3, head_dim, group, page, [1, 40, 5, 90], [700, 333, 5, 1024], window=500 if parts == 3 else 0, seed=parts)
-        assert d.op.kernel_variant == ("many, few" if many else "few") and d.op.kernel_tiles[2] == parts
+        assert d.op.kernel_variant == ("many" if many else "few") and d.op.kernel_tiles[2] == parts
         d = attention_case(kv_heads, 2, head_dim, group, page, [300], [900], seed=parts)
         assert d.op.kernel_variant == ("many" if many else "few")
 
@@ -349,6 +358,7 @@ def test_attention_in_parts(kv_heads, head_dim, group, page, many, parts):
 def test_attention_of_more_rows_than_it_is_sized_for():
     attention_case(1, 4, 64, 32, 16, [90, 200], [90, 230], most=1)
     attention_case(1, 4, 64, 32, 16, [90, 700], [90, 730], most=20)
+    attention_case(64, 1, 64, 32, 16, [90, 1, 300], [90, 9, 330], most=33)
 
 
 def test_attention_of_pages_that_are_not_there():
