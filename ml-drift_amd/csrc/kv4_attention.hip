@@ -44,7 +44,7 @@ struct AttendParams {
   __half* out;
   float* part_o;   // [parts][rows of the tensors][D]
   float2* part_ml; // [parts][rows]: maximum (of q . k) and sum
-  int heads, share, parts, causal, window;
+  int heads, share, parts, joined, causal, window;  // parts: of this kernel; joined: of the launch, 1 where outputs are written directly
   float c;  // scale * log2(e)
   int rows_from, rows_to;  // sequences of rows_from .. rows_to rows are this kernel's
 };
@@ -89,6 +89,9 @@ struct FewShape {
   static constexpr int kValueRegs = kPlanes * kCell / 2;  // and of its values (4 channels of 2 positions each)
   static constexpr int kStep = 32;                        // positions that a wave takes at a time: two steps are in registers
   static constexpr int kTiles = kStep / 16;
+  // The words of the keys belong to positions, which all 16 lanes of a quarter share: lane n loads those of tile n / kGroups, group n %
+  // kGroups, and they are broadcast from there.
+  static_assert(kTiles * kGroups <= 16);
 };
 
 // The cached bytes of one step, as a lane holds them.
@@ -96,36 +99,67 @@ template <int D, int GJ>
 struct FewStep {
   using S = FewShape<D, GJ>;
   uint32_t keys[S::kTiles][S::kKeyRegs], values[S::kTiles][S::kValueRegs];
-  u32x2 key_words[S::kTiles][S::kGroups], value_words[S::kTiles][S::kPlanes];
+  u32x2 key_words, value_words[S::kTiles][S::kPlanes];
 };
 
+// Lane `from` of each row of 16 lanes, in all of the row.
+template <int FROM>
+__device__ __forceinline__ uint32_t OfRow(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x150 + FROM /* row_newbcast */, 0xf, 0xf, true);
+}
+__device__ __forceinline__ uint32_t OfRow(uint32_t v, int from) {  // (`from` is a constant where it is inlined)
+  switch (from) {
+    case 0: return OfRow<0>(v);
+    case 1: return OfRow<1>(v);
+    case 2: return OfRow<2>(v);
+    case 3: return OfRow<3>(v);
+    case 4: return OfRow<4>(v);
+    case 5: return OfRow<5>(v);
+    case 6: return OfRow<6>(v);
+    case 7: return OfRow<7>(v);
+    case 8: return OfRow<8>(v);
+    case 9: return OfRow<9>(v);
+    case 10: return OfRow<10>(v);
+    case 11: return OfRow<11>(v);
+    case 12: return OfRow<12>(v);
+    case 13: return OfRow<13>(v);
+    case 14: return OfRow<14>(v);
+    default: return OfRow<15>(v);
+  }
+}
+
 template <int D, int GJ, int RT, bool BIG>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kernel(const AttendParams p) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_attention_few_kernel(const AttendParams p) {
   using S = FewShape<D, GJ>;
   constexpr int P = S::P, kPlanes = S::kPlanes, kCell = S::kCell, kGroups = S::kGroups, kKeyRegs = S::kKeyRegs, kTiles = S::kTiles, kStep = S::kStep;
   const Kv4Where& w = p.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
   const int kv_head = blockIdx.y, s = blockIdx.z;
+  const bool one_tile = (int)gridDim.x == p.parts;
+  const int part = one_tile ? blockIdx.x : blockIdx.x % p.parts, tile0 = one_tile ? 0 : blockIdx.x / p.parts, tile_step = one_tile ? 1 : gridDim.x / p.parts;
+  const int page_tokens = 1 << w.page_shift;
+  const int32_t* table = w.table + (size_t)s * w.pages_per_sequence;
+  // the first 64 pages, asked for with the lengths rather than after them
+  const int first_pages = lane < w.pages_per_sequence ? table[lane] : -1;
   const Kv4Sequence q = Kv4SequenceOf(w, s);
   const int rows = q.count * p.share;
   if (rows < p.rows_from || rows > p.rows_to) return;
-  const int part = blockIdx.x % p.parts;
-  const int page_tokens = 1 << w.page_shift;
-  const int32_t* table = w.table + (size_t)s * w.pages_per_sequence;
   __shared__ float4 sum_lds[4][16][D / 4 + 1];
   __shared__ float2 ml_lds[4][16 * RT];
   const Unpack unpack;
   const uint32_t key_at = (n * 4 + quad) * (P / 8), value_at = (quad * 16 + n) * (2 * kCell);  // a lane's piece of a tile's codes
   const uint32_t value_word_at = 32 * (n * kCell / (32 * GJ)) + 8 * quad;
 
-  for (int row0 = (blockIdx.x / p.parts) * 16 * RT; row0 < rows; row0 += gridDim.x / p.parts * 16 * RT) {
+  // (a sequence with one new token, the common case, divides nothing)
+  auto token_of = [&](int row) { return q.count == 1 ? 0 : row / p.share; };
+  for (int row0 = tile0 * 16 * RT; row0 < rows; row0 += tile_step * 16 * RT) {
     // the positions that the tile's rows see: [lo, hi), in steps dealt to the parts and, one by one, to their waves
-    const int first_row = q.first + row0 / p.share, last_row = q.first + (min(rows, row0 + 16 * RT) - 1) / p.share;
+    const int first_row = q.first + token_of(row0), last_row = q.first + token_of(min(rows, row0 + 16 * RT) - 1);
     const int hi = p.causal ? min(q.held, last_row + 1) : q.held;
     const int lo = p.window > 0 ? max(0, first_row + 1 - p.window) : 0;
     const int step0 = lo / kStep, steps = hi > lo ? (hi - 1) / kStep + 1 - step0 : 0;
-    const int each = (steps + p.parts - 1) / p.parts;
+    const int each = p.parts == 1 ? steps : (steps + p.parts - 1) / p.parts;
     const int begin = step0 + min(steps, part * each) + wave, end = step0 + min(steps, (part + 1) * each);
 
     // The pages of a step are looked up one step ahead of its bytes, and these asked for one step ahead of their use: a wave always has a
@@ -138,47 +172,69 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
     auto look_up = [&](int step) {
       Ids r;
 #pragma unroll
-      for (int u = 0; u < kIds; ++u)
-        r.id[u] = table[BIG ? step * kStep >> w.page_shift : min(step * kTiles + u, (q.held - 1) >> 4) * 16 >> w.page_shift];
+      for (int u = 0; u < kIds; ++u) {
+        const int page = BIG ? step * kStep >> w.page_shift : min(step * kTiles + u, (q.held - 1) >> 4) * 16 >> w.page_shift;
+        r.id[u] = page < 64 ? __builtin_amdgcn_readlane(first_pages, page) : table[page];
+      }
       return r;
     };
-    auto load = [&](int step, const Ids& ids, FewStep<D, GJ>& to) {
+    auto block_of = [&](int step, const Ids& ids, int u) {
+      const int id = ids.id[BIG ? 0 : u];
+      return p.cache + ((size_t)(id >= 0 && id < w.pages ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
+    };
+    auto in_page_of = [&](int step, int u) { return (BIG ? step * kStep : min(step * kTiles + u, (q.held - 1) >> 4) * 16) & (page_tokens - 1); };
+    constexpr int kCodes = 8 * D, kWordBytes = 32 * kGroups;  // of a tile
+    auto load_keys = [&](int step, const Ids& ids, FewStep<D, GJ>& to) {
 #pragma unroll
       for (int u = 0; u < kTiles; ++u) {
-        const int id = ids.id[BIG ? 0 : u];
-        const bool there = id >= 0 && id < w.pages;
-        const uint8_t* block = p.cache + ((size_t)(there ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
-        const int in_page = (BIG ? step * kStep : min(step * kTiles + u, (q.held - 1) >> 4) * 16) & (page_tokens - 1);
+        const uint8_t* block = block_of(step, ids, u);
+        const int in_page = in_page_of(step, u), t = BIG ? u : 0;
         const uint8_t* kc = block + in_page * (D / 2);
-        const uint8_t* vc = block + Kv4ValueCodes(page_tokens, D) + in_page * (D / 2);
         const uint8_t* kw = block + Kv4KeyWords(page_tokens, D) + in_page * kGroups * 2;
-        const uint8_t* vw = block + Kv4ValueWords(page_tokens, D, kGroups) + in_page * kGroups * 2;
-        constexpr int kCodes = 8 * D, kWordBytes = 32 * kGroups;  // of a tile
-        const int t = BIG ? u : 0;
 #pragma unroll
         for (int pl = 0; pl < kPlanes; ++pl) {
           if constexpr (P == 128) {
             const u32x4 a = *reinterpret_cast<const u32x4*>(kc + key_at + t * kCodes + pl * 8 * P);
-            const u32x4 b = *reinterpret_cast<const u32x4*>(vc + value_at + t * kCodes + pl * 8 * P);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to.keys[u][4 * pl + e] = a[e], to.values[u][4 * pl + e] = b[e];
+            for (int e = 0; e < 4; ++e) to.keys[u][4 * pl + e] = a[e];
           } else {
-            const u32x2 a = *reinterpret_cast<const u32x2*>(kc + key_at + t * kCodes), b = *reinterpret_cast<const u32x2*>(vc + value_at + t * kCodes);
-            to.keys[u][0] = a.x, to.keys[u][1] = a.y, to.values[u][0] = b.x, to.values[u][1] = b.y;
+            const u32x2 a = *reinterpret_cast<const u32x2*>(kc + key_at + t * kCodes);
+            to.keys[u][0] = a.x, to.keys[u][1] = a.y;
           }
         }
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) to.key_words[u][g] = *reinterpret_cast<const u32x2*>(kw + 8u * quad + t * kWordBytes + 32 * g);
-#pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl)
-          to.value_words[u][pl] = *reinterpret_cast<const u32x2*>(vw + value_word_at + t * kWordBytes + 32 * (pl * P / (32 * GJ)));
+        if (BIG ? u == 0 : true) {
+          const int mine = min(n / kGroups, kTiles - 1);  // (lanes behind the words read the last tile's)
+          if (BIG || mine == u) to.key_words = *reinterpret_cast<const u32x2*>(kw + 8u * quad + (BIG ? mine * kWordBytes : 0) + 32 * (n % kGroups));
+        }
       }
     };
-    FewStep<D, GJ> buffer[2];
-    Ids ids_now, ids_next;
+    auto load_values = [&](int step, const Ids& ids, FewStep<D, GJ>& to) {
+#pragma unroll
+      for (int u = 0; u < kTiles; ++u) {
+        const uint8_t* block = block_of(step, ids, u);
+        const int in_page = in_page_of(step, u), t = BIG ? u : 0;
+        const uint8_t* vc = block + Kv4ValueCodes(page_tokens, D) + in_page * (D / 2);
+        const uint8_t* vw = block + Kv4ValueWords(page_tokens, D, kGroups) + in_page * kGroups * 2;
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl) {
+          if constexpr (P == 128) {
+            const u32x4 b = *reinterpret_cast<const u32x4*>(vc + value_at + t * kCodes + pl * 8 * P);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to.values[u][4 * pl + e] = b[e];
+          } else {
+            const u32x2 b = *reinterpret_cast<const u32x2*>(vc + value_at + t * kCodes);
+            to.values[u][0] = b.x, to.values[u][1] = b.y;
+          }
+          to.value_words[u][pl] = *reinterpret_cast<const u32x2*>(vw + value_word_at + t * kWordBytes + 32 * (pl * P / (32 * GJ)));
+        }
+      }
+    };
+    FewStep<D, GJ> c;
+    Ids ids, ids_next;
     if (begin < end) {
-      ids_now = look_up(begin);
-      load(begin, ids_now, buffer[0]);
+      ids = look_up(begin);
+      load_keys(begin, ids, c);
+      load_values(begin, ids, c);
       ids_next = look_up(min(begin + 4, end - 1));
     }
 
@@ -191,8 +247,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
     for (int rt = 0; rt < RT; ++rt) {
       const int row = row0 + rt * 16 + n;
       const bool there = row < rows;
-      const int token = (there ? row : 0) / p.share, head = kv_head * p.share + (there ? row : 0) % p.share;
-      const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + (size_t)head * (D / 4) * w.tokens + q.start + token;
+      const int token = token_of(there ? row : 0), head = kv_head * p.share + (there ? row : 0) - token * p.share;
+      // (one address of the lane and uniform strides: the lanes' own products would be hoisted out of the loop, two registers each)
+      const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + ((size_t)head * (D / 4) + 2 * quad) * w.tokens + q.start + token;
       const int position = q.first + token;
       row_hi[rt] = there ? (p.causal ? min(q.held, position + 1) : q.held) : 0;
       row_lo[rt] = p.window > 0 ? max(0, position + 1 - p.window) : 0;
@@ -202,8 +259,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
       for (int k = 0; k < kKeyRegs; ++k) {
         u32x2 a = {0u, 0u}, b = {0u, 0u};
         if (there) {
-          a = src[(size_t)(8 * k + 2 * quad) * w.tokens];
-          b = src[(size_t)(8 * k + 2 * quad + 1) * w.tokens];
+          a = src[(size_t)(8 * k) * w.tokens];
+          b = src[(size_t)(8 * k + 1) * w.tokens];
         }
         qa[rt][k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
                           __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
@@ -235,9 +292,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
         for (int j = 0; j < kCell; ++j) acc[rt][pl][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    auto attend = [&](int step, const Ids& ids, FewStep<D, GJ>& c) {
+    for (int step = begin; step < end; step += 4) {
       // scores: score[rt][u][i] = q . k of row n and position 16 u + 4 quad + i
       float score[RT][kTiles][4];
+      if constexpr (kGroups == 8) {  // (what the sums start from, four times each, would stay in 32 registers over the loop)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) asm volatile("" : "+v"(qbase[0][g]));
+      }
 #pragma unroll
       for (int u = 0; u < kTiles; ++u) {
         float4_t raw[RT][kGroups];
@@ -261,13 +322,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
         for (int g = 0; g < kGroups; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t word = c.key_words[u][g][i / 2];
+            const uint32_t word = OfRow(c.key_words[i / 2], u * kGroups + g);
             const float scale = (float)AsHalf2(word & unpack.scale_mask)[i % 2], zero = (float)AsHalf2(unpack.Low(word))[i % 2];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
               score[rt][u][i] = fmaf(scale, fmaf(zero, qsum[rt][g], raw[rt][g][i]), score[rt][u][i]);
           }
+        // (a tile's products and sums at a time: left alone, the compiler puts all the step's products first and needs registers for them)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(score[rt][u][i]));
       }
+      // (the next step's keys come while this one's values are taken, and the other way round)
+      if (step + 4 < end) load_keys(step + 4, ids_next, c);
+      __builtin_amdgcn_sched_barrier(0);
       // a step inside what every row sees, on pages that there are, needs no masks
       bool whole = step * kStep + kStep <= (p.causal ? min(q.held, first_row + 1) : q.held);
       if (p.window > 0) whole = whole && step * kStep > last_row - p.window;
@@ -369,28 +438,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
             }
         }
       }
-    };
-
-    // (two steps a turn, so that the buffers are registers with names)
-    for (int step = begin; step < end; step += 8) {
-      Ids ids_after = ids_next;
-      if (step + 4 < end) {
-        load(step + 4, ids_next, buffer[1]);
-        ids_after = look_up(min(step + 8, end - 1));
-      }
+      if (step + 4 < end) load_values(step + 4, ids_next, c);
+      ids = ids_next;
+      ids_next = look_up(min(step + 8, end - 1));
       __builtin_amdgcn_sched_barrier(0);
-      attend(step, ids_now, buffer[0]);
-      if (step + 4 >= end) break;
-      ids_now = ids_next;
-      ids_next = ids_after;
-      if (step + 8 < end) {
-        load(step + 8, ids_next, buffer[0]);
-        ids_after = look_up(min(step + 12, end - 1));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      attend(step + 4, ids_now, buffer[1]);
-      ids_now = ids_next;
-      ids_next = ids_after;
     }
 
     // the waves' outputs of each tile of rows, at the common maximum
@@ -411,21 +462,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
         total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
       }
       const float mine = top[rt] == best ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - best) * p.c);
-      const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
+      const float factor = mine * (p.joined > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
+      if (row0 + rt * 16 + n < rows)
 #pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl)
+        for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int h = 0; h < kCell / 4; ++h)
-            sum_lds[wave][n][(pl * P + (4 * quad + i) * kCell) / 4 + h] =
+            for (int h = 0; h < kCell / 4; ++h)
+              sum_lds[wave][n][(pl * P + (4 * quad + i) * kCell) / 4 + h] =
                 make_float4(acc[rt][pl][4 * h][i] * factor, acc[rt][pl][4 * h + 1][i] * factor, acc[rt][pl][4 * h + 2][i] * factor,
                             acc[rt][pl][4 * h + 3][i] * factor);
       __syncthreads();
       // the rows that there are x D / 4 slices
       const int mine_rows = min(16, rows - row0 - rt * 16);
       for (int item = threadIdx.x; item < mine_rows * (D / 4); item += 256) {
-        const int r = p.parts > 1 ? item / (D / 4) : item % mine_rows, slice = p.parts > 1 ? item % (D / 4) : item / mine_rows;
+        const int r = item / (D / 4), slice = item % (D / 4);
         const int row = row0 + rt * 16 + r;
         float4 v = sum_lds[0][r][slice];
 #pragma unroll
@@ -433,19 +485,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_attention_few_kerne
           const float4 o = sum_lds[k][r][slice];
           v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
         }
-        const size_t token = q.start + row / p.share;
-        const int head = kv_head * p.share + row % p.share;
-        if (p.parts > 1) {
+        const int of_sequence = token_of(row), head = kv_head * p.share + row - of_sequence * p.share;
+        const size_t token = q.start + of_sequence;
+        if (p.joined > 1) {
           reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = v;
         } else {
           const half2_t a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
           reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
         }
       }
-      if (p.parts > 1 && wave == 0 && quad == 0) {
+      if (p.joined > 1 && wave == 0 && quad == 0) {
         const int row = row0 + rt * 16 + n;
-        if (row < rows)
-          p.part_ml[((size_t)part * w.tokens + q.start + row / p.share) * p.heads + kv_head * p.share + row % p.share] = make_float2(best, total);
+        if (row < rows) {
+          float2* to = p.part_ml + (size_t)(q.start + token_of(row)) * p.heads + kv_head * p.share + row - token_of(row) * p.share;
+          to[(size_t)part * w.tokens * p.heads] = make_float2(best, total);
+          if (part == 0)
+            for (int k = p.parts; k < p.joined; ++k) to[(size_t)k * w.tokens * p.heads] = make_float2(-INFINITY, 0.0f);
+        }
       }
       __syncthreads();  // (the arrays are written again)
     }
@@ -592,7 +648,6 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     const int row_hi = is_row ? (p.causal ? min(q.held, position + 1) : q.held) : 0, row_lo = p.window > 0 ? max(0, position + 1 - p.window) : 0;
     u32x4 qa[kQ];
     {
-      // (one address of the lane and uniform strides: the lanes' own products would be hoisted out of the loops, two registers each)
       const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + ((size_t)head * (D / 4) + 2 * half) * w.tokens + token;
 #pragma unroll
       for (int k = 0; k < kQ; ++k) {
@@ -775,7 +830,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     if (is_row) {
-      const float factor = p.parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+      const float factor = p.joined > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
       u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
       float4* part_to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + half * kCell;
 #pragma unroll
@@ -788,83 +843,110 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = acc[pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
             const int slice = (pl * P + (8 * (m / 4) + m % 4) * kCell) / 4 + h;  // behind the half's own first
-            if (p.parts > 1) {
+            if (p.joined > 1) {
               part_to[slice] = make_float4(v[0], v[1], v[2], v[3]);
             } else {
               const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
               to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
             }
           }
-      if (p.parts > 1 && half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
+      if (p.joined > 1 && half == 0) {
+        float2* ml = p.part_ml + (size_t)token * p.heads + head;
+        ml[(size_t)part * w.tokens * p.heads] = make_float2(top, total);
+        if (part == 0)
+          for (int k = p.parts; k < p.joined; ++k) ml[(size_t)k * w.tokens * p.heads] = make_float2(-INFINITY, 0.0f);
+      }
     }
   }
 }
 
-// The parts of each row, joined: a work-group per row, its threads over the row's slices and, in turn, the parts.
+// The parts of each row, joined.  A row per work-group of WAVES waves, whose threads share its slices and, in turn, its parts: four waves
+// where parts are many, one where they are few.  Everything is asked for before the first wait (the loads of the parts' outputs do not depend
+// on their sums), and nothing is looked up but where the first sequence begins and the last one ends.
 struct JoinParams {
   Kv4Where w;
   const float* part_o;
   const float2* part_ml;
   __half* out;
-  int heads, share;
+  int heads, parts;
   float c;
-  int few_rows, few_parts, many_parts;  // sequences of up to few_rows rows were dealt in few_parts parts, the others in many_parts
 };
-constexpr int kMostParts = 256;
+constexpr int kMostParts = 256, kFewParts = 8;
 constexpr int kFewRows = 32;  // rows of a sequence up to which the kernel for few rows serves it where there are more in a batch
-template <int D>
+template <int D, int WAVES>
 __global__ __launch_bounds__(256) void kv4_attention_join_kernel(const JoinParams p) {
-  constexpr int kSlices = D / 4, kTurns = 256 / kSlices;
+  constexpr int kSlices = D / 4, kTurns = 64 * WAVES / kSlices, kFirst = 4;
   const Kv4Where& w = p.w;
-  const int slice = threadIdx.x % kSlices, turn = threadIdx.x / kSlices;
-  __shared__ float factors[kMostParts];
-  __shared__ float4 sums[kTurns][kSlices];
-  __shared__ float wave_best[4], wave_total[4];
-  const Kv4Sequence q = Kv4SequenceOf(w, blockIdx.y);
-  const int parts = q.count * p.share <= p.few_rows ? p.few_parts : p.many_parts;
-  if (parts == 1) return;
-  const int rows = q.count * p.heads;
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const size_t token = q.start + row / p.heads;
-    const int head = row % p.heads;
-    const size_t at = token * p.heads + head, step = (size_t)w.tokens * p.heads;
-    // each part's factor: a thread per part
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if ((int)threadIdx.x < parts) ml = p.part_ml[threadIdx.x * step + at];
-    float best = ml.x;
+  const int thread = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, slice = thread % kSlices, turn = thread / kSlices;
+  const size_t row = WAVES == 1 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x, step = (size_t)w.tokens * p.heads;
+  __shared__ float factors[WAVES == 1 ? 1 : kMostParts];
+  __shared__ float4 sums[WAVES == 1 ? 1 : kTurns][kSlices];
+  __shared__ float2 of_wave[WAVES];
+  if (row >= step) return;  // (whole waves)
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (thread < p.parts) ml = p.part_ml[thread * step + row];  // each part's: a thread per part
+  const float4* from = reinterpret_cast<const float4*>(p.part_o) + row * kSlices + slice;
+  float4 first[kFirst];
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) best = fmaxf(best, __shfl_xor(best, off));
-    if ((threadIdx.x & 63) == 0) wave_best[threadIdx.x >> 6] = best;
-    __syncthreads();
-    best = fmaxf(fmaxf(wave_best[0], wave_best[1]), fmaxf(wave_best[2], wave_best[3]));
-    const float f = ml.y == 0.0f ? 0.0f : ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c);  // (0: a part that saw nothing)
-    factors[threadIdx.x] = f;
-    float total = ml.y * f;
+  for (int j = 0; j < kFirst; ++j) first[j] = turn + j * kTurns < p.parts ? from[(turn + j * kTurns) * step * kSlices] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int token = (int)(row / p.heads), head = (int)(row - (size_t)token * p.heads);
+  if (token < w.starts[0] || token >= w.starts[w.sequences]) return;  // of no sequence (the whole row)
+  float best = ml.x;
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) total += __shfl_xor(total, off);
-    if ((threadIdx.x & 63) == 0) wave_total[threadIdx.x >> 6] = total;
+  for (int off = 1; off < 64; off *= 2) best = fmaxf(best, __shfl_xor(best, off));
+  if constexpr (WAVES > 1) {
+    if ((thread & 63) == 0) of_wave[thread >> 6].x = best;
     __syncthreads();
-    total = (wave_total[0] + wave_total[1]) + (wave_total[2] + wave_total[3]);
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = turn; k < parts; k += kTurns) {
-      const float g = factors[k];
-      if (g == 0.0f) continue;  // (nothing there, or nothing left of it)
-      const float4 o = reinterpret_cast<const float4*>(p.part_o)[(k * step + at) * kSlices + slice];
-      v.x += o.x * g, v.y += o.y * g, v.z += o.z * g, v.w += o.w * g;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) best = fmaxf(best, of_wave[k].x);
+  }
+  const float f = ml.y == 0.0f ? 0.0f : ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c);  // (0: a part that saw nothing)
+  float total = ml.y * f;
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) total += __shfl_xor(total, off);
+  if constexpr (WAVES > 1) {
+    factors[thread] = f;
+    if ((thread & 63) == 0) of_wave[thread >> 6].y = total;
+    __syncthreads();
+    total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) total += of_wave[k].y;
+  }
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](int k, const float4& o) {
+    const float g = WAVES == 1 ? __shfl(f, k) : factors[k];
+    if (g != 0.0f) v.x += o.x * g, v.y += o.y * g, v.z += o.z * g, v.w += o.w * g;  // (0: nothing there, whatever the array holds)
+  };
+#pragma unroll
+  for (int j = 0; j < kFirst; ++j) {
+    const int k = min(turn + j * kTurns, kMostParts - 1);
+    if (j * kTurns < p.parts) add(WAVES == 1 ? k & 63 : k, first[j]);
+  }
+  for (int k0 = kFirst * kTurns; k0 < p.parts; k0 += kTurns) {
+    const int k = k0 + turn;
+    add(WAVES == 1 ? k & 63 : min(k, kMostParts - 1), k < p.parts ? from[k * step * kSlices] : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+  }
+  if constexpr (WAVES == 1) {
+#pragma unroll
+    for (int off = kSlices; off < 64; off *= 2) {
+      v.x += __shfl_xor(v.x, off);
+      v.y += __shfl_xor(v.y, off);
+      v.z += __shfl_xor(v.z, off);
+      v.w += __shfl_xor(v.w, off);
     }
+  } else {
     sums[turn][slice] = v;
     __syncthreads();
-    if (turn == 0) {
 #pragma unroll
-      for (int k = 1; k < kTurns; ++k) {
-        const float4 o = sums[k][slice];
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-      }
-      const float g = total == 0.0f ? 0.0f : 1.0f / total;
-      const half2_t a = {(_Float16)(v.x * g), (_Float16)(v.y * g)}, b = {(_Float16)(v.z * g), (_Float16)(v.w * g)};
-      reinterpret_cast<u32x2*>(p.out)[((size_t)head * kSlices + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
+    for (int k = 1; k < kTurns; ++k) {
+      const float4 o = sums[k][slice];
+      if (turn == 0) v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
     }
-    __syncthreads();
+  }
+  if (turn == 0) {
+    const float g = total == 0.0f ? 0.0f : 1.0f / total;
+    const half2_t a = {(_Float16)(v.x * g), (_Float16)(v.y * g)}, b = {(_Float16)(v.z * g), (_Float16)(v.w * g)};
+    reinterpret_cast<u32x2*>(p.out)[((size_t)head * kSlices + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
   }
 }
 
@@ -883,7 +965,9 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
   p.window = a.window;
   p.c = a.scale * kLog2e;
   p.part_o = a.partial;
-  p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)std::max(plan.few_parts, plan.many_parts) * a.max_tokens * a.heads * D);
+  const int parts = std::max(plan.few_parts, plan.many_parts);  // (what a kernel of fewer parts leaves is marked as having seen nothing)
+  p.joined = parts;
+  p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)parts * a.max_tokens * a.heads * D);
   if (plan.few_rows > 0) {
     p.parts = plan.few_parts;
     p.rows_from = 1;
@@ -902,19 +986,20 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
     const dim3 grid(a.where.kv_heads, std::min(p.parts * DivUp(most_new * share, 32 * ManyWaves(D)), 65535 / p.parts * p.parts), a.where.sequences);
     kv4_attention_many_kernel<D, GJ><<<grid, 64 * ManyWaves(D), 0, stream>>>(p);
   }
-  if (plan.few_parts > 1 || plan.many_parts > 1) {
+  if (parts > 1) {
     JoinParams j;
     j.w = a.where;
     j.part_o = p.part_o;
     j.part_ml = p.part_ml;
     j.out = p.out;
     j.heads = a.heads;
-    j.share = share;
+    j.parts = parts;
     j.c = p.c;
-    j.few_rows = plan.few_rows;
-    j.few_parts = plan.few_parts;
-    j.many_parts = plan.many_parts;
-    kv4_attention_join_kernel<D><<<dim3(most_new * a.heads, a.where.sequences), 256, 0, stream>>>(j);
+    const int rows = a.where.tokens * a.heads;
+    if (parts <= kFewParts)
+      kv4_attention_join_kernel<D, 1><<<DivUp(rows, 4), 256, 0, stream>>>(j);
+    else
+      kv4_attention_join_kernel<D, 4><<<rows, 256, 0, stream>>>(j);
   }
 }
 
@@ -932,7 +1017,7 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   const long long seen = a.window > 0 ? std::min<long long>(keys, a.window) : keys;
   plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && (heads >= 64 || seen > 4096) ? kFewRows : 0;
   // work-groups that are on the chip at once, and parts of at least a step for each wave
-  const long long few_groups = heads * (many ? kFewRows / 16 : (rows + 15) / 16), slots = a.head_dim == 64 ? 768 : a.head_dim == 128 ? 512 : 256;
+  const long long few_groups = heads * (many ? kFewRows / 16 : (rows + 15) / 16), slots = a.head_dim == 64 ? 1024 : a.head_dim == 128 ? 768 : 512;
   const long long many_rows = 32 * ManyWaves(a.head_dim), many_groups = heads * ((rows + many_rows - 1) / many_rows);
   long long few = plan.few_rows > 0 ? std::min(slots / few_groups, (keys + 127) / 128) : 1;
   long long each = many ? std::min(256 / many_groups, (keys + 511) / 512) : 1;

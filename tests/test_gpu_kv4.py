@@ -355,6 +355,51 @@ def test_attention_in_parts(kv_heads, head_dim, group, page, many, parts):
         assert d.op.kernel_variant == ("many" if many else "few")
 
 
+@pytest.mark.parametrize("parts", [-1, 5, 256])
+def test_attention_shares_over_many_sequences(parts):
+    """More sequences than lanes, shares that begin and end inside sequences, and launches again with other lengths."""
+    rng = np.random.default_rng(21)
+    counts = list(rng.integers(0, 3, 150))
+    lengths = [int(c + rng.integers(0, 500)) if c else 0 for c in counts]
+    with M.tuning(kv4_many=0, kv4_parts=parts):
+        d = attention_case(1, 9, 64, 32, 16, counts, lengths, seed=5)
+        q = rng.standard_normal((d.tokens, 9, 64)).astype(np.float16)
+        src, out = dev(slices(q)), torch.zeros((9 * 16, d.tokens, 4), dtype=torch.float16, device="cuda")
+        op = M.kv4_attention_create(d.desc, 9, max_tokens=d.tokens, max_new_tokens=2)
+        op.bind([src, d.cache] + d.where, [out])
+        op.set_shape(1, 1, d.tokens)
+        for turn in range(3):
+            now = [l if turn == 0 else max(int(c), l // (turn + 1)) for c, l in zip(counts, lengths)]
+            d.where[1].copy_(torch.tensor(now, dtype=torch.int32))
+            op.launch(stream())
+            torch.cuda.synchronize()
+            exact, largest, score = attention(q, d.host, d.table, np.array(now), d.starts, 64**-0.5, True, 0)
+            check_attention(unslices(out.cpu().numpy(), 64), exact, largest, score)
+
+
+def test_attention_of_more_than_a_thousand_sequences():
+    attention_case(2, 2, 64, 64, 16, [1] * 1100, [1 + i % 40 for i in range(1100)], seed=6)
+
+
+def test_attention_of_starts_that_decrease_stays_in_bounds():
+    """Not a batch that means anything: whatever is written, it is written into the output, and what is in front of and behind it stays."""
+    starts, lengths = np.array([0, 60, 0, 60, 5, 60, -7, 90]), np.array([60, 0, 60, 0, 60, 0, 60])
+    d = Device(2, 64, 32, 16, 30, starts, lengths, np.arange(28).reshape(7, 4), tokens=60)
+    d.fill(np.random.default_rng(1))
+    size, room = 4 * 16 * 60 * 4, 4096
+    around = torch.full((size + 2 * room,), 7.0, dtype=torch.float16, device="cuda")
+    src = torch.zeros((64, 60, 4), dtype=torch.float16, device="cuda")
+    for many in (0, 1):
+        for parts in (1, 5):
+            with M.tuning(kv4_many=many, kv4_parts=parts):
+                op = M.kv4_attention_create(d.desc, 4, max_tokens=60, max_new_tokens=60)
+            op.bind([src, d.cache] + d.where, [around[room:room + size]])
+            op.set_shape(1, 1, 60)
+            op.launch(stream())
+            torch.cuda.synchronize()
+            assert (around[:room] == 7).all() and (around[room + size:] == 7).all()
+
+
 def test_attention_of_more_rows_than_it_is_sized_for():
     attention_case(1, 4, 64, 32, 16, [90, 200], [90, 230], most=1)
     attention_case(1, 4, 64, 32, 16, [90, 700], [90, 730], most=20)
