@@ -44,7 +44,7 @@ struct AttendParams {
   __half* out;
   float* part_o;   // [parts][rows of the tensors][D]
   float2* part_ml; // [parts][rows]: maximum (of q . k) and sum
-  int heads, share, parts, joined, causal, window;  // parts: of this kernel; joined: of the launch, 1 where outputs are written directly
+  int heads, share, parts, causal, window;
   float c;  // scale * log2(e)
   int rows_from, rows_to;  // sequences of rows_from .. rows_to rows are this kernel's
 };
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
         total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
       }
       const float mine = top[rt] == best ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - best) * p.c);
-      const float factor = mine * (p.joined > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
+      const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
       if (row0 + rt * 16 + n < rows)
 #pragma unroll
         for (int pl = 0; pl < kPlanes; ++pl)
@@ -487,20 +487,18 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
         }
         const int of_sequence = token_of(row), head = kv_head * p.share + row - of_sequence * p.share;
         const size_t token = q.start + of_sequence;
-        if (p.joined > 1) {
+        if (p.parts > 1) {
           reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = v;
         } else {
           const half2_t a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
           reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
         }
       }
-      if (p.joined > 1 && wave == 0 && quad == 0) {
+      if (p.parts > 1 && wave == 0 && quad == 0) {
         const int row = row0 + rt * 16 + n;
         if (row < rows) {
-          float2* to = p.part_ml + (size_t)(q.start + token_of(row)) * p.heads + kv_head * p.share + row - token_of(row) * p.share;
-          to[(size_t)part * w.tokens * p.heads] = make_float2(best, total);
-          if (part == 0)
-            for (int k = p.parts; k < p.joined; ++k) to[(size_t)k * w.tokens * p.heads] = make_float2(-INFINITY, 0.0f);
+          const int of_sequence = token_of(row), head = kv_head * p.share + row - of_sequence * p.share;
+          p.part_ml[((size_t)part * w.tokens + q.start + of_sequence) * p.heads + head] = make_float2(best, total);
         }
       }
       __syncthreads();  // (the arrays are written again)
@@ -830,7 +828,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     if (is_row) {
-      const float factor = p.joined > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+      const float factor = p.parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
       u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
       float4* part_to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + half * kCell;
 #pragma unroll
@@ -843,26 +841,22 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = acc[pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
             const int slice = (pl * P + (8 * (m / 4) + m % 4) * kCell) / 4 + h;  // behind the half's own first
-            if (p.joined > 1) {
+            if (p.parts > 1) {
               part_to[slice] = make_float4(v[0], v[1], v[2], v[3]);
             } else {
               const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
               to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
             }
           }
-      if (p.joined > 1 && half == 0) {
-        float2* ml = p.part_ml + (size_t)token * p.heads + head;
-        ml[(size_t)part * w.tokens * p.heads] = make_float2(top, total);
-        if (part == 0)
-          for (int k = p.parts; k < p.joined; ++k) ml[(size_t)k * w.tokens * p.heads] = make_float2(-INFINITY, 0.0f);
-      }
+      if (p.parts > 1 && half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
     }
   }
 }
 
 // The parts of each row, joined.  A row per work-group of WAVES waves, whose threads share its slices and, in turn, its parts: four waves
 // where parts are many, one where they are few.  Everything is asked for before the first wait (the loads of the parts' outputs do not depend
-// on their sums), and nothing is looked up but where the first sequence begins and the last one ends.
+// on their sums), and nothing is looked up but where the first sequence begins and the last one ends; where both kernels above have a share
+// of the batch, sequence by sequence, those of one kernel only.
 struct JoinParams {
   Kv4Where w;
   const float* part_o;
@@ -870,15 +864,23 @@ struct JoinParams {
   __half* out;
   int heads, parts;
   float c;
+  int share, rows_from, rows_to;  // sequence by sequence: those of rows_from .. rows_to rows
 };
 constexpr int kMostParts = 256, kFewParts = 8;
 constexpr int kFewRows = 32;  // rows of a sequence up to which the kernel for few rows serves it where there are more in a batch
-template <int D, int WAVES>
+template <int D, int WAVES, bool BY_SEQUENCE>
 __global__ __launch_bounds__(256) void kv4_attention_join_kernel(const JoinParams p) {
   constexpr int kSlices = D / 4, kTurns = 64 * WAVES / kSlices, kFirst = 4;
   const Kv4Where& w = p.w;
   const int thread = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, slice = thread % kSlices, turn = thread / kSlices;
-  const size_t row = WAVES == 1 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x, step = (size_t)w.tokens * p.heads;
+  const size_t step = (size_t)w.tokens * p.heads;
+  size_t row = WAVES == 1 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if constexpr (BY_SEQUENCE) {
+    const Kv4Sequence q = Kv4SequenceOf(w, blockIdx.y);
+    const int rows = q.count * p.share;
+    if (rows < p.rows_from || rows > p.rows_to || row >= (size_t)q.count * p.heads) return;
+    row += (size_t)q.start * p.heads;
+  }
   __shared__ float factors[WAVES == 1 ? 1 : kMostParts];
   __shared__ float4 sums[WAVES == 1 ? 1 : kTurns][kSlices];
   __shared__ float2 of_wave[WAVES];
@@ -965,9 +967,7 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
   p.window = a.window;
   p.c = a.scale * kLog2e;
   p.part_o = a.partial;
-  const int parts = std::max(plan.few_parts, plan.many_parts);  // (what a kernel of fewer parts leaves is marked as having seen nothing)
-  p.joined = parts;
-  p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)parts * a.max_tokens * a.heads * D);
+  p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)std::max(plan.few_parts, plan.many_parts) * a.max_tokens * a.heads * D);
   if (plan.few_rows > 0) {
     p.parts = plan.few_parts;
     p.rows_from = 1;
@@ -986,21 +986,21 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
     const dim3 grid(a.where.kv_heads, std::min(p.parts * DivUp(most_new * share, 32 * ManyWaves(D)), 65535 / p.parts * p.parts), a.where.sequences);
     kv4_attention_many_kernel<D, GJ><<<grid, 64 * ManyWaves(D), 0, stream>>>(p);
   }
-  if (parts > 1) {
-    JoinParams j;
-    j.w = a.where;
-    j.part_o = p.part_o;
-    j.part_ml = p.part_ml;
-    j.out = p.out;
-    j.heads = a.heads;
-    j.parts = parts;
-    j.c = p.c;
-    const int rows = a.where.tokens * a.heads;
-    if (parts <= kFewParts)
-      kv4_attention_join_kernel<D, 1><<<DivUp(rows, 4), 256, 0, stream>>>(j);
+  const bool both = plan.few_rows > 0 && plan.few_rows < INT32_MAX;
+  auto join = [&](int of, int rows_from, int rows_to) {
+    if (of == 1) return;
+    const JoinParams j = {a.where, p.part_o, p.part_ml, p.out, a.heads, of, p.c, share, rows_from, rows_to};
+    // (a launch of more rows of a sequence than the op was made for: as many as the tensors have)
+    const int rows = both && rows_to < INT32_MAX ? rows_to / share * a.heads : a.where.tokens * a.heads;
+    const bool few = of <= kFewParts;
+    const dim3 grid(few ? DivUp(rows, 4) : rows, both ? a.where.sequences : 1);
+    if (both)
+      few ? kv4_attention_join_kernel<D, 1, true><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, 4, true><<<grid, 256, 0, stream>>>(j);
     else
-      kv4_attention_join_kernel<D, 4><<<rows, 256, 0, stream>>>(j);
-  }
+      few ? kv4_attention_join_kernel<D, 1, false><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, 4, false><<<grid, 256, 0, stream>>>(j);
+  };
+  if (plan.few_rows > 0) join(plan.few_parts, 1, plan.few_rows);
+  if (plan.few_rows < INT32_MAX) join(plan.many_parts, plan.few_rows + 1, INT32_MAX);
 }
 
 }  // namespace
@@ -1015,18 +1015,34 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   // In a ragged batch sequences of few rows go to the kernel for few where they could be many, or see more than the prompts' own work-groups
   // take anyway; else a work-group of the other kernel each, beside the prompts', costs less than one more launch.
   const long long seen = a.window > 0 ? std::min<long long>(keys, a.window) : keys;
-  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && (heads >= 64 || seen > 4096) ? kFewRows : 0;
-  // work-groups that are on the chip at once, and parts of at least a step for each wave
-  const long long few_groups = heads * (many ? kFewRows / 16 : (rows + 15) / 16), slots = a.head_dim == 64 ? 1024 : a.head_dim == 128 ? 768 : 512;
-  const long long many_rows = 32 * ManyWaves(a.head_dim), many_groups = heads * ((rows + many_rows - 1) / many_rows);
-  long long few = plan.few_rows > 0 ? std::min(slots / few_groups, (keys + 127) / 128) : 1;
-  long long each = many ? std::min(256 / many_groups, (keys + 511) / 512) : 1;
-  if (t.kv4_parts > 0) few = each = std::min<long long>(t.kv4_parts, (keys + 127) / 128);
+  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && share <= kFewRows && (heads >= 64 || seen > 4096) ? kFewRows : 0;
   // the parts' outputs: at most 256 MB
-  const long long room = ((long long)256 << 20) / ((long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4);
-  const auto parts = [&](long long v) { return (int)std::max(1LL, std::min(std::min(v, room), (long long)kMostParts)); };
-  plan.few_parts = plan.few_rows > 0 ? parts(few) : 1;
-  plan.many_parts = many ? parts(each) : 1;
+  const long long row_bytes = (long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4, room = ((long long)256 << 20) / row_bytes;
+  const auto parts = [&](long long v) { return (int)std::max(1LL, std::min({v, room, (long long)kMostParts})); };
+  if (plan.few_rows > 0) {
+    // as many work-groups as are on the chip at once (32 sequences of up to 4096 positions, 8 key heads of 128: 33.9 us in 2 parts, 31.8 in 3,
+    // 34.6 in 4), each with at least a step for each of its waves
+    const long long groups = heads * (((many ? std::min<long long>(rows, kFewRows) : rows) + 15) / 16);
+    const long long slots = a.head_dim == 64 ? 1024 : a.head_dim == 128 ? 768 : 512;
+    plan.few_parts = parts(std::min(t.kv4_parts > 0 ? t.kv4_parts : slots / groups, (keys + 127) / 128));
+  }
+  if (many) {
+    // Parts level the work-groups' shares, and their outputs go through memory: the number with the least estimated time.  Steps that the
+    // longest work-group takes, and those that each of the 256 takes where they are level; a step and a byte by what they measured.
+    const int step = 16 * ManyWaves(a.head_dim), tile = 32 * ManyWaves(a.head_dim);
+    const double step_us = a.head_dim == 64 ? 2.7 : a.head_dim == 128 ? 3.7 : 2.6;
+    const double groups = (double)heads * ((rows + tile - 1) / tile), longest = std::max<double>(1, (double)(a.window > 0 ? std::min<long long>(keys, a.window + tile / share) : keys) / step);
+    const double level = groups * longest / 256 * (a.window > 0 || !a.causal ? 1.0 : 1.0 - 0.5 * std::min<double>(1, (double)most_new / keys));
+    double least = 0;
+    for (int n = 1; n <= kMostParts && n <= std::max(1.0, longest / 2); ++n) {
+      const double steps = groups * n <= 256 ? longest / n : level + 0.5 * longest / n;
+      const double us = steps * step_us + (n > 1 ? 5 + 2 * n * (double)row_bytes / 4.5e6 : 0);
+      if (n > 1 && us >= least) continue;
+      least = us;
+      plan.many_parts = n;
+    }
+    plan.many_parts = parts(t.kv4_parts > 0 ? std::min<long long>(t.kv4_parts, (keys + 127) / 128) : plan.many_parts);
+  }
   return plan;
 }
 

@@ -355,6 +355,22 @@ def test_attention_in_parts(kv_heads, head_dim, group, page, many, parts):
         assert d.op.kernel_variant == ("many" if many else "few")
 
 
+def test_attention_of_many_heads_for_a_key_head():
+    """More heads on a key head than rows that the kernel for few takes: every row of a ragged batch is the other kernel's."""
+    d = attention_case(8, 40, 64, 32, 16, [1, 3, 0, 2, 1, 1, 1, 1], [90, 40, 3, 333, 200, 1, 17, 64])
+    assert d.op.kernel_variant == "many"
+    with M.tuning(kv4_parts=3):
+        attention_case(8, 40, 64, 32, 16, [1, 3, 0, 2, 1, 1, 1, 1], [90, 40, 3, 333, 200, 1, 17, 64])
+
+
+def test_attention_parts_of_one_kernel_beside_whole_rows_of_the_other():
+    """Long tables: sequences of few rows in parts, prompts not, and the other way round."""
+    for parts in (-1, 2):
+        with M.tuning(kv4_parts=parts):
+            d = attention_case(1, 4, 128, 64, 64, [1, 80, 2, 1], [5000, 200, 4400, 70], seed=parts + 1)
+        assert d.op.kernel_variant == "many, few"
+
+
 @pytest.mark.parametrize("parts", [-1, 5, 256])
 def test_attention_shares_over_many_sequences(parts):
     """More sequences than lanes, shares that begin and end inside sequences, and launches again with other lengths."""
@@ -465,6 +481,181 @@ def test_attention_of_rows_that_are_not_finite():
         with M.tuning(kv4_many=many):
             got, rest = d.attend(q, 2), d.attend(q2, 2)
         assert np.isnan(got[1, 0]).all() and np.array_equal(got[same], rest[same])
+
+
+# ---- launches ------------------------------------------------------------------------------------------------------------------------
+
+def decode_step(rng, kv_heads=2, share=4, head_dim=128, group=32, page=16, counts=(1, 1, 2, 1), lengths=(40, 300, 65, 1)):
+    """The ops of one layer's step over one batch, bound one behind the other, and the host's copies of what they read."""
+    starts, lengths, table, pages = batch(rng, list(counts), list(lengths), page, extra=5)
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table)
+    d.fill(rng)
+    heads, t = kv_heads * share, d.tokens
+    host = [rng.standard_normal((t, h, head_dim)).astype(np.float16) for h in (heads, kv_heads, kv_heads)]
+    q, k, v = [dev(slices(x)) for x in host]
+    positions = np.concatenate([np.arange(l - c, l) for c, l in zip(counts, lengths)])
+    weights = [rng.standard_normal(head_dim).astype(np.float16) for _ in range(2)]
+    most = max(counts)
+    rope = M.qk_norm_rope_create(M.FLOAT16, heads, kv_heads, head_dim, norm=True, weight_offset=1.0, max_tokens=t)
+    d.keep = [dev(positions.astype(np.int32))] + [dev(w) for w in weights]  # (an op holds raw pointers)
+    rope.bind([q, k] + d.keep, [q, k])
+    append = M.kv4_append_create(d.desc, M.FLOAT16, t, most)
+    append.bind([k, v] + d.where, [d.cache])
+    out = torch.zeros_like(q)
+    attend = M.kv4_attention_create(d.desc, heads, max_tokens=t, max_new_tokens=most)
+    attend.bind([q, d.cache] + d.where, [out])
+    for op in (rope, append, attend):
+        op.set_shape(1, 1, t)
+    return d, host, positions, weights, (q, k, v), out, (rope, append, attend), table, starts
+
+
+def check_step(d, host, positions, weights, out, table, starts):
+    """The step's output against 64 bits throughout, but for what the step itself rounds to halfs on the way."""
+    head_dim = d.desc.head_dim
+    q, k = [norm_rope(x, positions, head_dim, False, weight=w, offset=1.0).astype(np.float16) for x, w in zip(host[:2], weights)]
+    for s in range(len(d.lengths)):
+        for i in range(starts[s], starts[s + 1]):
+            p = positions[i]
+            d.host.set_token(table[s][p // d.desc.page_size], p % d.desc.page_size, k[i], host[2][i])
+    exact, largest, score = attention(q, d.host, table, d.lengths, starts, head_dim**-0.5, True, 0)
+    # The step's q and k may be a half's step off these where the rounding falls the other way, and a key's code with it: a scale (of at most
+    # 2 max|k| / 15) of one key channel and 2^-10 of q, of which a score of `score` is at most (1/4 + 2^-10) off, in all but a few rows much
+    # less; an output moves by at most twice that of the values' range.
+    tol = 2 * (0.25 + 2.0**-10) * score * largest + 2.0**-10 * largest
+    err = np.abs(unslices(out.cpu().numpy(), head_dim).astype(np.float64) - exact)
+    rms = np.sqrt((err**2).mean()) / np.sqrt((exact**2).mean())
+    assert (err <= tol).all() and rms < 2.0**-7, rms
+
+
+def test_a_step_captured_and_replayed():
+    """The step in a graph: replays with other inputs in the same buffers, eager work in between, every one against the eager launches."""
+    rng = np.random.default_rng(31)
+    d, host, positions, weights, (q, k, v), out, ops, table, starts = decode_step(rng)
+    first = [x.clone() for x in (q, k, v)]
+    cache = d.cache.clone()
+
+    def reset(scale):
+        for x, y in zip((q, k, v), first):
+            x.copy_(y * scale)
+        d.cache.copy_(cache)
+
+    def run():
+        for op in ops:
+            op.launch(stream())
+
+    eager = []
+    for scale in (1.0, 0.5, 2.0):
+        reset(scale)
+        run()
+        torch.cuda.synchronize()
+        eager.append((out.clone(), d.cache.clone()))
+    check_step(d, [x.astype(np.float64) * 2 for x in host], positions, weights, out, table, starts)
+    reset(1.0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+    for turn in range(6):
+        reset((1.0, 0.5, 2.0)[turn % 3])
+        out.fill_(3.0)
+        graph.replay()
+        if turn % 2:
+            torch.cuda.synchronize()
+            (out * 2).sum().item()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[turn % 3][0]) and torch.equal(d.cache, eager[turn % 3][1])
+
+
+def test_a_step_on_another_stream():
+    rng = np.random.default_rng(32)
+    d, host, positions, weights, tensors, out, ops, table, starts = decode_step(rng)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for op in ops:
+            op.launch(side.cuda_stream)
+    side.synchronize()
+    check_step(d, host, positions, weights, out, table, starts)
+
+
+def test_two_ops_at_the_same_time():
+    """Two batches on two streams, each with ops (and workspaces) of its own."""
+    steps = [decode_step(np.random.default_rng(40 + i), page=64, counts=(1, 1), lengths=(2000, 777)) for i in range(2)]
+    alone = []
+    for s in steps:
+        keep = [x.clone() for x in s[4]] + [s[0].cache.clone()]
+        for op in s[6]:
+            op.launch(stream())
+        torch.cuda.synchronize()
+        alone.append(s[5].clone())
+        for x, y in zip(list(s[4]) + [s[0].cache], keep):
+            x.copy_(y)
+        s[5].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for k in range(3):
+        for s, st in zip(steps, streams):
+            s[6][k].launch(st.cuda_stream)
+    torch.cuda.synchronize()
+    for s, want in zip(steps, alone):
+        assert torch.equal(s[5], want)
+
+
+@pytest.mark.parametrize("many", [0, 1])
+def test_attention_is_the_same_every_time(many):
+    rng = np.random.default_rng(33)
+    starts, lengths, table, pages = batch(rng, [3, 40, 1], [2000, 300, 1500], 16)
+    d = Device(2, 64, 32, 16, pages, starts, lengths, table)
+    d.fill(rng)
+    q = rng.standard_normal((44, 6, 64)).astype(np.float16)
+    with M.tuning(kv4_many=many):
+        a = d.attend(q, 6)
+        assert all(np.array_equal(d.attend(q, 6, launches=n), a) for n in (1, 2, 3))
+
+
+def test_a_cache_of_more_than_four_gigabytes():
+    """Pages whose bytes lie behind 2^32: written, read and attended there."""
+    kv_heads, head_dim, group, page = 8, 256, 32, 1024
+    per_page = kv_heads * page * (head_dim + 4 * head_dim // group)
+    pages = (9 << 30) // per_page
+    cache = M.kv4_cache_desc(kv_heads, head_dim, group, page, pages, 2, 1)
+    assert M.kv4_cache_bytes(cache) > 8 << 30
+    rng = np.random.default_rng(34)
+    big = torch.zeros(M.kv4_cache_bytes(cache), dtype=torch.uint8, device="cuda")
+    starts, lengths, table = np.array([0, 20, 30]), np.array([20, 10]), np.array([[pages - 1], [pages // 2 + 1]])
+    where = [dev(np.asarray(a).astype(np.int32)) for a in (table, lengths, starts)]
+    k, v = [rng.standard_normal((30, kv_heads, head_dim)).astype(np.float16) for _ in range(2)]
+    q = rng.standard_normal((30, kv_heads * 2, head_dim)).astype(np.float16)
+    src = [dev(slices(x)) for x in (k, v, q)]
+    append = M.kv4_append_create(cache, M.FLOAT16, 30, 20)
+    append.bind(src[:2] + where, [big])
+    back = [torch.zeros_like(x) for x in src[:2]]
+    read = M.kv4_read_create(cache, M.FLOAT16, 30, 20)
+    read.bind([big] + where, back)
+    for op in (append, read):
+        op.set_shape(1, 1, 30)
+        op.launch(stream())
+    torch.cuda.synchronize()
+    for x, y in zip(back, (k, v)):
+        assert np.array_equal(unslices(x.cpu().numpy(), head_dim).astype(np.float64), kept(y.astype(np.float64), group))
+    small = Cache(kv_heads, head_dim, group, 32, 2)
+    for s in range(2):
+        for i in range(lengths[s]):
+            small.set_token(s, i, k[starts[s] + i], v[starts[s] + i])
+    exact, largest, score = attention(q, small, np.array([[0], [1]]), lengths, starts, head_dim**-0.5, True, 0)
+    for many in (0, 1):
+        with M.tuning(kv4_many=many):
+            op = M.kv4_attention_create(cache, kv_heads * 2, max_tokens=30, max_new_tokens=20)
+        out = torch.zeros_like(src[2])
+        op.bind([src[2], big] + where, [out])
+        op.set_shape(1, 1, 30)
+        op.launch(stream())
+        torch.cuda.synchronize()
+        check_attention(unslices(out.cpu().numpy(), head_dim), exact, largest, score)
+    op = None
+    del big
+    torch.cuda.empty_cache()
 
 
 # ---- together --------------------------------------------------------------------------------------------------------------------
