@@ -430,7 +430,7 @@ int mldhip_conv_int8_create(const mldhip_conv_int8_desc* desc, mldhip_op** op);
  * the o projection reads, [channels / 4][tokens][4] with channel = head * head_dim + channel of the head, and follow the op contract
  * above: objects bound by index, mldhip_op_set_shape(op, 1, 1, tokens), launches on the caller's stream that neither allocate nor
  * synchronise and may be captured.  An op runs on the device that was current when it was created (FAILED_PRECONDITION with another one
- * current); launches of one op that has a workspace must not overlap in time. */
+ * current); launches of one op that has a workspace must not overlap in time.  max_tokens is at most 2^24. */
 
 /* Norms of the query and key heads (left out where norm is 0) and the rotation by position, in one pass:
  *   y = x / sqrt(mean over the head's channels of x^2 + eps) * (weight_offset + weight)
@@ -504,7 +504,7 @@ int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int
  * max_new_tokens chooses between the kernels for few and for many rows of a sequence; launches with more rows than that are served. */
 typedef struct {
   mldhip_kv4_cache_desc cache;
-  int32_t heads; /* a multiple of cache.kv_heads */
+  int32_t heads; /* a multiple of cache.kv_heads; max_tokens * heads is at most 2^30 */
   float scale;   /* positive */
   int32_t causal;
   int32_t window; /* 0: none */

@@ -616,6 +616,8 @@ static int CurrentDevice() {
   return device;
 }
 
+constexpr int kMostTokens = 1 << 24;  // of one launch: work-items of a grid stay below 2^32
+
 int mldhip_qk_norm_rope_create(const mldhip_qk_norm_rope_desc* d, mldhip_op** out) {
   if (!d || !out) return Fail(MLDHIP_INVALID_ARGUMENT, "null argument");
   *out = nullptr;
@@ -623,6 +625,7 @@ int mldhip_qk_norm_rope_create(const mldhip_qk_norm_rope_desc* d, mldhip_op** ou
     return Fail(MLDHIP_INVALID_ARGUMENT, "tensors must be FLOAT16 or FLOAT32");
   if (d->heads < 1 || d->kv_heads < 1 || d->max_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "bad shape");
   if ((long long)d->heads + d->kv_heads > 65535) return Fail(MLDHIP_OUT_OF_RANGE, "more than 65535 heads");
+  if (d->max_tokens > kMostTokens) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens exceeds 2^24");
   if (d->head_dim < 8 || d->head_dim % 8 != 0) return Fail(MLDHIP_INVALID_ARGUMENT, "head_dim must be a multiple of 8");
   if (d->head_dim > 256) return Fail(MLDHIP_UNIMPLEMENTED, "heads of more than 256 channels are not served");
   if (d->rotary_dim < 0 || d->rotary_dim % 8 != 0 || d->rotary_dim > d->head_dim)
@@ -680,6 +683,9 @@ static int CheckKv4Cache(const mldhip_kv4_cache_desc* c) {
     return Fail(MLDHIP_INVALID_ARGUMENT, "page_size must be a power of two, 16 .. 1024");
   if (c->kv_heads > 32767 || c->sequences > 65535) return Fail(MLDHIP_OUT_OF_RANGE, "at most 32767 key / value heads and 65535 sequences");
   if ((long long)c->pages_per_sequence * c->page_size > 1 << 30) return Fail(MLDHIP_OUT_OF_RANGE, "more than 2^30 positions in a sequence");
+  // (pages * kv_heads < 2^46; a block has at most 2^19 bytes)
+  if ((double)c->pages * c->kv_heads * (double)Kv4BlockBytes(c->page_size, c->head_dim, c->head_dim / c->group_size) > 0x1p48)
+    return Fail(MLDHIP_OUT_OF_RANGE, "a cache of more than 2^48 bytes");
   return MLDHIP_OK;
 }
 
@@ -700,6 +706,7 @@ static int CreateKv4Move(const mldhip_kv4_cache_desc* cache, int type, int max_t
   if (int rc = CheckKv4Cache(cache)) return rc;
   if (type != MLDHIP_FLOAT16 && type != MLDHIP_FLOAT32) return Fail(MLDHIP_INVALID_ARGUMENT, "tensors must be FLOAT16 or FLOAT32");
   if (max_tokens < 1 || max_new_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "max_tokens and max_new_tokens must be positive");
+  if (max_tokens > kMostTokens) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens exceeds 2^24");
   mldhip_op* op = new (std::nothrow) mldhip_op();
   if (!op) return Fail(MLDHIP_INTERNAL, "out of memory");
   op->kind = read ? mldhip_op::kKv4Read : mldhip_op::kKv4Append;
@@ -780,6 +787,7 @@ int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* d, mldhip_op** 
   if (int rc = CheckKv4Cache(&d->cache)) return rc;
   if (d->heads < 1 || d->heads % d->cache.kv_heads != 0) return Fail(MLDHIP_INVALID_ARGUMENT, "heads must be a multiple of kv_heads");
   if (d->max_tokens < 1 || d->max_new_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "max_tokens and max_new_tokens must be positive");
+  if (d->max_tokens > kMostTokens) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens exceeds 2^24");
   if ((long long)d->max_tokens * d->heads > 1 << 30) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens * heads exceeds 2^30");
   if (!(d->scale > 0.0f && std::isfinite(d->scale))) return Fail(MLDHIP_INVALID_ARGUMENT, "scale must be positive");
   if (d->causal != 0 && d->causal != 1) return Fail(MLDHIP_INVALID_ARGUMENT, "causal must be 0 or 1");
@@ -813,6 +821,8 @@ int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* d, mldhip_op** 
 
 // Launches of these ops.
 static int LaunchAroundAttention(mldhip_op* op, hipStream_t stream) {
+  if (op->kind == mldhip_op::kKv4Attention && op->dst_ptr[0] == op->src_ptr[0])
+    return Fail(MLDHIP_INVALID_ARGUMENT, "dst_tensor must not be src_q");
   int device = -1;
   if (hipGetDevice(&device) != hipSuccess || device != op->device) {
     (void)hipGetLastError();

@@ -74,7 +74,7 @@ struct Unpack {
 // Few rows for each key head (single tokens, speculated ones): the cache's bytes bound it, so the keys of a sequence are dealt to the
 // waves of `parts` work-groups, each wave with its own maximum, sum and output, joined at the end.
 //
-// A wave takes 32 positions at a time against RT tiles of 16 rows, by 16x16x32 products:
+// A wave takes 32 positions at a time against a tile of 16 rows, by 16x16x32 products:
 //   scores^T [16 positions][16 rows] = codes of keys x q^T     a lane has one row (lane & 15) and 4 positions (4 (lane >> 4) + i)
 //   out^T   [16 cells][16 rows]     += values^T x p^T          of 32 positions: those that the lanes hold are the operand's order, so the
 //                                                              probabilities go from one product to the next in registers
@@ -128,7 +128,7 @@ __device__ __forceinline__ uint32_t OfRow(uint32_t v, int from) {  // (`from` is
   }
 }
 
-template <int D, int GJ, int RT, bool BIG>
+template <int D, int GJ, bool BIG>
 __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_attention_few_kernel(const AttendParams p) {
   using S = FewShape<D, GJ>;
   constexpr int P = S::P, kPlanes = S::kPlanes, kCell = S::kCell, kGroups = S::kGroups, kKeyRegs = S::kKeyRegs, kTiles = S::kTiles, kStep = S::kStep;
@@ -146,16 +146,16 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
   const int rows = q.count * p.share;
   if (rows < p.rows_from || rows > p.rows_to) return;
   __shared__ float4 sum_lds[4][16][D / 4 + 1];
-  __shared__ float2 ml_lds[4][16 * RT];
+  __shared__ float2 ml_lds[4][16];
   const Unpack unpack;
   const uint32_t key_at = (n * 4 + quad) * (P / 8), value_at = (quad * 16 + n) * (2 * kCell);  // a lane's piece of a tile's codes
   const uint32_t value_word_at = 32 * (n * kCell / (32 * GJ)) + 8 * quad;
 
   // (a sequence with one new token, the common case, divides nothing)
   auto token_of = [&](int row) { return q.count == 1 ? 0 : row / p.share; };
-  for (int row0 = tile0 * 16 * RT; row0 < rows; row0 += tile_step * 16 * RT) {
+  for (int row0 = tile0 * 16; row0 < rows; row0 += tile_step * 16) {
     // the positions that the tile's rows see: [lo, hi), in steps dealt to the parts and, one by one, to their waves
-    const int first_row = q.first + token_of(row0), last_row = q.first + token_of(min(rows, row0 + 16 * RT) - 1);
+    const int first_row = q.first + token_of(row0), last_row = q.first + token_of(min(rows, row0 + 16) - 1);
     const int hi = p.causal ? min(q.held, last_row + 1) : q.held;
     const int lo = p.window > 0 ? max(0, first_row + 1 - p.window) : 0;
     const int step0 = lo / kStep, steps = hi > lo ? (hi - 1) / kStep + 1 - step0 : 0;
@@ -238,101 +238,83 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
       ids_next = look_up(min(begin + 4, end - 1));
     }
 
-    u32x4 qa[RT][kKeyRegs];       // operands of the first product: channel s and channel s + 4 of 8 in each register
+    u32x4 qa[kKeyRegs];  // operands of the first product: channel s and channel s + 4 of 8 in each register
     // minus the sum of the row's q over a group; what the sums of products start from: minus the sum of q times the codes' bases, and the
     // base of the zero points times the sum of q
-    float qsum[RT][kGroups], qbase[RT][kGroups];
-    int row_lo[RT], row_hi[RT];   // what the lane's row sees
+    float qsum[kGroups], qbase[kGroups];
+    const int row = row0 + n;
+    const bool there = row < rows;
+    const int token = token_of(there ? row : 0), head = kv_head * p.share + (there ? row : 0) - token * p.share;
+    // (one address of the lane and uniform strides: the lanes' own products would be hoisted out of the loop, two registers each)
+    const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + ((size_t)head * (D / 4) + 2 * quad) * w.tokens + q.start + token;
+    const int position = q.first + token;
+    // what the lane's row sees
+    const int row_hi = there ? (p.causal ? min(q.held, position + 1) : q.held) : 0, row_lo = p.window > 0 ? max(0, position + 1 - p.window) : 0;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int row = row0 + rt * 16 + n;
-      const bool there = row < rows;
-      const int token = token_of(there ? row : 0), head = kv_head * p.share + (there ? row : 0) - token * p.share;
-      // (one address of the lane and uniform strides: the lanes' own products would be hoisted out of the loop, two registers each)
-      const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + ((size_t)head * (D / 4) + 2 * quad) * w.tokens + q.start + token;
-      const int position = q.first + token;
-      row_hi[rt] = there ? (p.causal ? min(q.held, position + 1) : q.held) : 0;
-      row_lo[rt] = p.window > 0 ? max(0, position + 1 - p.window) : 0;
+    for (int g = 0; g < kGroups; ++g) qsum[g] = qbase[g] = 0.0f;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) qsum[rt][g] = qbase[rt][g] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kKeyRegs; ++k) {
-        u32x2 a = {0u, 0u}, b = {0u, 0u};
-        if (there) {
-          a = src[(size_t)(8 * k) * w.tokens];
-          b = src[(size_t)(8 * k + 1) * w.tokens];
-        }
-        qa[rt][k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
-                          __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
-        float low = 0.0f, high = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const half2_t v = AsHalf2(qa[rt][k][e]);
-          ((e & 1) ? high : low) += (float)v.x + (float)v.y;
-        }
-        qsum[rt][k / GJ] += low + high;
-        qbase[rt][k / GJ] += kLowOffset * low + kHighOffset * high;
+    for (int k = 0; k < kKeyRegs; ++k) {
+      u32x2 a = {0u, 0u}, b = {0u, 0u};
+      if (there) {
+        a = src[(size_t)(8 * k) * w.tokens];
+        b = src[(size_t)(8 * k + 1) * w.tokens];
       }
+      qa[k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
+                    __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
+      float low = 0.0f, high = 0.0f;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        qsum[rt][g] = -SumAcrossQuarters(qsum[rt][g]);
-        qbase[rt][g] = -SumAcrossQuarters(qbase[rt][g]) - kLowOffset * qsum[rt][g];
+      for (int e = 0; e < 4; ++e) {
+        const half2_t v = AsHalf2(qa[k][e]);
+        ((e & 1) ? high : low) += (float)v.x + (float)v.y;
       }
+      qsum[k / GJ] += low + high;
+      qbase[k / GJ] += kLowOffset * low + kHighOffset * high;
+    }
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      qsum[g] = -SumAcrossQuarters(qsum[g]);
+      qbase[g] = -SumAcrossQuarters(qbase[g]) - kLowOffset * qsum[g];
     }
 
-    float4_t acc[RT][kPlanes][kCell];
-    float top[RT], sum[RT];
+    float4_t acc[kPlanes][kCell];
+    float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      top[rt] = -INFINITY;
-      sum[rt] = 0.0f;
+    for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl)
-#pragma unroll
-        for (int j = 0; j < kCell; ++j) acc[rt][pl][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+      for (int j = 0; j < kCell; ++j) acc[pl][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
     for (int step = begin; step < end; step += 4) {
-      // scores: score[rt][u][i] = q . k of row n and position 16 u + 4 quad + i
-      float score[RT][kTiles][4];
+      // scores: score[u][i] = q . k of row n and position 16 u + 4 quad + i
+      float score[kTiles][4];
       if constexpr (kGroups == 8) {  // (what the sums start from, four times each, would stay in 32 registers over the loop)
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) asm volatile("" : "+v"(qbase[0][g]));
+        for (int g = 0; g < kGroups; ++g) asm volatile("" : "+v"(qbase[g]));
       }
 #pragma unroll
       for (int u = 0; u < kTiles; ++u) {
-        float4_t raw[RT][kGroups];
+        float4_t raw[kGroups];
 #pragma unroll
         for (int k = 0; k < kKeyRegs; ++k) {
           const uint32_t a = c.keys[u][k], b = a >> 8;
           const u32x4 codes = {unpack.Low(a), unpack.High(a), unpack.Low(b), unpack.High(b)};
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const float o = qbase[rt][k / GJ];
-            const float4_t from = k % GJ == 0 ? float4_t{o, o, o, o} : raw[rt][k / GJ];
-            raw[rt][k / GJ] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes),
-                                                                    __builtin_bit_cast(half8_t, qa[rt][k]), from, 0, 0, 0);
-          }
+          const float o = qbase[k / GJ];
+          const float4_t from = k % GJ == 0 ? float4_t{o, o, o, o} : raw[k / GJ];
+          raw[k / GJ] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes),
+                                                                  __builtin_bit_cast(half8_t, qa[k]), from, 0, 0, 0);
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) score[rt][u][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) score[u][i] = 0.0f;
 #pragma unroll
         for (int g = 0; g < kGroups; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t word = OfRow(c.key_words[i / 2], u * kGroups + g);
             const float scale = (float)AsHalf2(word & unpack.scale_mask)[i % 2], zero = (float)AsHalf2(unpack.Low(word))[i % 2];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              score[rt][u][i] = fmaf(scale, fmaf(zero, qsum[rt][g], raw[rt][g][i]), score[rt][u][i]);
+            score[u][i] = fmaf(scale, fmaf(zero, qsum[g], raw[g][i]), score[u][i]);
           }
         // (a tile's products and sums at a time: left alone, the compiler puts all the step's products first and needs registers for them)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(score[rt][u][i]));
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(score[u][i]));
       }
       // (the next step's keys come while this one's values are taken, and the other way round)
       if (step + 4 < end) load_keys(step + 4, ids_next, c);
@@ -349,10 +331,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
           const bool there = id >= 0 && id < w.pages;
           const int at = step * kStep + 16 * u + 4 * quad;
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!there || at + i >= row_hi[rt] || at + i < row_lo[rt]) score[rt][u][i] = -INFINITY;
+          for (int i = 0; i < 4; ++i)
+            if (!there || at + i >= row_hi || at + i < row_lo) score[u][i] = -INFINITY;
           // what lies behind the held positions may be anything: as values it is 0 (0 * NaN would not be)
 #pragma unroll
           for (int pl = 0; pl < kPlanes; ++pl)
@@ -365,40 +345,34 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
       }
 
       // the running maximum; what the new one is above the old scales the sums so far
+      float best = score[0][0];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float best = score[rt][0][0];
+      for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u)
+        for (int i = 0; i < 4; ++i) best = fmaxf(best, score[u][i]);
+      best = MaxAcrossQuarters(best);
+      if (__any(best > top)) {
+        const float now = fmaxf(top, best);
+        const float down = top == now ? 1.0f : __builtin_amdgcn_exp2f((top - now) * p.c);  // (-inf - finite: 0)
+        top = now;
+        sum *= down;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) best = fmaxf(best, score[rt][u][i]);
-        best = MaxAcrossQuarters(best);
-        if (__any(best > top[rt])) {
-          const float now = fmaxf(top[rt], best);
-          const float down = top[rt] == now ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - now) * p.c);  // (-inf - finite: 0)
-          top[rt] = now;
-          sum[rt] *= down;
+        for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
-          for (int pl = 0; pl < kPlanes; ++pl)
-#pragma unroll
-            for (int j = 0; j < kCell; ++j) acc[rt][pl][j] *= down;
-        }
+          for (int j = 0; j < kCell; ++j) acc[pl][j] *= down;
       }
 
-      half2_t prob[RT][kTiles][2];
+      half2_t prob[kTiles][2];
+      const float base = top == -INFINITY ? 0.0f : kLift - top * p.c;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float base = top[rt] == -INFINITY ? 0.0f : kLift - top[rt] * p.c;
+      for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float a = __builtin_amdgcn_exp2f(fmaf(score[rt][u][2 * i], p.c, base));
-            const float b = __builtin_amdgcn_exp2f(fmaf(score[rt][u][2 * i + 1], p.c, base));
-            sum[rt] += a + b;
-            prob[rt][u][i] = half2_t{(_Float16)a, (_Float16)b};
-          }
-      }
+        for (int i = 0; i < 2; ++i) {
+          const float a = __builtin_amdgcn_exp2f(fmaf(score[u][2 * i], p.c, base));
+          const float b = __builtin_amdgcn_exp2f(fmaf(score[u][2 * i + 1], p.c, base));
+          sum += a + b;
+          prob[u][i] = half2_t{(_Float16)a, (_Float16)b};
+        }
 
       // out^T += values^T x p^T, 32 positions at a time
 #pragma unroll
@@ -429,12 +403,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
                   const half2_t x = (e & 1) ? AsHalf2(unpack.High(word)) - high_zero[v][i] : AsHalf2(unpack.Low(word)) - low_zero[v][i];
                   op[2 * v + i] = AsU32(x * scale[v][i]);
                 }
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt) {
-                const u32x4 pr = {AsU32(prob[rt][u][0]), AsU32(prob[rt][u][1]), AsU32(prob[rt][u + 1][0]), AsU32(prob[rt][u + 1][1])};
-                acc[rt][pl][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    __builtin_bit_cast(half8_t, op), __builtin_bit_cast(half8_t, pr), acc[rt][pl][4 * h + e], 0, 0, 0);
-              }
+              const u32x4 pr = {AsU32(prob[u][0]), AsU32(prob[u][1]), AsU32(prob[u + 1][0]), AsU32(prob[u + 1][1])};
+              acc[pl][4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(half8_t, op), __builtin_bit_cast(half8_t, pr), acc[pl][4 * h + e], 0, 0, 0);
             }
         }
       }
@@ -444,65 +415,53 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
       __builtin_amdgcn_sched_barrier(0);
     }
 
-    // the waves' outputs of each tile of rows, at the common maximum
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      sum[rt] = SumAcrossQuarters(sum[rt]);
-      if (quad == 0) ml_lds[wave][rt * 16 + n] = make_float2(top[rt], sum[rt]);
-    }
+    // the waves' outputs, at the common maximum
+    sum = SumAcrossQuarters(sum);
+    if (quad == 0) ml_lds[wave][n] = make_float2(top, sum);
     __syncthreads();
+    float best = -INFINITY, total = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float best = -INFINITY, total = 0.0f;
+    for (int v = 0; v < 4; ++v) best = fmaxf(best, ml_lds[v][n].x);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) best = fmaxf(best, ml_lds[v][rt * 16 + n].x);
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float2 ml = ml_lds[v][rt * 16 + n];
-        total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
-      }
-      const float mine = top[rt] == best ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - best) * p.c);
-      const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
-      if (row0 + rt * 16 + n < rows)
-#pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int h = 0; h < kCell / 4; ++h)
-              sum_lds[wave][n][(pl * P + (4 * quad + i) * kCell) / 4 + h] =
-                make_float4(acc[rt][pl][4 * h][i] * factor, acc[rt][pl][4 * h + 1][i] * factor, acc[rt][pl][4 * h + 2][i] * factor,
-                            acc[rt][pl][4 * h + 3][i] * factor);
-      __syncthreads();
-      // the rows that there are x D / 4 slices
-      const int mine_rows = min(16, rows - row0 - rt * 16);
-      for (int item = threadIdx.x; item < mine_rows * (D / 4); item += 256) {
-        const int r = item / (D / 4), slice = item % (D / 4);
-        const int row = row0 + rt * 16 + r;
-        float4 v = sum_lds[0][r][slice];
-#pragma unroll
-        for (int k = 1; k < 4; ++k) {
-          const float4 o = sum_lds[k][r][slice];
-          v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-        }
-        const int of_sequence = token_of(row), head = kv_head * p.share + row - of_sequence * p.share;
-        const size_t token = q.start + of_sequence;
-        if (p.parts > 1) {
-          reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = v;
-        } else {
-          const half2_t a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
-          reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
-        }
-      }
-      if (p.parts > 1 && wave == 0 && quad == 0) {
-        const int row = row0 + rt * 16 + n;
-        if (row < rows) {
-          const int of_sequence = token_of(row), head = kv_head * p.share + row - of_sequence * p.share;
-          p.part_ml[((size_t)part * w.tokens + q.start + of_sequence) * p.heads + head] = make_float2(best, total);
-        }
-      }
-      __syncthreads();  // (the arrays are written again)
+    for (int v = 0; v < 4; ++v) {
+      const float2 ml = ml_lds[v][n];
+      total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
     }
+    const float mine = top == best ? 1.0f : __builtin_amdgcn_exp2f((top - best) * p.c);
+    const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
+    if (there)
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < kCell / 4; ++h)
+            sum_lds[wave][n][(pl * P + (4 * quad + i) * kCell) / 4 + h] =
+              make_float4(acc[pl][4 * h][i] * factor, acc[pl][4 * h + 1][i] * factor, acc[pl][4 * h + 2][i] * factor,
+                          acc[pl][4 * h + 3][i] * factor);
+    __syncthreads();
+    // the rows that there are x D / 4 slices
+    const int mine_rows = min(16, rows - row0);
+    for (int item = threadIdx.x; item < mine_rows * (D / 4); item += 256) {
+      const int r = item / (D / 4), slice = item % (D / 4);
+      const int row = row0 + r;
+      float4 v = sum_lds[0][r][slice];
+#pragma unroll
+      for (int k = 1; k < 4; ++k) {
+        const float4 o = sum_lds[k][r][slice];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      const int of_sequence = token_of(row), head = kv_head * p.share + row - of_sequence * p.share;
+      const size_t token = q.start + of_sequence;
+      if (p.parts > 1) {
+        reinterpret_cast<float4*>(p.part_o)[(((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + slice] = v;
+      } else {
+        const half2_t a = {(_Float16)v.x, (_Float16)v.y}, b = {(_Float16)v.z, (_Float16)v.w};
+        reinterpret_cast<u32x2*>(p.out)[((size_t)head * (D / 4) + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
+      }
+    }
+    if (p.parts > 1 && wave == 0 && quad == 0 && there) p.part_ml[((size_t)part * w.tokens + q.start + token) * p.heads + head] = make_float2(best, total);
+    __syncthreads();  // (the arrays are written again)
   }
 }
 
@@ -972,12 +931,12 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
     p.parts = plan.few_parts;
     p.rows_from = 1;
     p.rows_to = plan.few_rows;
-    const int row_tiles = DivUp(std::min(most_new * share, plan.few_rows), 16);
+    const int row_tiles = std::min(DivUp(std::min(most_new * share, plan.few_rows), 16), 16384);  // (more are taken in turn)
     const dim3 grid(p.parts * row_tiles, a.where.kv_heads, a.where.sequences);
     if (a.where.page_shift >= 5)
-      kv4_attention_few_kernel<D, GJ, 1, true><<<grid, 256, 0, stream>>>(p);
+      kv4_attention_few_kernel<D, GJ, true><<<grid, 256, 0, stream>>>(p);
     else
-      kv4_attention_few_kernel<D, GJ, 1, false><<<grid, 256, 0, stream>>>(p);
+      kv4_attention_few_kernel<D, GJ, false><<<grid, 256, 0, stream>>>(p);
   }
   if (plan.few_rows < INT32_MAX) {
     p.parts = plan.many_parts;

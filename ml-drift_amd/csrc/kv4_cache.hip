@@ -257,10 +257,11 @@ void LaunchForm(const Kv4MoveArgs& p, hipStream_t stream) {
   const dim3 grid(DivUp(std::min(p.max_new, p.where.tokens), 4 * (64 * CH / D)), 2 * p.where.kv_heads, p.where.sequences);
   kv4_move_kernel<T, D, CH, READ><<<grid, 256, 0, stream>>>(p);
 }
+constexpr int kFewNew = 8;
 template <typename T, int D, bool READ>
 void LaunchHead(const Kv4MoveArgs& p, hipStream_t stream) {
   // few rows: a lane has one slice, so that a row is spread over as many lanes as it can; else 16 channels (reading: a tile for each wave)
-  if (p.max_new <= 8) {
+  if (p.max_new <= kFewNew) {
     LaunchForm<T, D, 4, READ>(p, stream);
   } else if constexpr (READ) {
     const int tiles = DivUp(std::min(p.max_new, p.where.tokens), kKv4Tile) + 1;
@@ -291,7 +292,7 @@ hipError_t LaunchKv4Append(const Kv4MoveArgs& a, hipStream_t stream, const char*
 }
 
 hipError_t LaunchKv4Read(const Kv4MoveArgs& a, hipStream_t stream, const char** kernel_name) {
-  *kernel_name = "kv4_move_kernel";
+  *kernel_name = a.max_new <= kFewNew ? "kv4_move_kernel" : "kv4_read_tiles_kernel";
   if (a.f16)
     LaunchTyped<__half, true>(a, stream);
   else

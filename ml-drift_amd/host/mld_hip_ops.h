@@ -278,6 +278,54 @@ inline Status CreateConvInt8WithDequantization(DataType dst_type, const OHWI& we
   return {};
 }
 
+// Between the q / k / v projections and the o projection (no counterparts in the reference's FullyConnected path; include/mldhip.h:
+// arithmetic, layouts, objects).  Norms of the query and key heads and the rotation by position; `frequencies` as for
+// mldhip_qk_norm_rope_desc (read here, need not outlive the call).
+struct QkNormRopeAttributes {
+  int heads = 0, kv_heads = 0, head_dim = 0, rotary_dim = 0;
+  double base = 10000.0;
+  const double* frequencies = nullptr;
+  bool interleaved = false;
+  bool norm = false;
+  float eps = 1e-6f, weight_offset = 0.0f;
+};
+inline Status CreateQkNormRope(DataType tensor_type, const QkNormRopeAttributes& attr, int max_tokens, HipOperation* result) {
+  const mldhip_qk_norm_rope_desc d{(int)tensor_type, attr.heads, attr.kv_heads, attr.head_dim, attr.rotary_dim, attr.base, attr.frequencies,
+                                   attr.interleaved, attr.norm, attr.eps, attr.weight_offset, max_tokens};
+  mldhip_op* op = nullptr;
+  const int rc = mldhip_qk_norm_rope_create(&d, &op);
+  if (rc != MLDHIP_OK) return Status::FromCode(rc);
+  *result = HipOperation(op);
+  return {};
+}
+
+// The key / value cache of 4-bit codes in pages, and the ops over it.
+using Kv4Cache = mldhip_kv4_cache_desc;
+inline Status GetKv4CacheBytes(const Kv4Cache& cache, size_t* bytes) { return Status::FromCode(mldhip_kv4_cache_bytes(&cache, bytes)); }
+inline Status CreateKv4Append(const Kv4Cache& cache, DataType src_type, int max_tokens, int max_new_tokens, HipOperation* result) {
+  mldhip_op* op = nullptr;
+  const int rc = mldhip_kv4_append_create(&cache, (int)src_type, max_tokens, max_new_tokens, &op);
+  if (rc != MLDHIP_OK) return Status::FromCode(rc);
+  *result = HipOperation(op);
+  return {};
+}
+inline Status CreateKv4Read(const Kv4Cache& cache, DataType dst_type, int max_tokens, int max_new_tokens, HipOperation* result) {
+  mldhip_op* op = nullptr;
+  const int rc = mldhip_kv4_read_create(&cache, (int)dst_type, max_tokens, max_new_tokens, &op);
+  if (rc != MLDHIP_OK) return Status::FromCode(rc);
+  *result = HipOperation(op);
+  return {};
+}
+inline Status CreateKv4Attention(const Kv4Cache& cache, int heads, float scale, bool causal, int window, int max_tokens,
+                                 int max_new_tokens, HipOperation* result) {
+  const mldhip_kv4_attention_desc d{cache, heads, scale, causal, window, max_tokens, max_new_tokens};
+  mldhip_op* op = nullptr;
+  const int rc = mldhip_kv4_attention_create(&d, &op);
+  if (rc != MLDHIP_OK) return Status::FromCode(rc);
+  *result = HipOperation(op);
+  return {};
+}
+
 // One launch for FullyConnected nodes that read the same tensor (q/k/v, gate/up); the caller
 // falls back to AddToQueue per node when the status is FAILED_PRECONDITION.
 inline Status AddToQueueFused(const std::vector<HipOperation*>& ops, void* hip_stream) {

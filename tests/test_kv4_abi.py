@@ -153,3 +153,25 @@ def test_the_arithmetic_that_the_gpu_tests_check_against():
     widest = kept(np.array([[1e9, -1e9] + [0.0] * 30]), 32)
     assert np.isfinite(widest.astype(np.float16)).all() and abs(widest[0, 0] - 57344) < 8000
     assert not kept(np.full((1, 32), np.nan), 32).any()
+
+
+def test_sizes_past_what_a_launch_can_count_are_refused():
+    for create in creators():
+        refused(M.OUT_OF_RANGE, create, cache(head_dim=256, group_size=32, page_size=1024, pages=(1 << 31) - 1, kv_heads=32767))  # 2^64 and more
+        refused(M.OUT_OF_RANGE, create, cache(page_size=1024, pages=1 << 28, kv_heads=128))
+    most = 1 << 24
+    for create in (M.kv4_append_create, M.kv4_read_create):
+        create(cache(), M.FLOAT16, most)
+        refused(M.OUT_OF_RANGE, create, cache(), M.FLOAT16, most + 1)
+    refused(M.OUT_OF_RANGE, M.kv4_attention_create, cache(), 2, max_tokens=most + 1)
+    M.qk_norm_rope_create(M.FLOAT16, 8, 2, 128, max_tokens=most)
+    refused(M.OUT_OF_RANGE, M.qk_norm_rope_create, M.FLOAT16, 8, 2, 128, max_tokens=most + 1)
+
+
+def test_attention_into_its_own_queries_is_refused():
+    op = M.kv4_attention_create(cache(), 8, max_tokens=4)
+    op.set_shape(1, 1, 4)
+    for i, n in enumerate([8 * 128 * 4 * 2, M.kv4_cache_bytes(cache()), 3 * 4 * 4, 3 * 4, 4 * 4]):
+        op.set_src_raw(i, 4096 * (i + 1), n)
+    op.set_dst_raw(0, 4096, 8 * 128 * 4 * 2)
+    assert "src_q" in refused(M.INVALID_ARGUMENT, op.launch)
