@@ -2,13 +2,16 @@
 gated MLP 16384, int4 group-32 weights, fp16 tensors), as the reference's model builder emits
 it per layer (samples/llm/gemma3_model_builder.cc:1115-1128): q, k, v, o, gate, up, down.
 
-Only the FCs are reproduced (no attention, norm or activation): every FC reads a synthetic
+DecoderStack reproduces the FCs only (no attention, norm or activation): every FC reads a synthetic
 N(0,1) activation tensor of its input width and writes its own output tensor, and the FCs run
 in the graph's order on one stream, i.e. with the dependencies of the real layer.  Every FC of
 every layer has weights and scales of its own (seed layer * 7 + index), so a decode step streams
 the whole stack's 1.1 GB through HBM.  (What a GEMV or GEMM costs does not depend on the values of
 its activations, so the synthetic inputs time like the fed-forward ones; the chain with the values
 flowing through it is a parity test.)
+
+AttentionBlock is the attention of such a layer with the values flowing through it: q / k / v, the norms of the
+heads and the rotation, the new keys and values into a paged cache of 4-bit codes, attention over it, o.
 
 Nothing here computes a result on the host.
 """
@@ -175,3 +178,79 @@ class DecoderStack:
 
     def kernel_names(self):
         return [op.kernel_name for _, _, op, _, _, _ in self.nodes]
+
+
+class AttentionBlock:
+    """q / k / v -> norms and rotation -> cache -> attention -> o, five or six ops on one stream over ragged batches of `sequences`
+    sequences: prompts, chunks of prompts and single tokens alike.  set_batch() says which rows are whose and rebinds; launch() neither
+    allocates nor synchronises and may be captured, and page_table, lengths, starts and positions may be rewritten between replays.
+    The cache has `pages` pages, of which the caller gives each sequence its own in page_table."""
+
+    def __init__(self, heads=8, kv_heads=1, head_dim=256, hidden=2048, sequences=1, max_tokens=128, max_new_tokens=None, pages=64,
+                 pages_per_sequence=None, page_size=64, group_size=32, window=0, base=10000.0, seed=5, device="cuda"):
+        import torch
+        self.torch = torch
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.max_tokens = max_tokens
+        most_new = max_tokens if max_new_tokens is None else max_new_tokens
+        self.desc = M.kv4_cache_desc(kv_heads, head_dim, group_size, page_size, pages, sequences, pages_per_sequence or pages)
+        self.cache = torch.zeros(M.kv4_cache_bytes(self.desc), dtype=torch.uint8, device=device)
+        ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)
+        self.page_table, self.lengths = ints(sequences, self.desc.pages_per_sequence), ints(sequences)
+        self.starts, self.positions = ints(sequences + 1), ints(max_tokens)
+        rng = np.random.default_rng(seed)
+        self.norms = [torch.from_numpy(rng.uniform(0.5, 1.5, head_dim).astype(np.float16)).to(device) for _ in range(2)]
+        width = heads * head_dim
+        self.cases, self.fc, self._weights, self._buffers = [], [], [], {}
+        for i, (name, k, n) in enumerate([("q", hidden, width), ("k", hidden, kv_heads * head_dim), ("v", hidden, kv_heads * head_dim),
+                                          ("o", width, hidden)]):
+            case = W.make_fc_case(seed=seed * 7 + i, m=1, k=k, n=n, weight_bits=4, tensor_dtype=np.float16, groups=k // 32)
+            case["name"] = name
+            desc, w = W.pack_fc_weights(case)
+            sc = M.scale_to_tensor(case["scale"], M.FLOAT16).view(np.float16)
+            self._weights.append((torch.from_numpy(w).to(device), torch.from_numpy(sc).to(device)))
+            self.fc.append(M.fc_create(M.PRECISION_F32_F16, M.FLOAT16, M.FLOAT16, n, k, desc, scale_shape=(n, case["groups"]),
+                                       max_tokens=max_tokens))
+            self.cases.append(case)
+        for name, channels in [("x", hidden), ("q", width), ("k", kv_heads * head_dim), ("v", kv_heads * head_dim), ("attended", width),
+                               ("out", hidden)]:
+            self._buffers[name] = torch.zeros(channels * max_tokens, dtype=torch.float16, device=device)
+        self.rope = M.qk_norm_rope_create(M.FLOAT16, heads, kv_heads, head_dim, base=base, norm=True, max_tokens=max_tokens)
+        self.append = M.kv4_append_create(self.desc, M.FLOAT16, max_tokens, most_new)
+        self.attend = M.kv4_attention_create(self.desc, heads, window=window, max_tokens=max_tokens, max_new_tokens=most_new)
+
+    def set_batch(self, page_table, lengths, starts, tokens=None):
+        """page_table [sequences][pages_per_sequence], lengths and starts as the ops over the cache take them (lengths count the new
+        tokens).  tokens: rows of the tensors, starts[-1] unless given (padded batches)."""
+        torch = self.torch
+        lengths, starts = np.asarray(lengths, np.int32), np.asarray(starts, np.int32)
+        tokens = int(starts[-1]) if tokens is None else tokens
+        assert 1 <= tokens <= self.max_tokens
+        positions = np.zeros(self.max_tokens, np.int32)
+        for s, length in enumerate(lengths):
+            positions[starts[s]:starts[s + 1]] = np.arange(length - (starts[s + 1] - starts[s]), length)
+        for to, values in ((self.page_table, page_table), (self.lengths, lengths), (self.starts, starts), (self.positions, positions)):
+            to.copy_(torch.from_numpy(np.ascontiguousarray(values, np.int32)))
+        self.tokens = tokens
+        view = lambda name: self._buffers[name][:self._buffers[name].numel() // self.max_tokens * tokens].view(-1, tokens, 4)
+        self.x, self.q, self.k, self.v, self.attended, self.out = [view(n) for n in ("x", "q", "k", "v", "attended", "out")]
+        where = [self.page_table, self.lengths, self.starts]
+        for op, src, dst, weights in zip(self.fc, (self.x, self.x, self.x, self.attended), (self.q, self.k, self.v, self.out), self._weights):
+            op.bind([src, *weights], [dst])
+        self.rope.bind([self.q, self.k, self.positions, *self.norms], [self.q, self.k])
+        self.append.bind([self.k, self.v, *where], [self.cache])
+        self.attend.bind([self.q, self.cache, *where], [self.attended])
+        for op in (*self.fc, self.rope, self.append, self.attend):
+            op.set_shape(1, 1, tokens)
+
+    def launch(self, stream=None):
+        s = self.torch.cuda.current_stream().cuda_stream if stream is None else stream
+        try:
+            M.fc_launch_fused(self.fc[:3], s)
+        except M.MldhipError as e:
+            if e.code != M.FAILED_PRECONDITION:
+                raise
+            for op in self.fc[:3]:
+                op.launch(s)
+        for op in (self.rope, self.append, self.attend, self.fc[3]):
+            op.launch(s)

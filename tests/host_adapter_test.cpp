@@ -194,6 +194,33 @@ int main() {
   }
   // a gated launch over unbound ops is refused before anything reaches the GPU
   EXPECT(AddToQueueGated(&fc, &fc, GateActivation::kSilu, nullptr, 0, nullptr).code == MLDHIP_INVALID_ARGUMENT);
+
+  // between the projections: created, bound by name and shaped without a GPU
+  {
+    HipOperation op;
+    QkNormRopeAttributes rope;
+    rope.heads = 8;
+    rope.kv_heads = 1;
+    rope.head_dim = rope.rotary_dim = 256;
+    EXPECT(CreateQkNormRope(DataType::kFloat16, rope, 4, &op).ok());
+    EXPECT(op.GetSrcTensorsNames().size() == 3 && op.GetSrcTensorsNames()[2] == "positions" && op.GetDstTensorsNames()[1] == "dst_k");
+    rope.norm = true;
+    EXPECT(CreateQkNormRope(DataType::kFloat32, rope, 4, &op).ok() && op.GetSrcTensorsNames().size() == 5);
+    rope.rotary_dim = 12;
+    EXPECT(CreateQkNormRope(DataType::kFloat16, rope, 4, &op).code == MLDHIP_INVALID_ARGUMENT);
+    Kv4Cache cache{/*kv_heads=*/1, /*head_dim=*/256, /*group_size=*/32, /*page_size=*/64, /*pages=*/10, /*sequences=*/2, /*pages_per_sequence=*/5};
+    size_t bytes = 0;
+    EXPECT(GetKv4CacheBytes(cache, &bytes).ok() && bytes == (size_t)10 * 64 * (256 + 4 * 8));
+    EXPECT(CreateKv4Append(cache, DataType::kFloat16, 4, 2, &op).ok() && op.GetDstTensorsNames()[0] == "cache");
+    EXPECT(CreateKv4Read(cache, DataType::kFloat32, 4, 2, &op).ok() && op.GetSrcTensorsNames()[0] == "cache");
+    EXPECT(CreateKv4Attention(cache, 8, 0.0625f, true, 0, 4, 2, &op).ok() && op.GetSrcTensorsNames()[4] == "starts");
+    EXPECT(op.UpdateParams(BHWC{1, 1, 4, 2048}).ok());
+    EXPECT(op.UpdateParams(BHWC{1, 1, 5, 2048}).code == MLDHIP_OUT_OF_RANGE);
+    EXPECT(CreateKv4Attention(cache, 8, 0.0f, true, 0, 4, 2, &op).code == MLDHIP_INVALID_ARGUMENT);
+    cache.page_size = 48;
+    EXPECT(GetKv4CacheBytes(cache, &bytes).code == MLDHIP_INVALID_ARGUMENT);
+    EXPECT(CreateKv4Append(cache, DataType::kFloat16, 4, 2, &op).code == MLDHIP_INVALID_ARGUMENT);
+  }
   std::printf("host adapter ok\n");
   return 0;
 }
