@@ -511,9 +511,14 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     uint32_t keys[kKeyRegs], values[kValueRegs], key_words[kGroups];
     u32x2 value_words[kPlanes];
     bool there = false;
+    // The page of a step is looked up with the bytes of the step before: a wave would wait for it.  By a vector load, in order with these:
+    // scalar ones would be waited for with the next operands from LDS.
+    int zero = 0, looked_up = 0;
+    asm volatile("" : "+v"(zero));
+    auto look_up = [&](int step) { looked_up = table[zero + (min(step * kWaves + wave, (q.held - 1) >> 4) * 16 >> w.page_shift)]; };
     auto load = [&](int step) {
       const int tile = min(step * kWaves + wave, (q.held - 1) >> 4);
-      const int id = table[tile * 16 >> w.page_shift];
+      const int id = __builtin_amdgcn_readfirstlane(looked_up);
       there = id >= 0 && id < w.pages;
       const uint8_t* block = p.cache + ((size_t)(there ? id : 0) * w.kv_heads + kv_head) * w.block_bytes;
       const int in_page = (tile * 16) & (page_tokens - 1);
@@ -538,6 +543,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl)
         value_words[pl] = *reinterpret_cast<const u32x2*>(vw + 16 * ((pl * P + n * kCell) / (32 * GJ)) + 4 * quad);
+      look_up(step + 1);
     };
     // what lies behind the held positions may be anything: it is made 0 (0 * NaN would not be)
     auto clear = [&](int step, int buffer) {
@@ -596,7 +602,10 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
         }
     };
 
-    if (begin < end) load(begin);
+    if (begin < end) {
+      look_up(begin);
+      load(begin);
+    }
 
     const int wave_row = row0 + wave * 32, row = wave_row + col;
     const bool is_row = row < rows;
@@ -607,12 +616,8 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     {
       const u32x2* src = reinterpret_cast<const u32x2*>(p.q) + ((size_t)head * (D / 4) + 2 * half) * w.tokens + token;
 #pragma unroll
-      for (int k = 0; k < kQ; ++k) {
-        u32x2 a = {0u, 0u}, b = {0u, 0u};
-        if (is_row) {
-          a = src[(size_t)(4 * k) * w.tokens];
-          b = src[(size_t)(4 * k + 1) * w.tokens];
-        }
+      for (int k = 0; k < kQ; ++k) {  // (behind the last row: the first one again)
+        const u32x2 a = src[(size_t)(4 * k) * w.tokens], b = src[(size_t)(4 * k + 1) * w.tokens];
         qa[k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
                       __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
       }
@@ -692,11 +697,13 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           const float higher = fmaxf(top, best);
           const float down = top == higher ? 1.0f : __builtin_amdgcn_exp2f((top - higher) * p.c);
           top = higher;
-          sum *= down;
+          if (__any(sum != 0.0f)) {  // (not the first of the positions: nothing to scale)
+            sum *= down;
 #pragma unroll
-          for (int j = 0; j < kTilesD; ++j)
+            for (int j = 0; j < kTilesD; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[j][i] *= down;
+              for (int i = 0; i < 16; ++i) acc[j][i] *= down;
+          }
         }
         settle();
         const float base = top == -INFINITY ? 0.0f : kManyLift - top * p.c;
@@ -788,26 +795,30 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     if (is_row) {
       const float factor = p.parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
-      u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
-      float4* part_to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + half * kCell;
+      auto store = [&](auto to) {  // to(slice behind the half's own first, its 4 channels)
 #pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl)
+        for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
-        for (int m = 0; m < 8; ++m)  // cells 8 (m / 4) + 4 half + m % 4
+          for (int m = 0; m < 8; ++m)  // cells 8 (m / 4) + 4 half + m % 4
 #pragma unroll
-          for (int h = 0; h < kCell / 4; ++h) {
-            float v[4];
+            for (int h = 0; h < kCell / 4; ++h) {
+              float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
-            const int slice = (pl * P + (8 * (m / 4) + m % 4) * kCell) / 4 + h;  // behind the half's own first
-            if (p.parts > 1) {
-              part_to[slice] = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-              const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
-              to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
+              for (int e = 0; e < 4; ++e) v[e] = acc[pl * (kCell / 2) + (4 * h + e) / 2][8 * (e % 2) + m] * factor;
+              to((pl * P + (8 * (m / 4) + m % 4) * kCell) / 4 + h, v);
             }
-          }
-      if (p.parts > 1 && half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
+      };
+      if (p.parts > 1) {
+        float4* to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + half * kCell;
+        store([&](int slice, const float(&v)[4]) { to[slice] = make_float4(v[0], v[1], v[2], v[3]); });
+        if (half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
+      } else {
+        u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
+        store([&](int slice, const float(&v)[4]) {
+          const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
+          to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
+        });
+      }
     }
   }
 }
