@@ -602,10 +602,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
         }
     };
 
-    if (begin < end) {
-      look_up(begin);
-      load(begin);
-    }
+    if (begin < end) look_up(begin);
 
     const int wave_row = row0 + wave * 32, row = wave_row + col;
     const bool is_row = row < rows;
@@ -622,6 +619,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
                       __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
       }
     }
+    if (begin < end) load(begin);  // (behind the rows' own loads: these wait for no page)
     // what all of the wave's rows see, and what any of them does
     const int wave_first = q.first + min(wave_row, rows - 1) / p.share, wave_last = q.first + min(wave_row + 31, rows - 1) / p.share;
     const int all_hi = p.causal ? min(q.held, wave_first + 1) : q.held, all_lo = p.window > 0 ? max(0, wave_last + 1 - p.window) : 0;
@@ -986,13 +984,17 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   // take anyway; else a work-group of the other kernel each, beside the prompts', costs less than one more launch.
   const long long seen = a.window > 0 ? std::min<long long>(keys, a.window) : keys;
   plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && share <= kFewRows && (heads >= 64 || seen > 4096) ? kFewRows : 0;
+  // tiles of rows in a batch: sequences of the most rows, but no more rows than the tensors have
+  const auto row_tiles = [&](long long most, int tile) {
+    return std::min(heads * ((most + tile - 1) / tile), a.where.kv_heads * ((long long)a.max_tokens * share / tile + a.where.sequences));
+  };
   // the parts' outputs: at most 256 MB
   const long long row_bytes = (long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4, room = ((long long)256 << 20) / row_bytes;
   const auto parts = [&](long long v) { return (int)std::max(1LL, std::min({v, room, (long long)kMostParts})); };
   if (plan.few_rows > 0) {
     // as many work-groups as are on the chip at once (32 sequences of up to 4096 positions, 8 key heads of 128: 33.9 us in 2 parts, 31.8 in 3,
     // 34.6 in 4), each with at least a step for each of its waves
-    const long long groups = heads * (((many ? std::min<long long>(rows, kFewRows) : rows) + 15) / 16);
+    const long long groups = row_tiles(many ? std::min<long long>(rows, kFewRows) : rows, 16);
     const long long slots = a.head_dim == 64 ? 1024 : a.head_dim == 128 ? 768 : 512;
     plan.few_parts = parts(std::min(t.kv4_parts > 0 ? t.kv4_parts : slots / groups, (keys + 127) / 128));
   }
@@ -1000,13 +1002,13 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
     // Parts level the work-groups' shares, and their outputs go through memory: the number with the least estimated time.  Steps that the
     // longest work-group takes, and those that each of the 256 takes where they are level; a step and a byte by what they measured.
     const int step = 16 * ManyWaves(a.head_dim), tile = 32 * ManyWaves(a.head_dim);
-    const double step_us = a.head_dim == 64 ? 2.7 : a.head_dim == 128 ? 3.7 : 2.6;
-    const double groups = (double)heads * ((rows + tile - 1) / tile), longest = std::max<double>(1, (double)(a.window > 0 ? std::min<long long>(keys, a.window + tile / share) : keys) / step);
+    const double step_us = a.head_dim == 64 ? 2.7 : a.head_dim == 128 ? 3.7 : 2.6, around_us = 10;  // (before the first step and behind the last)
+    const double groups = (double)row_tiles(rows, tile), longest = std::max<double>(1, (double)(a.window > 0 ? std::min<long long>(keys, a.window + tile / share) : keys) / step);
     const double level = groups * longest / 256 * (a.window > 0 || !a.causal ? 1.0 : 1.0 - 0.5 * std::min<double>(1, (double)most_new / keys));
     double least = 0;
     for (int n = 1; n <= kMostParts && n <= std::max(1.0, longest / 2); ++n) {
       const double steps = groups * n <= 256 ? longest / n : level + 0.5 * longest / n;
-      const double us = steps * step_us + (n > 1 ? 5 + 2 * n * (double)row_bytes / 4.5e6 : 0);
+      const double us = steps * step_us + around_us * std::max(1.0, groups * n / 256) + (n > 1 ? 5 + 2 * n * (double)row_bytes / 4.5e6 : 0);
       if (n > 1 && us >= least) continue;
       least = us;
       plan.many_parts = n;
