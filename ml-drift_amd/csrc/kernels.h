@@ -281,7 +281,7 @@ hipError_t LaunchKv4Read(const Kv4MoveArgs& a, hipStream_t stream, const char** 
 // keys of a sequence: chosen when an op is created.
 struct Kv4AttentionPlan {
   int few_rows = 0;  // sequences of up to this many rows (new tokens x heads of a key head) go to the kernel for few rows
-  int few_parts = 1, many_parts = 1;
+  int few_parts = 1, few_waves = 4, many_parts = 1;  // (few_waves: of a work-group)
 };
 struct Kv4AttentionArgs {
   Kv4Where where;

@@ -128,8 +128,11 @@ __device__ __forceinline__ uint32_t OfRow(uint32_t v, int from) {  // (`from` is
   }
 }
 
-template <int D, int GJ, bool BIG>
-__global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_attention_few_kernel(const AttendParams p) {
+// Waves on a SIMD, as many as their registers allow.
+constexpr int FewOnSimd(int head_dim) { return head_dim == 256 ? 2 : head_dim == 128 ? 3 : 4; }
+
+template <int D, int GJ, int WAVES, bool BIG>
+__global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_kernel(const AttendParams p) {
   using S = FewShape<D, GJ>;
   constexpr int P = S::P, kPlanes = S::kPlanes, kCell = S::kCell, kGroups = S::kGroups, kKeyRegs = S::kKeyRegs, kTiles = S::kTiles, kStep = S::kStep;
   const Kv4Where& w = p.w;
@@ -145,8 +148,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
   const Kv4Sequence q = Kv4SequenceOf(w, s);
   const int rows = q.count * p.share;
   if (rows < p.rows_from || rows > p.rows_to) return;
-  __shared__ float4 sum_lds[4][16][D / 4 + 1];
-  __shared__ float2 ml_lds[4][16];
+  __shared__ float4 sum_lds[WAVES][16][D / 4 + 1];
+  __shared__ float2 ml_lds[WAVES][16];
   const Unpack unpack;
   const uint32_t key_at = (n * 4 + quad) * (P / 8), value_at = (quad * 16 + n) * (2 * kCell);  // a lane's piece of a tile's codes
   const uint32_t value_word_at = 32 * (n * kCell / (32 * GJ)) + 8 * quad;
@@ -235,7 +238,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
       ids = look_up(begin);
       load_keys(begin, ids, c);
       load_values(begin, ids, c);
-      ids_next = look_up(min(begin + 4, end - 1));
+      ids_next = look_up(min(begin + WAVES, end - 1));
     }
 
     u32x4 qa[kKeyRegs];  // operands of the first product: channel s and channel s + 4 of 8 in each register
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
 #pragma unroll
       for (int j = 0; j < kCell; ++j) acc[pl][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (int step = begin; step < end; step += 4) {
+    for (int step = begin; step < end; step += WAVES) {
       // scores: score[u][i] = q . k of row n and position 16 u + 4 quad + i
       float score[kTiles][4];
       if constexpr (kGroups == 8) {  // (what the sums start from, four times each, would stay in 32 registers over the loop)
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
         for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(score[u][i]));
       }
       // (the next step's keys come while this one's values are taken, and the other way round)
-      if (step + 4 < end) load_keys(step + 4, ids_next, c);
+      if (step + WAVES < end) load_keys(step + WAVES, ids_next, c);
       __builtin_amdgcn_sched_barrier(0);
       // a step inside what every row sees, on pages that there are, needs no masks
       bool whole = step * kStep + kStep <= (p.causal ? min(q.held, first_row + 1) : q.held);
@@ -409,9 +412,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
             }
         }
       }
-      if (step + 4 < end) load_values(step + 4, ids_next, c);
+      if (step + WAVES < end) load_values(step + WAVES, ids_next, c);
       ids = ids_next;
-      ids_next = look_up(min(step + 8, end - 1));
+      ids_next = look_up(min(step + 2 * WAVES, end - 1));
       __builtin_amdgcn_sched_barrier(0);
     }
 
@@ -421,9 +424,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
     __syncthreads();
     float best = -INFINITY, total = 0.0f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) best = fmaxf(best, ml_lds[v][n].x);
+    for (int v = 0; v < WAVES; ++v) best = fmaxf(best, ml_lds[v][n].x);
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < WAVES; ++v) {
       const float2 ml = ml_lds[v][n];
       total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
     }
@@ -442,12 +445,12 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) void kv4_atte
     __syncthreads();
     // the rows that there are x D / 4 slices
     const int mine_rows = min(16, rows - row0);
-    for (int item = threadIdx.x; item < mine_rows * (D / 4); item += 256) {
+    for (int item = threadIdx.x; item < mine_rows * (D / 4); item += 64 * WAVES) {
       const int r = item / (D / 4), slice = item % (D / 4);
       const int row = row0 + r;
       float4 v = sum_lds[0][r][slice];
 #pragma unroll
-      for (int k = 1; k < 4; ++k) {
+      for (int k = 1; k < WAVES; ++k) {
         const float4 o = sum_lds[k][r][slice];
         v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
       }
@@ -942,10 +945,12 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
     p.rows_to = plan.few_rows;
     const int row_tiles = std::min(DivUp(std::min(most_new * share, plan.few_rows), 16), 16384);  // (more are taken in turn)
     const dim3 grid(p.parts * row_tiles, a.where.kv_heads, a.where.sequences);
-    if (a.where.page_shift >= 5)
-      kv4_attention_few_kernel<D, GJ, true><<<grid, 256, 0, stream>>>(p);
+    constexpr int kFull = 4 * FewOnSimd(D);
+    const bool big = a.where.page_shift >= 5;
+    if (plan.few_waves == kFull)
+      big ? kv4_attention_few_kernel<D, GJ, kFull, true><<<grid, 64 * kFull, 0, stream>>>(p) : kv4_attention_few_kernel<D, GJ, kFull, false><<<grid, 64 * kFull, 0, stream>>>(p);
     else
-      kv4_attention_few_kernel<D, GJ, false><<<grid, 256, 0, stream>>>(p);
+      big ? kv4_attention_few_kernel<D, GJ, 4, true><<<grid, 256, 0, stream>>>(p) : kv4_attention_few_kernel<D, GJ, 4, false><<<grid, 256, 0, stream>>>(p);
   }
   if (plan.few_rows < INT32_MAX) {
     p.parts = plan.many_parts;
@@ -992,11 +997,15 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   const long long row_bytes = (long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4, room = ((long long)256 << 20) / row_bytes;
   const auto parts = [&](long long v) { return (int)std::max(1LL, std::min({v, room, (long long)kMostParts})); };
   if (plan.few_rows > 0) {
-    // as many work-groups as are on the chip at once (32 sequences of up to 4096 positions, 8 key heads of 128: 33.9 us in 2 parts, 31.8 in 3,
-    // 34.6 in 4), each with at least a step for each of its waves
     const long long groups = row_tiles(many ? std::min<long long>(rows, kFewRows) : rows, 16);
-    const long long slots = a.head_dim == 64 ? 1024 : a.head_dim == 128 ? 768 : 512;
-    plan.few_parts = parts(std::min(t.kv4_parts > 0 ? t.kv4_parts : slots / groups, (keys + 127) / 128));
+    // Work-groups of all the waves that a CU holds where they fill the CUs and each wave has a step: fewer outputs to join, none with as many
+    // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 30.5 us against 31.8 in 3 parts of 4 waves; 16 of up to 2047,
+    // four tokens each, 16 heads of 64: 16.9 against 17.8 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of
+    // 1000 positions, a key head of 256: 11.9 us against 12.8).
+    const int full = 4 * FewOnSimd(a.head_dim), waves = 256 * full;  // of a CU; of the chip
+    plan.few_waves = groups <= 256 && 256 / groups * groups >= 192 && 256 / groups * 32 * full <= keys ? full : 4;
+    plan.few_parts = parts(t.kv4_parts > 0 ? std::min<long long>(t.kv4_parts, (keys + 127) / 128)
+                                             : std::min(waves / plan.few_waves / groups, (keys + 32 * plan.few_waves - 1) / (32 * plan.few_waves)));
   }
   if (many) {
     // Parts level the work-groups' shares, and their outputs go through memory: the number with the least estimated time.  Steps that the
@@ -1022,7 +1031,7 @@ hipError_t LaunchKv4Attention(const Kv4AttentionArgs& a, hipStream_t stream, con
   const bool many = a.plan.few_rows < INT32_MAX;
   *kernel_name = many ? "kv4_attention_many_kernel" : "kv4_attention_few_kernel";
   SetVariant(a.variant, !many ? "few" : a.plan.few_rows > 0 ? "many, few" : "many");
-  SetTiles(a.tiles, many ? 32 * ManyWaves(a.head_dim) : 16, many ? ManyWaves(a.head_dim) : 4, many ? a.plan.many_parts : a.plan.few_parts);
+  SetTiles(a.tiles, many ? 32 * ManyWaves(a.head_dim) : 16, many ? ManyWaves(a.head_dim) : a.plan.few_waves, many ? a.plan.many_parts : a.plan.few_parts);
   const int gj = 1 << (a.where.group_shift - 5);
   if (a.head_dim == 64)
     gj == 1 ? Launch<64, 1>(a, stream) : Launch<64, 2>(a, stream);

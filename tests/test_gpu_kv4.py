@@ -393,6 +393,18 @@ def test_attention_shares_over_many_sequences(parts):
             check_attention(unslices(out.cpu().numpy(), 64), exact, largest, score)
 
 
+@pytest.mark.parametrize("head_dim,group,page", [(64, 32, 16), (64, 64, 64), (128, 32, 16), (128, 128, 32), (256, 64, 16), (256, 128, 64)])
+@pytest.mark.parametrize("sequences,kv_heads,parts", [(16, 16, 1), (8, 8, 4)])
+def test_attention_by_work_groups_of_whole_compute_units(head_dim, group, page, sequences, kv_heads, parts):
+    """As many tiles as compute units, or a share of them: all the waves of a unit take one tile's keys."""
+    waves = {64: 16, 128: 12, 256: 8}[head_dim]
+    most = parts * 32 * waves
+    lengths = [1 + (most + 40) * i // (sequences - 1) for i in range(sequences)]
+    counts = [min(l, 1 + i % 2) for i, l in enumerate(lengths)]
+    d = attention_case(kv_heads, 3, head_dim, group, page, counts, lengths, window=most // 2 if page == 32 else 0, behind=1, seed=head_dim + parts)
+    assert d.op.kernel_variant == "few" and d.op.kernel_tiles == (16, waves, parts)
+
+
 def test_attention_of_more_than_a_thousand_sequences():
     attention_case(2, 2, 64, 64, 16, [1] * 1100, [1 + i % 40 for i in range(1100)], seed=6)
 
