@@ -824,10 +824,9 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
   }
 }
 
-// The parts of each row, joined.  A row per work-group of WAVES waves, whose threads share its slices and, in turn, its parts: four waves
-// where parts are many, one where they are few.  Everything is asked for before the first wait (the loads of the parts' outputs do not depend
-// on their sums), and nothing is looked up but where the first sequence begins and the last one ends; where both kernels above have a share
-// of the batch, sequence by sequence, those of one kernel only.
+// The parts of each row, joined: everything is asked for before the first wait (the loads of the parts' outputs do not depend on their
+// sums), and nothing is looked up but where the first sequence begins and the last one ends; where both kernels above have a share of the
+// batch, sequence by sequence, those of one kernel only.
 struct JoinParams {
   Kv4Where w;
   const float* part_o;
@@ -839,88 +838,127 @@ struct JoinParams {
 };
 constexpr int kMostParts = 256, kFewParts = 8;
 constexpr int kFewRows = 32;  // rows of a sequence up to which the kernel for few rows serves it where there are more in a batch
-template <int D, int WAVES, bool BY_SEQUENCE>
+
+// Of a part the weight in a row whose largest maximum is `best`: 0 where it saw nothing, whatever its output holds.
+__device__ __forceinline__ float PartFactor(float2 ml, float best, float c) {
+  return ml.y == 0.0f ? 0.0f : ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * c);
+}
+__device__ __forceinline__ u32x2 Joined(const float4& v, float total) {
+  const float g = total == 0.0f ? 0.0f : 1.0f / total;
+  const half2_t a = {(_Float16)(v.x * g), (_Float16)(v.y * g)}, b = {(_Float16)(v.z * g), (_Float16)(v.w * g)};
+  return u32x2{AsU32(a), AsU32(b)};
+}
+
+// Few parts: a work-group takes 8 neighbouring tokens of one head, so that stores are runs of 64 bytes and loads of 128; a thread has one
+// token, and one or two slices in all parts.
+template <int D, bool BY_SEQUENCE>
 __global__ __launch_bounds__(256) void kv4_attention_join_kernel(const JoinParams p) {
-  constexpr int kSlices = D / 4, kTurns = 64 * WAVES / kSlices, kFirst = 4;
+  constexpr int kSlices = D / 4, kTokens = 8, kThreads = D == 64 ? 128 : 256, kItems = kTokens * kSlices / kThreads;
   const Kv4Where& w = p.w;
-  const int thread = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, slice = thread % kSlices, turn = thread / kSlices;
-  const size_t step = (size_t)w.tokens * p.heads;
-  size_t row = WAVES == 1 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int block = blockIdx.x / p.heads, head = blockIdx.x - block * p.heads;
+  int token = block * kTokens + threadIdx.x % kTokens;
   if constexpr (BY_SEQUENCE) {
     const Kv4Sequence q = Kv4SequenceOf(w, blockIdx.y);
     const int rows = q.count * p.share;
-    if (rows < p.rows_from || rows > p.rows_to || row >= (size_t)q.count * p.heads) return;
+    if (rows < p.rows_from || rows > p.rows_to || token >= q.count) return;
+    token += q.start;
+  }
+  if (token >= w.tokens) return;
+  const size_t rows = (size_t)w.tokens * p.heads, row = (size_t)token * p.heads + head;
+  const int slice0 = threadIdx.x / kTokens;
+  const float4* from = reinterpret_cast<const float4*>(p.part_o) + row * kSlices + slice0;
+  float2 ml[kFewParts];
+  float4 o[kFewParts][kItems];
+#pragma unroll
+  for (int k = 0; k < kFewParts; ++k)
+    if (k < p.parts) {
+      ml[k] = p.part_ml[k * rows + row];
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) o[k][i] = from[k * rows * kSlices + i * (kThreads / kTokens)];
+    }
+  if (!BY_SEQUENCE && (token < w.starts[0] || token >= w.starts[w.sequences])) return;  // of no sequence
+  float best = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kFewParts; ++k)
+    if (k < p.parts) best = fmaxf(best, ml[k].x);
+  float total = 0.0f;
+  float4 v[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int k = 0; k < kFewParts; ++k)
+    if (k < p.parts) {
+      const float f = PartFactor(ml[k], best, p.c);
+      total += ml[k].y * f;
+      if (f != 0.0f)
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) v[i].x += o[k][i].x * f, v[i].y += o[k][i].y * f, v[i].z += o[k][i].z * f, v[i].w += o[k][i].w * f;
+    }
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+    reinterpret_cast<u32x2*>(p.out)[((size_t)head * kSlices + slice0 + i * (kThreads / kTokens)) * w.tokens + token] = Joined(v[i], total);
+}
+
+// Many parts: a work-group takes one row, its threads share the slices and, in turn, the parts.
+template <int D, bool BY_SEQUENCE>
+__global__ __launch_bounds__(256) void kv4_attention_join_many_kernel(const JoinParams p) {
+  constexpr int kSlices = D / 4, kTurns = 256 / kSlices, kFirst = 4;
+  const Kv4Where& w = p.w;
+  const int thread = threadIdx.x, slice = thread % kSlices, turn = thread / kSlices;
+  const size_t rows = (size_t)w.tokens * p.heads;
+  size_t row = blockIdx.x;
+  if constexpr (BY_SEQUENCE) {
+    const Kv4Sequence q = Kv4SequenceOf(w, blockIdx.y);
+    const int of_sequence = q.count * p.share;
+    if (of_sequence < p.rows_from || of_sequence > p.rows_to || row >= (size_t)q.count * p.heads) return;
     row += (size_t)q.start * p.heads;
   }
-  __shared__ float factors[WAVES == 1 ? 1 : kMostParts];
-  __shared__ float4 sums[WAVES == 1 ? 1 : kTurns][kSlices];
-  __shared__ float2 of_wave[WAVES];
-  if (row >= step) return;  // (whole waves)
+  __shared__ float factors[kMostParts];
+  __shared__ float4 sums[kTurns][kSlices];
+  __shared__ float2 of_wave[4];
   float2 ml = make_float2(-INFINITY, 0.0f);
-  if (thread < p.parts) ml = p.part_ml[thread * step + row];  // each part's: a thread per part
+  if (thread < p.parts) ml = p.part_ml[thread * rows + row];  // each part's: a thread per part
   const float4* from = reinterpret_cast<const float4*>(p.part_o) + row * kSlices + slice;
   float4 first[kFirst];
 #pragma unroll
-  for (int j = 0; j < kFirst; ++j) first[j] = turn + j * kTurns < p.parts ? from[(turn + j * kTurns) * step * kSlices] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int j = 0; j < kFirst; ++j) first[j] = turn + j * kTurns < p.parts ? from[(turn + j * kTurns) * rows * kSlices] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int token = (int)(row / p.heads), head = (int)(row - (size_t)token * p.heads);
   if (token < w.starts[0] || token >= w.starts[w.sequences]) return;  // of no sequence (the whole row)
   float best = ml.x;
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) best = fmaxf(best, __shfl_xor(best, off));
-  if constexpr (WAVES > 1) {
-    if ((thread & 63) == 0) of_wave[thread >> 6].x = best;
-    __syncthreads();
+  if ((thread & 63) == 0) of_wave[thread >> 6].x = best;
+  __syncthreads();
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k) best = fmaxf(best, of_wave[k].x);
-  }
-  const float f = ml.y == 0.0f ? 0.0f : ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c);  // (0: a part that saw nothing)
+  for (int k = 0; k < 4; ++k) best = fmaxf(best, of_wave[k].x);
+  const float f = PartFactor(ml, best, p.c);
   float total = ml.y * f;
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) total += __shfl_xor(total, off);
-  if constexpr (WAVES > 1) {
-    factors[thread] = f;
-    if ((thread & 63) == 0) of_wave[thread >> 6].y = total;
-    __syncthreads();
-    total = 0.0f;
+  factors[thread] = f;
+  if ((thread & 63) == 0) of_wave[thread >> 6].y = total;
+  __syncthreads();
+  total = 0.0f;
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k) total += of_wave[k].y;
-  }
+  for (int k = 0; k < 4; ++k) total += of_wave[k].y;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto add = [&](int k, const float4& o) {
-    const float g = WAVES == 1 ? __shfl(f, k) : factors[k];
-    if (g != 0.0f) v.x += o.x * g, v.y += o.y * g, v.z += o.z * g, v.w += o.w * g;  // (0: nothing there, whatever the array holds)
+    const float g = factors[k];
+    if (g != 0.0f) v.x += o.x * g, v.y += o.y * g, v.z += o.z * g, v.w += o.w * g;
   };
 #pragma unroll
-  for (int j = 0; j < kFirst; ++j) {
-    const int k = min(turn + j * kTurns, kMostParts - 1);
-    if (j * kTurns < p.parts) add(WAVES == 1 ? k & 63 : k, first[j]);
-  }
-  for (int k0 = kFirst * kTurns; k0 < p.parts; k0 += kTurns) {
-    const int k = k0 + turn;
-    add(WAVES == 1 ? k & 63 : min(k, kMostParts - 1), k < p.parts ? from[k * step * kSlices] : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-  }
-  if constexpr (WAVES == 1) {
+  for (int j = 0; j < kFirst; ++j)
+    if (turn + j * kTurns < p.parts) add(turn + j * kTurns, first[j]);
+  for (int k = kFirst * kTurns + turn; k < p.parts; k += kTurns) add(k, from[k * rows * kSlices]);
+  sums[turn][slice] = v;
+  __syncthreads();
+  if (turn != 0) return;
 #pragma unroll
-    for (int off = kSlices; off < 64; off *= 2) {
-      v.x += __shfl_xor(v.x, off);
-      v.y += __shfl_xor(v.y, off);
-      v.z += __shfl_xor(v.z, off);
-      v.w += __shfl_xor(v.w, off);
-    }
-  } else {
-    sums[turn][slice] = v;
-    __syncthreads();
-#pragma unroll
-    for (int k = 1; k < kTurns; ++k) {
-      const float4 o = sums[k][slice];
-      if (turn == 0) v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-    }
+  for (int k = 1; k < kTurns; ++k) {
+    const float4 o = sums[k][slice];
+    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
   }
-  if (turn == 0) {
-    const float g = total == 0.0f ? 0.0f : 1.0f / total;
-    const half2_t a = {(_Float16)(v.x * g), (_Float16)(v.y * g)}, b = {(_Float16)(v.z * g), (_Float16)(v.w * g)};
-    reinterpret_cast<u32x2*>(p.out)[((size_t)head * kSlices + slice) * w.tokens + token] = u32x2{AsU32(a), AsU32(b)};
-  }
+  reinterpret_cast<u32x2*>(p.out)[((size_t)head * kSlices + slice) * w.tokens + token] = Joined(v, total);
 }
 
 template <int D, int GJ>
@@ -964,13 +1002,14 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
     if (of == 1) return;
     const JoinParams j = {a.where, p.part_o, p.part_ml, p.out, a.heads, of, p.c, share, rows_from, rows_to};
     // (a launch of more rows of a sequence than the op was made for: as many as the tensors have)
-    const int rows = both && rows_to < INT32_MAX ? rows_to / share * a.heads : a.where.tokens * a.heads;
-    const bool few = of <= kFewParts;
-    const dim3 grid(few ? DivUp(rows, 4) : rows, both ? a.where.sequences : 1);
-    if (both)
-      few ? kv4_attention_join_kernel<D, 1, true><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, 4, true><<<grid, 256, 0, stream>>>(j);
-    else
-      few ? kv4_attention_join_kernel<D, 1, false><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, 4, false><<<grid, 256, 0, stream>>>(j);
+    const int tokens = both && rows_to < INT32_MAX ? rows_to / share : a.where.tokens, sequences = both ? a.where.sequences : 1;
+    if (of <= kFewParts) {
+      const dim3 grid(DivUp(tokens, 8) * a.heads, sequences);
+      both ? kv4_attention_join_kernel<D, true><<<grid, D == 64 ? 128 : 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, false><<<grid, D == 64 ? 128 : 256, 0, stream>>>(j);
+    } else {
+      const dim3 grid(tokens * a.heads, sequences);
+      both ? kv4_attention_join_many_kernel<D, true><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_many_kernel<D, false><<<grid, 256, 0, stream>>>(j);
+    }
   };
   if (plan.few_rows > 0) join(plan.few_parts, 1, plan.few_rows);
   if (plan.few_rows < INT32_MAX) join(plan.many_parts, plan.few_rows + 1, INT32_MAX);
