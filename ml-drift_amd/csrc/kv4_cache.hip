@@ -260,7 +260,8 @@ void LaunchForm(const Kv4MoveArgs& p, hipStream_t stream) {
 constexpr int kFewNew = 8;
 template <typename T, int D, bool READ>
 void LaunchHead(const Kv4MoveArgs& p, hipStream_t stream) {
-  // few rows: a lane has one slice, so that a row is spread over as many lanes as it can; else 16 channels (reading: a tile for each wave)
+  // few rows: a lane has one slice, so that a row is spread over as many lanes as it can; else 16 channels (reading: a tile for each wave).
+  // Appending and reading back for 64 sequences, 8 heads of 128: 5.8 us against 9.9 at one row each, 7.5 against 8.4 at 8, 10.7 against 9.2 at 16.
   if (p.max_new <= kFewNew) {
     LaunchForm<T, D, 4, READ>(p, stream);
   } else if constexpr (READ) {
