@@ -711,6 +711,8 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
         if (sub + 1 < kSubs) start(sub + 1);
         __builtin_amdgcn_sched_barrier(0);
         u32x4 prob[2];
+        // two waves on a SIMD: the one with products goes first, the other's vector work fills in (8192 tokens, 32 heads of 128: 576 -> 567 us)
+        if (kWaves == 8) __builtin_amdgcn_s_setprio(1);
         if (sub + 1 < kSubs) {
 #pragma unroll
           for (int k = 0; k < kQ; ++k) key_product(sub + 1, k, next);
@@ -738,6 +740,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           if (sub * 2 * kTilesD + t + kAhead < kSubs * 2 * kTilesD) vf[t % kAhead] = value_piece(sub * 2 * kTilesD + t + kAhead);
           if (D != 256) __builtin_amdgcn_sched_barrier(0);
         }
+        if (kWaves == 8) __builtin_amdgcn_s_setprio(0);
         if constexpr (D == 256) {
           // one wave on a SIMD: its share of filling the other buffer goes under these products (behind the last step it is filled with what
           // is at hand and not looked at)
