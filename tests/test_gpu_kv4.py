@@ -357,10 +357,10 @@ def test_attention_in_parts(kv_heads, head_dim, group, page, many, parts):
 
 def test_attention_of_many_heads_for_a_key_head():
     """More heads on a key head than rows that the kernel for few takes: every row of a ragged batch is the other kernel's."""
-    d = attention_case(8, 40, 64, 32, 16, [1, 3, 0, 2, 1, 1, 1, 1], [90, 40, 3, 333, 200, 1, 17, 64])
+    d = attention_case(8, 56, 64, 32, 16, [1, 3, 0, 2, 1, 1, 1, 1], [90, 40, 3, 333, 200, 1, 17, 64])
     assert d.op.kernel_variant == "many"
     with M.tuning(kv4_parts=3):
-        attention_case(8, 40, 64, 32, 16, [1, 3, 0, 2, 1, 1, 1, 1], [90, 40, 3, 333, 200, 1, 17, 64])
+        attention_case(8, 56, 64, 32, 16, [1, 3, 0, 2, 1, 1, 1, 1], [90, 40, 3, 333, 200, 1, 17, 64])
 
 
 def test_attention_parts_of_one_kernel_beside_whole_rows_of_the_other():
