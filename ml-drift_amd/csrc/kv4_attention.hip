@@ -482,7 +482,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
 // The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.  Probabilities are up
 // to 2^(kManyLift + kSlack) = 2^14 then and keep 11 bits as halfs down to 2^-22 of the largest.
 // Measured: 8192 tokens, 32 heads over 8 of 128 (550 GFLOP): 567 us, 970 TFLOP/s where a large library product reaches 1156.  Vector
-// instructions take 57 % of a SIMD's cycles (exponentials 22, dequantizing 17), products 44 %: with one instruction issued at a time for a wave
+// instructions take 57 % of a SIMD's cycles (exponentials 22, dequantizing 15), products 44 %: with one instruction issued at a time for a wave
 // and two waves on a SIMD the two overlap little.  A fill, the first loads and the outputs of a work-group are 10 us around its steps.
 constexpr float kManyLift = 8.0f, kSlack = 6.0f;  // (in powers of two)
 constexpr int ManyWaves(int head_dim) { return head_dim == 256 ? 4 : 8; }
