@@ -823,6 +823,10 @@ int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* d, mldhip_op** 
 static int LaunchAroundAttention(mldhip_op* op, hipStream_t stream) {
   if (op->kind == mldhip_op::kKv4Attention && op->dst_ptr[0] == op->src_ptr[0])
     return Fail(MLDHIP_INVALID_ARGUMENT, "dst_tensor must not be src_q");
+  if (op->kind == mldhip_op::kNormRope && (op->dst_ptr[0] == op->src_ptr[1] || op->dst_ptr[1] == op->src_ptr[0]))
+    return Fail(MLDHIP_INVALID_ARGUMENT, "dst_q must not be src_k, nor dst_k src_q");
+  if ((op->kind == mldhip_op::kNormRope || op->kind == mldhip_op::kKv4Read) && op->dst_ptr[0] == op->dst_ptr[1])
+    return Fail(MLDHIP_INVALID_ARGUMENT, "the dst objects must not be one buffer");
   int device = -1;
   if (hipGetDevice(&device) != hipSuccess || device != op->device) {
     (void)hipGetLastError();

@@ -175,3 +175,19 @@ def test_attention_into_its_own_queries_is_refused():
         op.set_src_raw(i, 4096 * (i + 1), n)
     op.set_dst_raw(0, 4096, 8 * 128 * 4 * 2)
     assert "src_q" in refused(M.INVALID_ARGUMENT, op.launch)
+
+
+def test_results_into_one_buffer_are_refused():
+    def launch(op, srcs, dsts):
+        op.set_shape(1, 1, 4)
+        for i, p in enumerate(srcs):
+            op.set_src_raw(i, p, 1 << 30)
+        for i, p in enumerate(dsts):
+            op.set_dst_raw(i, p, 1 << 30)
+        return refused(M.INVALID_ARGUMENT, op.launch)
+
+    rope = M.qk_norm_rope_create(M.FLOAT16, 2, 2, 128, max_tokens=4)
+    assert "src_k" in launch(rope, [4096, 8192, 12288], [8192, 16384])
+    assert "src_q" in launch(rope, [4096, 8192, 12288], [16384, 4096])
+    assert "one buffer" in launch(rope, [4096, 8192, 12288], [16384, 16384])
+    assert "one buffer" in launch(M.kv4_read_create(cache(), M.FLOAT16, 4), [4096, 8192, 12288, 16384], [20480, 20480])
