@@ -505,7 +505,7 @@ int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int
 typedef struct {
   mldhip_kv4_cache_desc cache;
   int32_t heads; /* a multiple of cache.kv_heads; max_tokens * heads is at most 2^30 */
-  float scale;   /* positive */
+  float scale;   /* positive, below 2^100 */
   int32_t causal;
   int32_t window; /* 0: none */
   int32_t max_tokens;

@@ -789,7 +789,7 @@ int mldhip_kv4_attention_create(const mldhip_kv4_attention_desc* d, mldhip_op** 
   if (d->max_tokens < 1 || d->max_new_tokens < 1) return Fail(MLDHIP_INVALID_ARGUMENT, "max_tokens and max_new_tokens must be positive");
   if (d->max_tokens > kMostTokens) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens exceeds 2^24");
   if ((long long)d->max_tokens * d->heads > 1 << 30) return Fail(MLDHIP_OUT_OF_RANGE, "max_tokens * heads exceeds 2^30");
-  if (!(d->scale > 0.0f && std::isfinite(d->scale))) return Fail(MLDHIP_INVALID_ARGUMENT, "scale must be positive");
+  if (!(d->scale > 0.0f && d->scale < 0x1p100f)) return Fail(MLDHIP_INVALID_ARGUMENT, "scale must be positive and below 2^100");
   if (d->causal != 0 && d->causal != 1) return Fail(MLDHIP_INVALID_ARGUMENT, "causal must be 0 or 1");
   if (d->window < 0 || d->window > 1 << 30) return Fail(MLDHIP_INVALID_ARGUMENT, "window must be 0 .. 2^30");
   mldhip_op* op = new (std::nothrow) mldhip_op();

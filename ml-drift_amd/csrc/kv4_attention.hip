@@ -37,6 +37,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // their 11 bits down to 2^-28 of it.  The common factor leaves with the division by their sum, which is taken in fp32.
 constexpr float kLift = 14.0f;
 
+// x - max is one multiply-add where max * c is small enough that its rounding does not count (2^-12 in the exponent); beyond, the maximum is taken
+// away first: ulps of scores of 1e10 are thousands, which would be taken for powers of two.
+constexpr float kFar = 4096.0f;
+
 struct AttendParams {
   Kv4Where w;
   const __half* q;
@@ -284,6 +288,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
 
     float4_t acc[kPlanes][kCell];
     float top = -INFINITY, sum = 0.0f;
+    bool far = false;
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
@@ -361,6 +366,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
         const float now = fmaxf(top, best);
         const float down = top == now ? 1.0f : __builtin_amdgcn_exp2f((top - now) * p.c);  // (-inf - finite: 0)
         top = now;
+        far = __any(top != -INFINITY && fabsf(top) * p.c > kFar);
         sum *= down;
 #pragma unroll
         for (int pl = 0; pl < kPlanes; ++pl)
@@ -369,15 +375,22 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
       }
 
       half2_t prob[kTiles][2];
-      const float base = top == -INFINITY ? 0.0f : kLift - top * p.c;
+      float base = top == -INFINITY ? 0.0f : kLift - top * p.c;
+      if (far) {
+        base = top == -INFINITY ? 0.0f : kLift;
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) score[u][i] -= top == -INFINITY ? 0.0f : top;
+      }
 #pragma unroll
       for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2; ++i) {  // (the sum takes the probabilities as the product does, rounded to halfs)
           const float a = __builtin_amdgcn_exp2f(fmaf(score[u][2 * i], p.c, base));
           const float b = __builtin_amdgcn_exp2f(fmaf(score[u][2 * i + 1], p.c, base));
-          sum += a + b;
           prob[u][i] = half2_t{(_Float16)a, (_Float16)b};
+          sum = __builtin_amdgcn_fdot2(prob[u][i], half2_t{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
         }
 
       // out^T += values^T x p^T, 32 positions at a time
@@ -637,6 +650,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
 
     float16_t acc[kTilesD];
     float top = -INFINITY, sum = 0.0f;
+    bool far = false;
 #pragma unroll
     for (int j = 0; j < kTilesD; ++j)
 #pragma unroll
@@ -705,6 +719,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           const float higher = fmaxf(top, best);
           const float down = top == higher ? 1.0f : __builtin_amdgcn_exp2f((top - higher) * p.c);
           top = higher;
+          far = __any(top != -INFINITY && fabsf(top) * p.c > kFar);
           if (__any(sum != 0.0f)) {  // (not the first of the positions: nothing to scale)
             sum *= down;
 #pragma unroll
@@ -714,7 +729,12 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           }
         }
         settle();
-        const float base = top == -INFINITY ? 0.0f : kManyLift - top * p.c;
+        float base = top == -INFINITY ? 0.0f : kManyLift - top * p.c;
+        if (far) {
+          base = top == -INFINITY ? 0.0f : kManyLift;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) now[i] -= top == -INFINITY ? 0.0f : top;
+        }
         if (sub + 1 < kSubs) start(sub + 1);
         __builtin_amdgcn_sched_barrier(0);
         u32x4 prob[2];

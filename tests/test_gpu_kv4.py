@@ -476,6 +476,33 @@ def test_attention_sharp_and_far_apart_scores():
         attention_case(1, 2, 128, 64, 64, [65, 100], [1000, 100], q_scale=q_scale)
 
 
+@pytest.mark.parametrize("head_dim,group,page", [(64, 32, 16), (128, 64, 32), (256, 128, 64)])
+@pytest.mark.parametrize("many,parts", [(0, 1), (0, 3), (1, 1), (1, 2)])
+@pytest.mark.parametrize("size", [30.0, 1000.0, 60000.0])
+def test_attention_of_the_largest_scores(head_dim, group, page, many, parts, size):
+    """Two equal keys in far apart steps whose scores, up to 1e10, leave all others nothing: the output is the mean of their values, whatever
+    ulps of such scores are."""
+    rng = np.random.default_rng(head_dim + many + parts)
+    counts, lengths = [70, 2, 1], [700, 600, 555]
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    d = Device(2, head_dim, group, page, pages, starts, lengths, table)
+    d.fill(rng)
+    u = rng.choice([-1.0, 1.0], head_dim)
+    v = rng.standard_normal((2, 2, head_dim)) * 4
+    for s in range(3):
+        for i, p in enumerate((300, 17)):
+            d.host.set_token(table[s][p // page], p % page, np.stack([size * u] * 2), v[i])
+    d.cache.copy_(torch.from_numpy(d.host.bytes))
+    q = (size * u * np.ones((d.tokens, 6, 1))).astype(np.float16)
+    with M.tuning(kv4_many=many, kv4_parts=parts):
+        got = d.attend(q, 6)
+    exact, largest, _ = attention(q, d.host, table, lengths, starts, head_dim**-0.5, True, 0)
+    mean = np.repeat(kept(v, group).mean(0), 3, 0)  # [6][head_dim]
+    assert np.abs(exact - mean).max() < 1e-9
+    # two equal probabilities (rounded alike) and their sum, fp32 sums, one rounding to half
+    assert (np.abs(got - exact) <= 2.0**-11 * np.abs(exact) + 2.0**-20 * largest).all()
+
+
 def test_attention_of_rows_that_are_not_finite():
     rng = np.random.default_rng(9)
     starts, lengths, table, pages = batch(rng, [3, 1], [90, 70], 16)

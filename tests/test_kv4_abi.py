@@ -164,6 +164,7 @@ def test_sizes_past_what_a_launch_can_count_are_refused():
         create(cache(), M.FLOAT16, most)
         refused(M.OUT_OF_RANGE, create, cache(), M.FLOAT16, most + 1)
     refused(M.OUT_OF_RANGE, M.kv4_attention_create, cache(), 2, max_tokens=most + 1)
+    refused(M.INVALID_ARGUMENT, M.kv4_attention_create, cache(), 2, scale=3e38)
     M.qk_norm_rope_create(M.FLOAT16, 8, 2, 128, max_tokens=most)
     refused(M.OUT_OF_RANGE, M.qk_norm_rope_create, M.FLOAT16, 8, 2, 128, max_tokens=most + 1)
 
