@@ -503,6 +503,27 @@ def test_attention_of_the_largest_scores(head_dim, group, page, many, parts, siz
     assert (np.abs(got - exact) <= 2.0**-11 * np.abs(exact) + 2.0**-20 * largest).all()
 
 
+@pytest.mark.parametrize("many", [0, 1])
+def test_attention_of_many_small_probabilities(many):
+    """One key far above 66000 others, whose probabilities are subnormal halfs and yet add up to a hundredth of its own: they count in the outputs
+    and in their sum alike."""
+    rng = np.random.default_rng(31)
+    starts, lengths, table, pages = batch(rng, [50], [66000], 64)
+    d = Device(1, 64, 32, 64, pages, starts, lengths, table)
+    v = rng.uniform(-1, 1, 64) + np.where(np.arange(64) % 2, 2.0, -2.0)
+    shape = (pages, 1, 64, 64)
+    d.host.set_all(np.zeros(shape), np.broadcast_to(v, shape))
+    one = np.ones((1, 64))
+    d.host.set_token(table[0][500], 0, one, -v[None])
+    d.cache.copy_(torch.from_numpy(d.host.bytes))
+    q = np.full((50, 2, 64), 22.4 / math.log2(math.e) / 64 * 8).astype(np.float16)  # (the score of the one key is 22.4 in powers of two)
+    with M.tuning(kv4_many=many):
+        got = d.attend(q, 2)
+    exact, largest, score = attention(q, d.host, table, lengths, starts, 64**-0.5, True, 0)
+    assert np.abs(exact + kept(v[None], 32)).max() > 0.02  # (without the others it would be -v)
+    check_attention(got, exact, largest, score)
+
+
 def test_attention_of_rows_that_are_not_finite():
     rng = np.random.default_rng(9)
     starts, lengths, table, pages = batch(rng, [3, 1], [90, 70], 16)
