@@ -1081,7 +1081,10 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
     // four tokens each, 16 heads of 64: 16.9 against 17.8 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of
     // 1000 positions, a key head of 256: 11.9 us against 12.8).
     const int full = 4 * FewOnSimd(a.head_dim), waves = 256 * full;  // of a CU; of the chip
-    plan.few_waves = groups <= 256 && 256 / groups * groups >= 192 && 256 / groups * 32 * full <= keys ? full : 4;
+    // And where one such work-group has a step for each wave: no second kernel (one sequence of 256 positions, 8 heads of 128: 7.3 us against 10.4
+    // from the host, 6.8 against 7.7 in a graph; of 512, heads of 64: 7.9 / 11.0 and 7.2 / 6.8; up to 128 positions are one of 4 waves).
+    const bool fills = 256 / groups * groups >= 192 && 256 / groups * 32 * full <= keys, one_step = keys > 128 && keys <= 32 * full;
+    plan.few_waves = groups <= 256 && (fills || one_step) ? full : 4;
     plan.few_parts = parts(t.kv4_parts > 0 ? std::min<long long>(t.kv4_parts, (keys + 127) / 128)
                                              : std::min(waves / plan.few_waves / groups, (keys + 32 * plan.few_waves - 1) / (32 * plan.few_waves)));
   }
