@@ -1075,6 +1075,7 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
   const long long row_bytes = (long long)a.max_tokens * a.heads * (a.head_dim + 2) * 4, room = ((long long)256 << 20) / row_bytes;
   const auto parts = [&](long long v) { return (int)std::max(1LL, std::min({v, room, (long long)kMostParts})); };
   if (plan.few_rows > 0) {
+    const long long few_keys = a.window > 0 ? std::min<long long>(keys, a.window + most_new) : keys;  // that a tile may see
     const long long groups = row_tiles(many ? std::min<long long>(rows, few_rows) : rows, 16);
     // Work-groups of all the waves that a CU holds where they fill the CUs and each wave has a step: fewer outputs to join, none with as many
     // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 30.5 us against 31.8 in 3 parts of 4 waves; 16 of up to 2047,
@@ -1083,10 +1084,10 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
     const int full = 4 * FewOnSimd(a.head_dim), waves = 256 * full;  // of a CU; of the chip
     // And where one such work-group has a step for each wave: no second kernel (one sequence of 256 positions, 8 heads of 128: 7.3 us against 10.4
     // from the host, 6.8 against 7.7 in a graph; of 512, heads of 64: 7.9 / 11.0 and 7.2 / 6.8; up to 128 positions are one of 4 waves).
-    const bool fills = 256 / groups * groups >= 192 && 256 / groups * 32 * full <= keys, one_step = keys > 128 && keys <= 32 * full;
+    const bool fills = 256 / groups * groups >= 192 && 256 / groups * 32 * full <= few_keys, one_step = few_keys > 128 && few_keys <= 32 * full;
     plan.few_waves = groups <= 256 && (fills || one_step) ? full : 4;
     plan.few_parts = parts(t.kv4_parts > 0 ? std::min<long long>(t.kv4_parts, (keys + 127) / 128)
-                                             : std::min(waves / plan.few_waves / groups, (keys + 32 * plan.few_waves - 1) / (32 * plan.few_waves)));
+                                             : std::min(waves / plan.few_waves / groups, (few_keys + 32 * plan.few_waves - 1) / (32 * plan.few_waves)));
   }
   if (many) {
     // Parts level the work-groups' shares, and their outputs go through memory: the number with the least estimated time.  Steps that the
