@@ -402,7 +402,9 @@ def test_attention_by_work_groups_of_whole_compute_units(head_dim, group, page, 
     lengths = [1 + (most + 40) * i // (sequences - 1) for i in range(sequences)]
     counts = [min(l, 1 + i % 2) for i, l in enumerate(lengths)]
     d = attention_case(kv_heads, 3, head_dim, group, page, counts, lengths, window=most // 2 if page == 32 else 0, behind=1, seed=head_dim + parts)
-    assert d.op.kernel_variant == "few" and d.op.kernel_tiles == (16, waves, parts)
+    # (in a window of half the positions 4 parts have not a step for each of their waves: work-groups of 4 waves then)
+    form = (16, 4, 7) if page == 32 and parts == 4 else (16, waves, parts)
+    assert d.op.kernel_variant == "few" and d.op.kernel_tiles == form
 
 
 def test_attention_of_more_than_a_thousand_sequences():
