@@ -85,7 +85,7 @@ struct Unpack {
 // The first product runs on the codes as they are, exact small integers; their scale and zero point, which belong to (position, group),
 // are applied to its fp32 sums, one pair of multiply-adds per 32 .. 128 codes: sum q (code - zero) = sum q (base + code) - base sum q - zero
 // sum q.  The values are dequantized, exactly (kv4.h).
-// Measured: 4 sequences of 65536 positions, 8 key heads of 128 (285 MB): 62.9 us with the join, 4.5 TB/s where a large copy reaches 4.9.  Shorter
+// Measured: 4 sequences of 65536 positions, 8 key heads of 128 (285 MB): 56.9 us with the join, 5.0 TB/s where a large copy reaches 4.9.  Shorter
 // caches are bound by vector instructions (about 300 for 32 positions, most of them unpacking: they alone could take heads of 128 in at 10 TB/s,
 // of 64 at 5.4) and by what precedes the first product: lengths, table, codes, one after the other, 3 to 4 us.
 template <int D, int GJ>
@@ -499,8 +499,8 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
 // reads of a product are runs of neighbouring pieces.
 // The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.  Probabilities are up
 // to 2^(kManyLift + kSlack) = 2^14 then and keep 11 bits as halfs down to 2^-22 of the largest.
-// Measured: 8192 tokens, 32 heads over 8 of 128 (550 GFLOP): 567 us, 970 TFLOP/s where a large library product reaches 1156.  Vector
-// instructions take 57 % of a SIMD's cycles (exponentials 22, dequantizing 15), products 44 %: with one instruction issued at a time for a wave
+// Measured: 8192 tokens, 32 heads over 8 of 128 (550 GFLOP): 561 us, 980 TFLOP/s where a large library product reaches 1156.  Vector
+// instructions take 59 % of a SIMD's cycles (exponentials 23, dequantizing 15), products 46 %: with one instruction issued at a time for a wave
 // and two waves on a SIMD the two overlap little.  A fill, the first loads and the outputs of a work-group are 10 us around its steps.
 constexpr float kManyLift = 8.0f, kSlack = 6.0f;  // (in powers of two)
 constexpr int ManyWaves(int head_dim) { return head_dim == 256 ? 4 : 8; }
@@ -1078,8 +1078,8 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
     const long long few_keys = a.window > 0 ? std::min<long long>(keys, a.window + most_new) : keys;  // that a tile may see
     const long long groups = row_tiles(many ? std::min<long long>(rows, few_rows) : rows, 16);
     // Work-groups of all the waves that a CU holds where they fill the CUs and each wave has a step: fewer outputs to join, none with as many
-    // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 30.5 us against 31.8 in 3 parts of 4 waves; 16 of up to 2047,
-    // four tokens each, 16 heads of 64: 16.9 against 17.8 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of
+    // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 28.1 us against 29.9 in 3 parts of 4 waves; 16 of up to 2047,
+    // four tokens each, 16 heads of 64: 16.7 against 17.9 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of
     // 1000 positions, a key head of 256: 11.9 us against 12.8).
     const int full = 4 * FewOnSimd(a.head_dim), waves = 256 * full;  // of a CU; of the chip
     // And where one such work-group has a step for each wave: no second kernel (one sequence of 256 positions, 8 heads of 128: 7.3 us against 10.4
