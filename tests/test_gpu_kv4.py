@@ -526,6 +526,25 @@ def test_attention_of_many_small_probabilities(many):
     check_attention(got, exact, largest, score)
 
 
+@pytest.mark.parametrize("many,parts", [(0, 1), (0, 3), (0, 12), (1, 1), (1, 2), (-1, -1)])
+def test_rows_in_front_of_the_first_sequence_stay(many, parts):
+    rng = np.random.default_rng(17)
+    starts, lengths, table, pages = batch(rng, [2, 0, 60, 1], [900, 5, 1700, 1], 32)
+    starts = starts + 3
+    tokens = int(starts[-1]) + 2
+    d = Device(2, 64, 32, 32, pages, starts, lengths, table, tokens)
+    d.fill(rng)
+    q = rng.standard_normal((tokens, 6, 64)).astype(np.float16)
+    with M.tuning(kv4_many=many, kv4_parts=parts):
+        got = d.attend(q, 6)
+    exact, largest, score = attention(q, d.host, table, lengths, starts, 64**-0.5, True, 0, fill=5.0)
+    check_attention(got, exact, largest, score)
+    assert (got[:3] == 5.0).all() and (got[-2:] == 5.0).all()
+    for most in (1, 60):
+        for x in d.read(np.float32, most=most):
+            assert (x[:3] == 5.0).all() and (x[-2:] == 5.0).all() and (x[3:-2] != 5.0).any(-1).all()
+
+
 def test_attention_of_rows_that_are_not_finite():
     rng = np.random.default_rng(9)
     starts, lengths, table, pages = batch(rng, [3, 1], [90, 70], 16)
