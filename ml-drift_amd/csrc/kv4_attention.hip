@@ -46,7 +46,7 @@ struct AttendParams {
   const __half* q;
   const uint8_t* cache;
   __half* out;
-  float* part_o;   // [parts][rows of the tensors][D]
+  float* part_o;   // few rows: [parts][rows of the tensors][D]; many: [parts][heads][D / 4][tokens][4], the outputs' own order
   float2* part_ml; // [parts][rows]: maximum (of q . k) and sum
   int heads, share, parts, causal, window;
   float c;  // scale * log2(e)
@@ -845,8 +845,8 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
             }
       };
       if (p.parts > 1) {
-        float4* to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * w.tokens + token) * p.heads + head) * (D / 4) + half * kCell;
-        store([&](int slice, const float(&v)[4]) { to[slice] = make_float4(v[0], v[1], v[2], v[3]); });
+        float4* to = reinterpret_cast<float4*>(p.part_o) + (((size_t)part * p.heads + head) * (D / 4) + half * kCell) * w.tokens + token;
+        store([&](int slice, const float(&v)[4]) { to[(size_t)slice * w.tokens] = make_float4(v[0], v[1], v[2], v[3]); });
         if (half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
       } else {
         u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
@@ -870,6 +870,12 @@ struct JoinParams {
   int heads, parts;
   float c;
   int share, rows_from, rows_to;  // sequence by sequence: those of rows_from .. rows_to rows
+  int many;                       // the order of part_o
+  // slice 0 of a row's outputs, and how far its slices are apart
+  __device__ __forceinline__ const float4* First(int slices, int token, int head) const {
+    return reinterpret_cast<const float4*>(part_o) + (many ? (size_t)head * slices * w.tokens + token : ((size_t)token * heads + head) * slices);
+  }
+  __device__ __forceinline__ size_t Apart() const { return many ? w.tokens : 1; }
 };
 constexpr int kMostParts = 256, kFewParts = 8;
 // Rows of a sequence up to which the kernel for few rows serves it.  It does a tile of 16 rows at a time, the other one up to 256 at once.
@@ -904,7 +910,8 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(const JoinParam
   if (token >= w.tokens) return;
   const size_t rows = (size_t)w.tokens * p.heads, row = (size_t)token * p.heads + head;
   const int slice0 = threadIdx.x / kTokens;
-  const float4* from = reinterpret_cast<const float4*>(p.part_o) + row * kSlices + slice0;
+  const size_t apart = p.Apart();
+  const float4* from = p.First(kSlices, token, head) + slice0 * apart;
   float2 ml[kFewParts];
   float4 o[kFewParts][kItems];
 #pragma unroll
@@ -912,7 +919,7 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(const JoinParam
     if (k < p.parts) {
       ml[k] = p.part_ml[k * rows + row];
 #pragma unroll
-      for (int i = 0; i < kItems; ++i) o[k][i] = from[k * rows * kSlices + i * (kThreads / kTokens)];
+      for (int i = 0; i < kItems; ++i) o[k][i] = from[k * rows * kSlices + i * (kThreads / kTokens) * apart];
     }
   if (!BY_SEQUENCE && (token < w.starts[0] || token >= w.starts[w.sequences])) return;  // of no sequence
   float best = -INFINITY;
@@ -956,11 +963,11 @@ __global__ __launch_bounds__(256) void kv4_attention_join_many_kernel(const Join
   __shared__ float2 of_wave[4];
   float2 ml = make_float2(-INFINITY, 0.0f);
   if (thread < p.parts) ml = p.part_ml[thread * rows + row];  // each part's: a thread per part
-  const float4* from = reinterpret_cast<const float4*>(p.part_o) + row * kSlices + slice;
+  const int token = (int)(row / p.heads), head = (int)(row - (size_t)token * p.heads);
+  const float4* from = p.First(kSlices, token, head) + slice * p.Apart();
   float4 first[kFirst];
 #pragma unroll
   for (int j = 0; j < kFirst; ++j) first[j] = turn + j * kTurns < p.parts ? from[(turn + j * kTurns) * rows * kSlices] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const int token = (int)(row / p.heads), head = (int)(row - (size_t)token * p.heads);
   if (token < w.starts[0] || token >= w.starts[w.sequences]) return;  // of no sequence (the whole row)
   float best = ml.x;
 #pragma unroll
@@ -1015,6 +1022,21 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
   p.c = a.scale * kLog2e;
   p.part_o = a.partial;
   p.part_ml = reinterpret_cast<float2*>(a.partial + (size_t)std::max(plan.few_parts, plan.many_parts) * a.max_tokens * a.heads * D);
+  const bool both = plan.few_rows > 0 && plan.few_rows < INT32_MAX;
+  auto join = [&](int of, int rows_from, int rows_to, int many) {
+    if (of == 1) return;
+    const JoinParams j = {a.where, p.part_o, p.part_ml, p.out, a.heads, of, p.c, share, rows_from, rows_to, many};
+    // (a launch of more rows of a sequence than the op was made for: as many as the tensors have)
+    const int tokens = both && rows_to < INT32_MAX ? rows_to / share : a.where.tokens, sequences = both ? a.where.sequences : 1;
+    if (of <= kFewParts) {
+      const dim3 grid(DivUp(tokens, 8) * a.heads, sequences);
+      both ? kv4_attention_join_kernel<D, true><<<grid, D == 64 ? 128 : 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, false><<<grid, D == 64 ? 128 : 256, 0, stream>>>(j);
+    } else {
+      const dim3 grid(tokens * a.heads, sequences);
+      both ? kv4_attention_join_many_kernel<D, true><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_many_kernel<D, false><<<grid, 256, 0, stream>>>(j);
+    }
+  };
+  // (one kernel's parts are joined before the other's are written: their orders are not the same)
   if (plan.few_rows > 0) {
     p.parts = plan.few_parts;
     p.rows_from = 1;
@@ -1027,6 +1049,7 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
       big ? kv4_attention_few_kernel<D, GJ, kFull, true><<<grid, 64 * kFull, 0, stream>>>(p) : kv4_attention_few_kernel<D, GJ, kFull, false><<<grid, 64 * kFull, 0, stream>>>(p);
     else
       big ? kv4_attention_few_kernel<D, GJ, 4, true><<<grid, 256, 0, stream>>>(p) : kv4_attention_few_kernel<D, GJ, 4, false><<<grid, 256, 0, stream>>>(p);
+    join(plan.few_parts, 1, plan.few_rows, 0);
   }
   if (plan.few_rows < INT32_MAX) {
     p.parts = plan.many_parts;
@@ -1034,23 +1057,8 @@ void Launch(const Kv4AttentionArgs& a, hipStream_t stream) {
     p.rows_to = INT32_MAX;
     const dim3 grid(a.where.kv_heads, std::min(p.parts * DivUp(most_new * share, 32 * ManyWaves(D)), 65535 / p.parts * p.parts), a.where.sequences);
     kv4_attention_many_kernel<D, GJ><<<grid, 64 * ManyWaves(D), 0, stream>>>(p);
+    join(plan.many_parts, plan.few_rows + 1, INT32_MAX, 1);
   }
-  const bool both = plan.few_rows > 0 && plan.few_rows < INT32_MAX;
-  auto join = [&](int of, int rows_from, int rows_to) {
-    if (of == 1) return;
-    const JoinParams j = {a.where, p.part_o, p.part_ml, p.out, a.heads, of, p.c, share, rows_from, rows_to};
-    // (a launch of more rows of a sequence than the op was made for: as many as the tensors have)
-    const int tokens = both && rows_to < INT32_MAX ? rows_to / share : a.where.tokens, sequences = both ? a.where.sequences : 1;
-    if (of <= kFewParts) {
-      const dim3 grid(DivUp(tokens, 8) * a.heads, sequences);
-      both ? kv4_attention_join_kernel<D, true><<<grid, D == 64 ? 128 : 256, 0, stream>>>(j) : kv4_attention_join_kernel<D, false><<<grid, D == 64 ? 128 : 256, 0, stream>>>(j);
-    } else {
-      const dim3 grid(tokens * a.heads, sequences);
-      both ? kv4_attention_join_many_kernel<D, true><<<grid, 256, 0, stream>>>(j) : kv4_attention_join_many_kernel<D, false><<<grid, 256, 0, stream>>>(j);
-    }
-  };
-  if (plan.few_rows > 0) join(plan.few_parts, 1, plan.few_rows);
-  if (plan.few_rows < INT32_MAX) join(plan.many_parts, plan.few_rows + 1, INT32_MAX);
 }
 
 }  // namespace
