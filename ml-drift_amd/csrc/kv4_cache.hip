@@ -7,8 +7,8 @@
 // codes do not depend on how a division rounds.  Inputs are held to +-57344 and NaN counts as 0: a cached value is always a finite half,
 // and a masked position can never turn a product into NaN.
 //
-// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.63.  Reading 8 sequences of 8192 tokens, 8 heads of 128 (340 MB): 82 us,
-// 4.1 TB/s where a large copy reaches 4.9 (four fifths of the bytes are stores).  5000 fp32 tokens of one head of 256 (12 MB): 8.2 us to append, 6.9 to
+// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.63.  Reading 8 sequences of 8192 tokens, 8 heads of 128 (340 MB): 75 us,
+// 4.5 TB/s where a large copy reaches 4.9 (four fifths of the bytes are stores).  5000 fp32 tokens of one head of 256 (12 MB): 8.1 us to append, 6.8 to
 // read, and one token of 64 sequences 3.7 and 2.7: lengths, table and data, one after the other.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -78,6 +78,19 @@ __device__ __forceinline__ void Store4(uint2* p, const float v[4]) {  // (every 
   *p = raw;
 }
 __device__ __forceinline__ void Store4(float4* p, const float v[4]) { *p = make_float4(v[0], v[1], v[2], v[3]); }
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Stores past the L2, for results that are larger (8 sequences of 8192 tokens, 8 heads of 128: 83.6 -> 75.4 us).
+__device__ __forceinline__ void Stream4(uint2* p, const float v[4]) {
+  uint2 raw;
+  Store4(&raw, v);
+  __builtin_nontemporal_store(u32x2{raw.x, raw.y}, reinterpret_cast<u32x2*>(p));
+}
+__device__ __forceinline__ void Stream4(float4* p, const float v[4]) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(p));
+}
 
 // Byte offsets inside a tile's codes: of the 2 bytes of 4 channels from `channel` on.
 template <int D>
@@ -179,8 +192,6 @@ __global__ __launch_bounds__(256) void kv4_move_kernel(const Kv4MoveArgs p) {
 // Reading many rows: a wave takes one tile of the cache, whose codes it reads as a lane of attention's products does, 8 or 16 bytes at a time
 // (kv4.h); tokens run along the lanes of the stores, so that these are runs of 16 tokens.
 // Grid: tiles of a sequence's rows x (head, keys or values) x sequences.
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_read_tiles_kernel(const Kv4MoveArgs p) {
   using Raw = typename Slice<T>::type;
@@ -246,8 +257,8 @@ __global__ __launch_bounds__(256) void kv4_read_tiles_kernel(const Kv4MoveArgs p
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e / 4][e % 4] = scale * (float)((int)((nibbles >> (4 * e)) & 15u) - (int)(word & 15u));
         if (is_row) {
-          Store4(tensor + (size_t)(channel / 4) * w.tokens + row, v[0]);
-          Store4(tensor + (size_t)(channel / 4 + 1) * w.tokens + row, v[1]);
+          Stream4(tensor + (size_t)(channel / 4) * w.tokens + row, v[0]);
+          Stream4(tensor + (size_t)(channel / 4 + 1) * w.tokens + row, v[1]);
         }
       }
     __builtin_amdgcn_wave_barrier();  // (the exchange is written again)
