@@ -43,15 +43,19 @@ __host__ __device__ constexpr int Kv4ValueWords(int page, int head_dim, int grou
 struct Kv4Sequence {
   int start, count, first, held;
 };
-__device__ __forceinline__ Kv4Sequence Kv4SequenceOf(const Kv4Where& w, int s) {
-  Kv4Sequence q;
-  const int a = w.starts[s], b = w.starts[s + 1];
-  q.start = min(max(a, 0), w.tokens);
-  q.count = max(min(b, w.tokens) - q.start, 0);
-  const int length = min(max(w.lengths[s], 0), 1 << 30);
+__host__ __device__ constexpr int Kv4Within(int v, int low, int high) { return v < low ? low : v > high ? high : v; }
+__host__ __device__ constexpr Kv4Sequence Kv4SequenceFrom(int from, int to, int length, int tokens, int pages_per_sequence, int page_shift) {
+  Kv4Sequence q{};
+  q.start = Kv4Within(from, 0, tokens);
+  q.count = Kv4Within(to, q.start, tokens) - q.start;  // (both ends in range first: a difference of what the arrays hold may overflow)
+  length = Kv4Within(length, 0, 1 << 30);
   q.first = length - q.count;
-  q.held = (int)min((long long)length, (long long)w.pages_per_sequence << w.page_shift);
+  const long long room = (long long)pages_per_sequence << page_shift;
+  q.held = length < room ? length : (int)room;
   return q;
+}
+__device__ __forceinline__ Kv4Sequence Kv4SequenceOf(const Kv4Where& w, int s) {
+  return Kv4SequenceFrom(w.starts[s], w.starts[s + 1], w.lengths[s], w.tokens, w.pages_per_sequence, w.page_shift);
 }
 
 }  // namespace mldhip
