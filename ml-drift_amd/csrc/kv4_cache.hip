@@ -238,7 +238,8 @@ __global__ __launch_bounds__(256) void kv4_read_tiles_kernel(const Kv4MoveArgs p
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    const uint16_t* mine = reinterpret_cast<const uint16_t*>(exchange[threadIdx.x >> 6]);
+    const uint32_t* mine = exchange[threadIdx.x >> 6];
+    const uint32_t of_token = n % 2 ? 0x07060302u : 0x05040100u;  // the half of a word that is the lane's token's
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl)
 #pragma unroll
@@ -248,8 +249,8 @@ __global__ __launch_bounds__(256) void kv4_read_tiles_kernel(const Kv4MoveArgs p
         uint32_t nibbles = piece[pl][k];
         if (is_value) {
           const int i = channel % P, j = i + 4;  // (of 4 channels each)
-          const int at = (pl * 64 + n / 4 * 16) * 2 * kWords + n % 4;
-          nibbles = mine[at + i / kCell * 2 * kWords + i % kCell / 4 * 4] | (uint32_t)mine[at + j / kCell * 2 * kWords + j % kCell / 4 * 4] << 16;
+          const int at = (pl * 64 + n / 4 * 16) * kWords + n % 4 / 2;
+          nibbles = __builtin_amdgcn_perm(mine[at + j / kCell * kWords + j % kCell / 4 * 2], mine[at + i / kCell * kWords + i % kCell / 4 * 2], of_token);
         }
         const uint32_t word = held ? words[(channel >> w.group_shift) * 16 + n] : 0;  // (scale 0: zeros)
         const float scale = __half2float(__ushort_as_half((unsigned short)(word & 0xFFF0u)));
@@ -261,7 +262,11 @@ __global__ __launch_bounds__(256) void kv4_read_tiles_kernel(const Kv4MoveArgs p
           Stream4(tensor + (size_t)(channel / 4 + 1) * w.tokens + row, v[1]);
         }
       }
-    __builtin_amdgcn_wave_barrier();  // (the exchange is written again)
+    if (is_value) {  // the exchange is written again: behind all lanes' reads
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
   }
 }
 

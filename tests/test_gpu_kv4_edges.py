@@ -5,7 +5,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 import mldhip as M
-from test_gpu_kv4 import Device, stream
+from test_gpu_kv4 import SHAPES, Device, batch, stream
 
 torch = pytest.importorskip("torch")
 
@@ -50,3 +50,19 @@ def test_starts_of_any_values_stay_in_bounds(head_dim):
             out, around = guarded(src[0].numel(), torch.float16)
             print("attend", head_dim, many, parts, flush=True)
             launched(op, [src[0], cache], [out], [around])
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_read_of_many_tiles_for_a_wave(kv_heads, head_dim, group, page, dtype):
+    """Launches sized for a few rows of a sequence: each wave reads many tiles, one after the other, through the same LDS."""
+    rng = np.random.default_rng(head_dim + group + page + 2)
+    counts, lengths = [333, 1, 150], [333, 40, 170]
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table)
+    d.fill(rng)
+    values = d.host.values()
+    for got, y in zip(d.read(dtype, most=9), values):
+        for s, n in enumerate(counts):
+            at = np.arange(lengths[s] - n, lengths[s])
+            assert np.array_equal(got[starts[s]:starts[s + 1]].astype(np.float64), y[table[s][at // page], :, at % page])
