@@ -16,6 +16,7 @@
 namespace mldhip {
 namespace {
 
+typedef _Float16 half_t;
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
@@ -29,7 +30,6 @@ __device__ __forceinline__ uint32_t AsU32(half2_t v) { return __builtin_bit_cast
 // A nibble at bits 0..3 of a half's mantissa under the exponent of 1024 is 1024 + nibble, at bits 4..7 under that of 64 it is 64 + nibble:
 // one and-or unpacks two nibbles, and only every other pair needs a shift.
 constexpr uint32_t kLowMask = 0x000F000Fu, kHighMask = 0x00F000F0u, kLowBase = 0x64006400u, kHighBase = 0x54005400u;
-constexpr float kLowOffset = 1024.0f, kHighOffset = 64.0f;
 constexpr uint32_t kScaleMask = 0xFFF0FFF0u;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -82,9 +82,8 @@ struct Unpack {
 //   scores^T [16 positions][16 rows] = codes of keys x q^T     a lane has one row (lane & 15) and 4 positions (4 (lane >> 4) + i)
 //   out^T   [16 cells][16 rows]     += values^T x p^T          of 32 positions: those that the lanes hold are the operand's order, so the
 //                                                              probabilities go from one product to the next in registers
-// The first product runs on the codes as they are, exact small integers; their scale and zero point, which belong to (position, group),
-// are applied to its fp32 sums, one pair of multiply-adds per 32 .. 128 codes: sum q (code - zero) = sum q (base + code) - base sum q - zero
-// sum q.  The values are dequantized, exactly (kv4.h).
+// Keys and values are dequantized, exactly (kv4.h), so that the scores are fp32 sums of exact products: sums over the codes on their bases
+// would be rounded at the size of 1024 sum |q| and lose the small codes of a group with one channel far from zero.
 // Measured: 4 sequences of 65536 positions, 8 key heads of 128 (285 MB): 56.9 us with the join, 5.0 TB/s where a large copy reaches 4.9.  Shorter
 // caches are bound by vector instructions (about 300 for 32 positions, most of them unpacking: they alone could take heads of 128 in at 10 TB/s,
 // of 64 at 5.4) and by what precedes the first product: lengths, table, codes, one after the other, 3 to 4 us.
@@ -96,9 +95,10 @@ struct FewShape {
   static constexpr int kValueRegs = kPlanes * kCell / 2;  // and of its values (4 channels of 2 positions each)
   static constexpr int kStep = 32;                        // positions that a wave takes at a time: two steps are in registers
   static constexpr int kTiles = kStep / 16;
-  // The words of the keys belong to positions, which all 16 lanes of a quarter share: lane n loads those of tile n / kGroups, group n %
-  // kGroups, and they are broadcast from there.
-  static_assert(kTiles * kGroups <= 16);
+  // A lane needs the words of the keys of its position (lane & 15) for all groups, as the other quarters do: quarter i loads those of groups
+  // i, i + 4, and they change quarters by register exchanges, those of both tiles in one register.
+  static constexpr int kGroupsAtOnce = kGroups < 4 ? kGroups : 4, kWordRegs = kGroups / kGroupsAtOnce;
+  static_assert(kTiles == 2);
 };
 
 // The cached bytes of one step, as a lane holds them.
@@ -106,32 +106,22 @@ template <int D, int GJ>
 struct FewStep {
   using S = FewShape<D, GJ>;
   uint32_t keys[S::kTiles][S::kKeyRegs], values[S::kTiles][S::kValueRegs];
-  u32x2 key_words, value_words[S::kTiles][S::kPlanes];
+  uint32_t key_words[S::kTiles][S::kWordRegs];
+  u32x2 value_words[S::kTiles][S::kPlanes];
 };
 
-// Lane `from` of each row of 16 lanes, in all of the row.
-template <int FROM>
-__device__ __forceinline__ uint32_t OfRow(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x150 + FROM /* row_newbcast */, 0xf, 0xf, true);
-}
-__device__ __forceinline__ uint32_t OfRow(uint32_t v, int from) {  // (`from` is a constant where it is inlined)
-  switch (from) {
-    case 0: return OfRow<0>(v);
-    case 1: return OfRow<1>(v);
-    case 2: return OfRow<2>(v);
-    case 3: return OfRow<3>(v);
-    case 4: return OfRow<4>(v);
-    case 5: return OfRow<5>(v);
-    case 6: return OfRow<6>(v);
-    case 7: return OfRow<7>(v);
-    case 8: return OfRow<8>(v);
-    case 9: return OfRow<9>(v);
-    case 10: return OfRow<10>(v);
-    case 11: return OfRow<11>(v);
-    case 12: return OfRow<12>(v);
-    case 13: return OfRow<13>(v);
-    case 14: return OfRow<14>(v);
-    default: return OfRow<15>(v);
+// From the registers of all quarters (GROUPS of them with words of their own, the others repeat these) those of every group.
+template <int GROUPS>
+__device__ __forceinline__ void OfQuarters(uint32_t v, uint32_t* to) {
+  if constexpr (GROUPS == 1) {
+    to[0] = v;
+  } else if constexpr (GROUPS == 2) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    to[0] = r[0], to[1] = r[1];
+  } else {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    OfQuarters<2>(r[0], to);
+    OfQuarters<2>(r[1], to + 2);
   }
 }
 
@@ -159,6 +149,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
   __shared__ float2 ml_lds[WAVES][16];
   const Unpack unpack;
   const uint32_t key_at = (n * 4 + quad) * (P / 8), value_at = (quad * 16 + n) * (2 * kCell);  // a lane's piece of a tile's codes
+  const uint32_t key_word_at = 32 * (quad % S::kGroupsAtOnce) + 2 * n;
   const uint32_t value_word_at = 32 * (n * kCell / (32 * GJ)) + 8 * quad;
 
   // (a sequence with one new token, the common case, divides nothing)
@@ -168,6 +159,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
     const int first_row = q.first + token_of(row0), last_row = q.first + token_of(min(rows, row0 + 16) - 1);
     const int hi = p.causal ? min(q.held, last_row + 1) : q.held;
     const int lo = p.window > 0 ? max(0, first_row + 1 - p.window) : 0;
+    const int all_hi = p.causal ? min(q.held, first_row + 1) : q.held, all_lo = p.window > 0 ? last_row + 1 - p.window : 0;  // (what all of them see)
     const int step0 = lo / kStep, steps = hi > lo ? (hi - 1) / kStep + 1 - step0 : 0;
     const int each = p.parts == 1 ? steps : (steps + p.parts - 1) / p.parts;
     const int begin = step0 + min(steps, part * each) + wave, end = step0 + min(steps, (part + 1) * each);
@@ -212,10 +204,8 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
             to.keys[u][0] = a.x, to.keys[u][1] = a.y;
           }
         }
-        if (BIG ? u == 0 : true) {
-          const int mine = min(n / kGroups, kTiles - 1);  // (lanes behind the words read the last tile's)
-          if (BIG || mine == u) to.key_words = *reinterpret_cast<const u32x2*>(kw + 8u * quad + (BIG ? mine * kWordBytes : 0) + 32 * (n % kGroups));
-        }
+#pragma unroll
+        for (int j = 0; j < S::kWordRegs; ++j) to.key_words[u][j] = *reinterpret_cast<const uint16_t*>(kw + key_word_at + t * kWordBytes + 128 * j);
       }
     };
     auto load_values = [&](int step, const Ids& ids, FewStep<D, GJ>& to) {
@@ -249,9 +239,6 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
     }
 
     u32x4 qa[kKeyRegs];  // operands of the first product: channel s and channel s + 4 of 8 in each register
-    // minus the sum of the row's q over a group; what the sums of products start from: minus the sum of q times the codes' bases, and the
-    // base of the zero points times the sum of q
-    float qsum[kGroups], qbase[kGroups];
     const int row = row0 + n;
     const bool there = row < rows;
     const int token = token_of(there ? row : 0), head = kv_head * p.share + (there ? row : 0) - token * p.share;
@@ -261,8 +248,6 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
     // what the lane's row sees
     const int row_hi = there ? (p.causal ? min(q.held, position + 1) : q.held) : 0, row_lo = p.window > 0 ? max(0, position + 1 - p.window) : 0;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) qsum[g] = qbase[g] = 0.0f;
-#pragma unroll
     for (int k = 0; k < kKeyRegs; ++k) {
       u32x2 a = {0u, 0u}, b = {0u, 0u};
       if (there) {
@@ -271,19 +256,6 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
       }
       qa[k] = u32x4{__builtin_amdgcn_perm(b.x, a.x, 0x05040100u), __builtin_amdgcn_perm(b.x, a.x, 0x07060302u),
                     __builtin_amdgcn_perm(b.y, a.y, 0x05040100u), __builtin_amdgcn_perm(b.y, a.y, 0x07060302u)};
-      float low = 0.0f, high = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const half2_t v = AsHalf2(qa[k][e]);
-        ((e & 1) ? high : low) += (float)v.x + (float)v.y;
-      }
-      qsum[k / GJ] += low + high;
-      qbase[k / GJ] += kLowOffset * low + kHighOffset * high;
-    }
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      qsum[g] = -SumAcrossQuarters(qsum[g]);
-      qbase[g] = -SumAcrossQuarters(qbase[g]) - kLowOffset * qsum[g];
     }
 
     float4_t acc[kPlanes][kCell];
@@ -300,45 +272,39 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
       __builtin_amdgcn_s_setprio(1);
       // scores: score[u][i] = q . k of row n and position 16 u + 4 quad + i
       float score[kTiles][4];
-      if constexpr (kGroups == 8) {  // (what the sums start from, four times each, would stay in 32 registers over the loop)
+      uint32_t words[kGroups];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) asm volatile("" : "+v"(qbase[g]));
-      }
+      for (int j = 0; j < S::kWordRegs; ++j) OfQuarters<S::kGroupsAtOnce>(c.key_words[0][j] | c.key_words[1][j] << 16, words + 4 * j);
 #pragma unroll
       for (int u = 0; u < kTiles; ++u) {
-        float4_t raw[kGroups];
+        float4_t raw = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < kKeyRegs; ++k) {
-          const uint32_t a = c.keys[u][k], b = a >> 8;
-          const u32x4 codes = {unpack.Low(a), unpack.High(a), unpack.Low(b), unpack.High(b)};
-          const float o = qbase[k / GJ];
-          const float4_t from = k % GJ == 0 ? float4_t{o, o, o, o} : raw[k / GJ];
-          raw[k / GJ] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes),
-                                                                  __builtin_bit_cast(half8_t, qa[k]), from, 0, 0, 0);
+          const uint32_t a = c.keys[u][k], b = a >> 8, word = words[k / GJ];
+          const half_t scale = AsHalf2(word & unpack.scale_mask)[u], low_zero = AsHalf2(unpack.Low(word))[u], high_zero = AsHalf2(unpack.High(word << 4))[u];
+          const half2_t scales = {scale, scale}, low_zeros = {low_zero, low_zero}, high_zeros = {high_zero, high_zero};
+          const u32x4 key = {AsU32((AsHalf2(unpack.Low(a)) - low_zeros) * scales), AsU32((AsHalf2(unpack.High(a)) - high_zeros) * scales),
+                             AsU32((AsHalf2(unpack.Low(b)) - low_zeros) * scales), AsU32((AsHalf2(unpack.High(b)) - high_zeros) * scales)};
+          raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, key), __builtin_bit_cast(half8_t, qa[k]), raw, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) score[u][i] = 0.0f;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t word = OfRow(c.key_words[i / 2], u * kGroups + g);
-            const float scale = (float)AsHalf2(word & unpack.scale_mask)[i % 2], zero = (float)AsHalf2(unpack.Low(word))[i % 2];
-            score[u][i] = fmaf(scale, fmaf(zero, qsum[g], raw[g][i]), score[u][i]);
-          }
+        for (int i = 0; i < 4; ++i) score[u][i] = raw[i];
         // (a tile's products and sums at a time: left alone, the compiler puts all the step's products first and needs registers for them)
 #pragma unroll
         for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(score[u][i]));
       }
       __builtin_amdgcn_s_setprio(2);
-      // (the next step's keys come while this one's values are taken, and the other way round)
-      if (step + WAVES < end) load_keys(step + WAVES, ids_next, c);
+      // (the next step's keys come while this one's values are taken, and the other way round; behind the last step it comes again: branches
+      // around the loads would have the next step wait for all of them)
+      load_keys(min(step + WAVES, end - 1), ids_next, c);
       __builtin_amdgcn_sched_barrier(0);
       // a step inside what every row sees, on pages that there are, needs no masks
-      bool whole = step * kStep + kStep <= (p.causal ? min(q.held, first_row + 1) : q.held);
-      if (p.window > 0) whole = whole && step * kStep > last_row - p.window;
+      bool whole = step * kStep + kStep <= all_hi && step * kStep >= all_lo;
 #pragma unroll
-      for (int u = 0; u < kIds; ++u) whole = whole && ids.id[u] >= 0 && ids.id[u] < w.pages;
+      for (int u = 0; u < kIds; ++u) {
+        const int id = __builtin_amdgcn_readfirstlane(ids.id[u]);  // (uniform: scalar comparisons)
+        whole = whole && id >= 0 && id < w.pages;
+      }
       if (!whole) {
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) {
@@ -433,7 +399,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
         }
       }
       __builtin_amdgcn_s_setprio(0);
-      if (step + WAVES < end) load_values(step + WAVES, ids_next, c);
+      load_values(min(step + WAVES, end - 1), ids_next, c);
       ids = ids_next;
       ids_next = look_up(min(step + 2 * WAVES, end - 1));
       __builtin_amdgcn_sched_barrier(0);

@@ -5,6 +5,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 import mldhip as M
+from kv4math import attention
 from test_gpu_kv4 import SHAPES, Device, batch, stream
 
 torch = pytest.importorskip("torch")
@@ -66,3 +67,66 @@ def test_read_of_many_tiles_for_a_wave(kv_heads, head_dim, group, page, dtype):
         for s, n in enumerate(counts):
             at = np.arange(lengths[s] - n, lengths[s])
             assert np.array_equal(got[starts[s]:starts[s + 1]].astype(np.float64), y[table[s][at // page], :, at % page])
+
+
+# ---- groups of keys with a channel far from zero ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kv_heads,head_dim,group,page", SHAPES)
+@pytest.mark.parametrize("many,parts", [(0, 1), (0, 2), (1, 1)])
+def test_attention_scores_are_sums_of_the_few_products_that_there_are(kv_heads, head_dim, group, page, many, parts):
+    """Every group of a key has one channel at 100, which the queries do not look at, two a step of its scale from zero and all others at zero,
+    while the queries' mean is far from zero: the score is the sum of two products for each group, and nothing else may be seen of the rest."""
+    rng = np.random.default_rng(head_dim + group)
+    counts, lengths = [3, 1, 40], [5, 2, 40]
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table)
+    groups = head_dim // group
+    shape = (pages, kv_heads, page)
+    k = np.zeros((*shape, groups, group))
+    k[..., 0] = 100.0
+    step = 6.6875  # (the least half of 7 significant bits whose 15-fold is 100)
+    for _ in range(2):
+        at = rng.integers(1, group, (*shape, groups))
+        np.put_along_axis(k, at[..., None], rng.choice([0.0, step], (*shape, groups))[..., None], -1)
+    v = rng.standard_normal((*shape, head_dim))
+    d.host.set_all(k.reshape(*shape, head_dim), v)
+    d.cache.copy_(torch.from_numpy(d.host.bytes))
+    q = (8 + 8 * rng.standard_normal((d.tokens, kv_heads * 3, groups, group))).astype(np.float16)
+    q[..., 0] = 0
+    q = q.reshape(d.tokens, kv_heads * 3, head_dim)
+    with M.tuning(kv4_many=many, kv4_parts=parts):
+        got = d.attend(q, kv_heads * 3, scale=1 / 128)
+    exact, largest, score = attention(q, d.host, table, lengths, starts, 1 / 128, True, 0)
+    # 2 * groups products at most that are not zero, an fp32 sum of them (2^-23 each, whichever way it rounds); the exponent's own error and the
+    # multiply-add in front of it, 2^-20 for scores of up to 8 or so; probabilities and outputs rounded to halfs, 2^-11 each, of what is averaged
+    assert score.max() < 32
+    tol = (2.0**-11 + 2 * (2 * groups * 2.0**-23 * score + 2.0**-20)) * largest + 2.0**-11 * np.abs(exact) + 2.0**-24
+    err = np.abs(got.astype(np.float64) - exact)
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("head_dim,group", [(64, 64), (128, 128), (128, 32), (256, 128)])
+@pytest.mark.parametrize("away,mean", [(50.0, 5.0), (100.0, 3.0)])
+def test_attention_of_keys_with_a_channel_far_away(head_dim, group, away, mean):
+    """A key channel of 50 and 100, where queries are small, and queries with a mean elsewhere: outputs are as near the exact ones as the roundings of
+    the probabilities and of the outputs let them be, in both kernels."""
+    rng = np.random.default_rng(head_dim + group + int(away))
+    counts, lengths, page, kv_heads, share = [2, 1], [500, 301], 64, 2, 4
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    d = Device(kv_heads, head_dim, group, page, pages, starts, lengths, table)
+    shape = (pages, kv_heads, page, head_dim)
+    k = rng.standard_normal(shape)
+    k[..., 7] += away
+    d.host.set_all(k, rng.standard_normal(shape))
+    d.cache.copy_(torch.from_numpy(d.host.bytes))
+    q = mean + mean * rng.standard_normal((d.tokens, kv_heads * share, head_dim))
+    q[..., 7] = 0.05 * rng.standard_normal(q.shape[:-1])
+    q = q.astype(np.float16)
+    exact, _, _ = attention(q, d.host, table, lengths, starts, head_dim**-0.5, True, 0)
+    for many in (0, 1):
+        with M.tuning(kv4_many=many):
+            got = d.attend(q, kv_heads * share)
+        off = np.sqrt(((got - exact)**2).mean() / (exact**2).mean())
+        # a half rounds by 2^-11 at most, 2^-11 / sqrt(3) in the mean of squares, the probabilities and the outputs once each: 4.0e-4
+        print("off", many, off, flush=True)
+        assert off <= 2.0**-11, (many, off)
