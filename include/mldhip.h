@@ -498,7 +498,7 @@ int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int
 
 /* Attention of the rows over what the cache holds of their sequence (their own positions appended before):
  *   out_r = sum_t softmax_t(scale * q_r . k_t) v_t,  t < lengths[s]; causal: t <= position of r; window > 0: t > position of r - window.
- * A row that sees no position is 0.  Query head h reads key / value head h / (heads / kv_heads).  src objects: 0 "src_q"
+ * A row that sees no position is 0, one with an infinity or a NaN that sees any is NaN.  Query head h reads key / value head h / (heads / kv_heads).  src objects: 0 "src_q"
  * [heads * head_dim / 4][tokens][4] halfs, 1 "cache", 2 "page_table", 3 "lengths", 4 "starts"; dst 0 "dst_tensor", as src_q (another buffer).
  * fp16 tensors; scores, softmax and sums in fp32, the probabilities rounded to halfs for the second product.
  * max_new_tokens chooses between the kernels for few and for many rows of a sequence; launches with more rows than that are served. */

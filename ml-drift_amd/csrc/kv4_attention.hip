@@ -67,6 +67,16 @@ __device__ __forceinline__ float SumAcrossQuarters(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// A row of queries with an infinity or a NaN has no softmax: NaN, unless it sees no position, which is 0 whatever the row holds.  Its scores may
+// be -inf like the ones that masks leave, or NaN behind the masks too: a row whose sum is not above 0 is looked at again, whether any of the
+// positions from .. to - 1, which no mask hides, lies on a page that there is.
+__device__ __forceinline__ bool SeesAny(const Kv4Where& w, const int32_t* table, int from, int to) {
+  if (from < to)
+    for (int page = from >> w.page_shift; page <= (to - 1) >> w.page_shift; ++page)
+      if (table[page] >= 0 && table[page] < w.pages) return true;
+  return false;
+}
+
 // The masks and bases in registers whose values the compiler does not see: as literals each and-or would be two instructions.
 struct Unpack {
   uint32_t low_mask = kLowMask, high_mask = kHighMask, low_base = kLowBase, high_base = kHighBase, scale_mask = kScaleMask;
@@ -162,7 +172,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
     const int all_hi = p.causal ? min(q.held, first_row + 1) : q.held, all_lo = p.window > 0 ? last_row + 1 - p.window : 0;  // (what all of them see)
     const int step0 = lo / kStep, steps = hi > lo ? (hi - 1) / kStep + 1 - step0 : 0;
     const int each = p.parts == 1 ? steps : (steps + p.parts - 1) / p.parts;
-    const int begin = step0 + min(steps, part * each) + wave, end = step0 + min(steps, (part + 1) * each);
+    const int part_begin = step0 + min(steps, part * each), begin = part_begin + wave, end = step0 + min(steps, (part + 1) * each);
 
     // The pages of a step are looked up one step ahead of its bytes, and these asked for one step ahead of their use: a wave always has a
     // step's bytes in flight.  Pages of at least a step are one look-up and one address.  (Small pages: tiles behind the last held position
@@ -336,7 +346,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
         const float now = fmaxf(top, best);
         const float down = top == now ? 1.0f : __builtin_amdgcn_exp2f((top - now) * p.c);  // (-inf - finite: 0)
         top = now;
-        far = __any(top != -INFINITY && fabsf(top) * p.c > kFar);
+        far = __any(fabsf(top) * p.c > kFar && fabsf(top) != INFINITY);  // (a row of infinities is NaN either way, and its neighbours as without it)
         sum *= down;
 #pragma unroll
         for (int pl = 0; pl < kPlanes; ++pl)
@@ -417,6 +427,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
       const float2 ml = ml_lds[v][n];
       total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
     }
+    if (total == 0.0f && SeesAny(w, table, max(row_lo, part_begin * kStep), min(row_hi, end * kStep))) total = __builtin_nanf("");
     const float mine = top == best ? 1.0f : __builtin_amdgcn_exp2f((top - best) * p.c);
     const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
     if (there)
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
           const float higher = fmaxf(top, best);
           const float down = top == higher ? 1.0f : __builtin_amdgcn_exp2f((top - higher) * p.c);
           top = higher;
-          far = __any(top != -INFINITY && fabsf(top) * p.c > kFar);
+          far = __any(fabsf(top) * p.c > kFar && fabsf(top) != INFINITY);  // (a row of infinities is NaN either way, and its neighbours as without it)
           if (__any(sum != 0.0f)) {  // (not the first of the positions: nothing to scale)
             sum *= down;
 #pragma unroll
@@ -794,9 +805,16 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
     }
 
     const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    const float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    if (!(total > 0.0f)) {
+      int thread = threadIdx.x;  // (worked out again, out of the compiler's sight: kept over the steps, what the row sees would be spilled)
+      asm volatile("" : "+v"(thread));
+      const int same_row = wave_row + (thread & 31), at = q.first + (same_row < rows ? same_row : 0) / p.share;
+      const int from = p.window > 0 ? max(0, at + 1 - p.window) : 0, to = same_row < rows ? (p.causal ? min(q.held, at + 1) : q.held) : 0;
+      total = SeesAny(w, table, max(from, begin * kStep), min(to, end * kStep)) ? __builtin_nanf("") : 0.0f;
+    }
     if (is_row) {
-      const float factor = p.parts > 1 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+      const float factor = p.parts > 1 ? 1.0f : 1.0f / total;
       auto store = [&](auto to) {  // to(slice behind the half's own first, its 4 channels)
 #pragma unroll
         for (int pl = 0; pl < kPlanes; ++pl)
@@ -816,10 +834,15 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
         if (half == 0) p.part_ml[((size_t)part * w.tokens + token) * p.heads + head] = make_float2(top, total);
       } else {
         u32x2* to = reinterpret_cast<u32x2*>(p.out) + ((size_t)head * (D / 4) + half * kCell) * w.tokens + token;
-        store([&](int slice, const float(&v)[4]) {
-          const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
-          to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
-        });
+        if (total > 0.0f) {
+          store([&](int slice, const float(&v)[4]) {
+            const half2_t a = {(_Float16)v[0], (_Float16)v[1]}, b = {(_Float16)v[2], (_Float16)v[3]};
+            to[(size_t)slice * w.tokens] = u32x2{AsU32(a), AsU32(b)};
+          });
+        } else {  // 0 or NaN, whatever the sums are
+          const half2_t same = {(_Float16)total, (_Float16)total};
+          store([&](int slice, const float(&)[4]) { to[(size_t)slice * w.tokens] = u32x2{AsU32(same), AsU32(same)}; });
+        }
       }
     }
   }

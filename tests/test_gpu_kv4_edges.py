@@ -130,3 +130,35 @@ def test_attention_of_keys_with_a_channel_far_away(head_dim, group, away, mean):
         # a half rounds by 2^-11 at most, 2^-11 / sqrt(3) in the mean of squares, the probabilities and the outputs once each: 4.0e-4
         print("off", many, off, flush=True)
         assert off <= 2.0**-11, (many, off)
+
+
+# ---- rows of queries that are not finite ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("head_dim,group,page", [(64, 32, 16), (128, 64, 32), (256, 128, 64)])
+@pytest.mark.parametrize("many,parts", [(0, 1), (0, 3), (0, 12), (1, 1), (1, 2), (1, 12)])
+@pytest.mark.parametrize("odd", [np.nan, np.inf, -np.inf])
+def test_attention_of_odd_rows_is_nan_or_nothing(head_dim, group, page, many, parts, odd):
+    """An infinity or a NaN in a row of queries: NaN where the row sees a position (also if all its scores are -inf), 0 where it sees none, and no
+    difference in any other row."""
+    rng = np.random.default_rng(head_dim + parts)
+    # sequence 0: the first 40 rows have positions below 0; 1: no page that is the cache's; 2: the first two pages are not, the window leaves some
+    # rows only these; 3: two rows of a sequence of nothing; 4: ordinary
+    counts, lengths, window = [60, 50, 40, 2, 33], [20, 50, 2 * page + 8, 0, 1500], 24
+    starts, lengths, table, pages = batch(rng, counts, lengths, page)
+    table[1, :], table[2, :2] = -1, pages + 5
+    d = Device(2, head_dim, group, page, pages, starts, lengths, table)
+    d.host.set_all(*(np.abs(rng.standard_normal((pages, 2, page, head_dim))) + 1 for _ in range(2)))  # (keys above 0: scores of one sign)
+    d.cache.copy_(torch.from_numpy(d.host.bytes))
+    q = rng.standard_normal((d.tokens, 6, head_dim)).astype(np.float16)
+    odd_rows = rng.random((d.tokens, 6)) < 0.4
+    with_odd = q.copy()
+    at = rng.integers(0, head_dim, q.shape[:2])
+    np.put_along_axis(with_odd, at[..., None], np.where(odd_rows, odd, np.take_along_axis(q, at[..., None], -1)[..., 0])[..., None].astype(np.float16), -1)
+    _, largest, _ = attention(q, d.host, table, lengths, starts, head_dim**-0.5, True, window)
+    sees = np.broadcast_to(largest[..., 0] > 0, odd_rows.shape)
+    assert (odd_rows & sees).sum() > 50 and (odd_rows & ~sees).sum() > 50
+    with M.tuning(kv4_many=many, kv4_parts=parts):
+        got, rest = d.attend(with_odd, 6, window=window), d.attend(q, 6, window=window)
+    assert np.isnan(got[odd_rows & sees]).all()
+    assert (got[odd_rows & ~sees] == 0).all() and (rest[~sees] == 0).all()
+    assert np.array_equal(got[~odd_rows], rest[~odd_rows])
