@@ -437,7 +437,8 @@ int mldhip_conv_int8_create(const mldhip_conv_int8_desc* desc, mldhip_op** op);
  *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * frequency_i, for the pairs of the first rotary_dim channels of a head:
  *   channels (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved is set; frequency_i = base^(-2 i / rotary_dim), or
  *   frequencies[i] (host memory, read by the create call) where that is given.  Channels behind rotary_dim are normed only.
- * fp32 arithmetic, one rounding to the tensors' type; angles are exact to 2^-32 turns at every int32 position.
+ * fp32 arithmetic, one rounding to the tensors' type.  Whole turns are taken out exactly at every int32 position (frequencies of up to 2^60); what
+ * is left of an angle is off by 2^-28 turns at most where tensors are fp32, and by 2^-26 where they are halfs.
  * src objects: 0 "src_q" [heads * head_dim / 4][tokens][4], 1 "src_k" [kv_heads * head_dim / 4][tokens][4], 2 "positions" int32 [tokens],
  * and with norms 3 "q_norm_weight", 4 "k_norm_weight" [head_dim] of the tensors' type.  dst objects: 0 "dst_q", 1 "dst_k", as the sources;
  * each may be its source's buffer itself.  head_dim and rotary_dim are multiples of 8, head_dim at most 256. */

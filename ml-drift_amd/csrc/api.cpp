@@ -618,6 +618,16 @@ static int CurrentDevice() {
 
 constexpr int kMostTokens = 1 << 24;  // of one launch: work-items of a grid stay below 2^32
 
+// f / (2 pi) modulo 1 as a 64-bit fraction.  1 / (2 pi) in two parts, the product with the first one exact (p + e): positions multiply what is lost,
+// and a frequency of many turns would leave a quotient of 64 bits few behind the point.  Right to the last bit or so up to frequencies of 2^60.
+static uint64_t TurnsOf(long double f) {
+  const long double high = 0xa2f9836e4e44152ap-66L, low = -0xf62a0b82b2c88fc9p-136L;
+  const long double p = f * high, e = std::fma(f, high, -p), r = f * low;
+  __int128 sum = (__int128)1 << 31;  // in 2^-96 turns; half of the last bit
+  for (const long double part : {p, e, r}) sum += (__int128)std::ldexp(part - std::trunc(part), 96);
+  return (uint64_t)(sum >> 32);
+}
+
 int mldhip_qk_norm_rope_create(const mldhip_qk_norm_rope_desc* d, mldhip_op** out) {
   if (!d || !out) return Fail(MLDHIP_INVALID_ARGUMENT, "null argument");
   *out = nullptr;
@@ -639,10 +649,7 @@ int mldhip_qk_norm_rope_create(const mldhip_qk_norm_rope_desc* d, mldhip_op** ou
   for (int i = 0; i < d->rotary_dim / 2; ++i) {
     const long double f = d->frequencies ? (long double)d->frequencies[i] : std::pow((long double)d->base, -2.0L * i / d->rotary_dim);
     if (!std::isfinite(f)) return Fail(MLDHIP_INVALID_ARGUMENT, "frequencies must be finite");
-    long double t = f / 6.283185307179586476925286766559005768L;
-    t -= std::floor(t);
-    const long double whole = std::floor(std::ldexp(t, 64) + 0.5L);
-    turns[i] = whole >= 18446744073709551616.0L ? 0 : (uint64_t)whole;
+    turns[i] = TurnsOf(f);
   }
   mldhip_op* op = new (std::nothrow) mldhip_op();
   if (!op) return Fail(MLDHIP_INTERNAL, "out of memory");
