@@ -181,8 +181,8 @@ class DecoderStack:
 
 
 class AttentionBlock:
-    """q / k / v -> norms and rotation -> cache -> attention -> o, five or six ops on one stream over ragged batches of `sequences`
-    sequences: prompts, chunks of prompts and single tokens alike.  set_batch() says which rows are whose and rebinds; launch() neither
+    """q / k / v -> norms and rotation -> cache -> attention -> o, on one stream (q / k / v as one launch where they can be) over ragged batches of
+    `sequences` sequences: prompts, chunks of prompts and single tokens alike.  set_batch() says which rows are whose and rebinds; launch() neither
     allocates nor synchronises and may be captured, and page_table, lengths, starts and positions may be rewritten between replays.
     The cache has `pages` pages, of which the caller gives each sequence its own in page_table."""
 
@@ -223,9 +223,15 @@ class AttentionBlock:
         """page_table [sequences][pages_per_sequence], lengths and starts as the ops over the cache take them (lengths count the new
         tokens).  tokens: rows of the tensors, starts[-1] unless given (padded batches)."""
         torch = self.torch
-        lengths, starts = np.asarray(lengths, np.int32), np.asarray(starts, np.int32)
+        page_table, lengths, starts = [np.asarray(a, np.int32) for a in (page_table, lengths, starts)]
+        for name, a, to in (("page_table", page_table, self.page_table), ("lengths", lengths, self.lengths), ("starts", starts, self.starts)):
+            if a.shape != tuple(to.shape):
+                raise ValueError("%s: %s where the block has %s" % (name, a.shape, tuple(to.shape)))
         tokens = int(starts[-1]) if tokens is None else tokens
-        assert 1 <= tokens <= self.max_tokens
+        if not 1 <= tokens <= self.max_tokens:
+            raise ValueError("%d rows where the block was made for 1 .. %d" % (tokens, self.max_tokens))
+        if starts[0] < 0 or starts[-1] > tokens or (np.diff(starts) < 0).any():
+            raise ValueError("starts must not decrease, and lie within the %d rows" % tokens)
         positions = np.zeros(self.max_tokens, np.int32)
         for s, length in enumerate(lengths):
             positions[starts[s]:starts[s + 1]] = np.arange(length - (starts[s + 1] - starts[s]), length)
