@@ -391,7 +391,7 @@ def _read(state):
     case = state["case"]
     s, position, inside = _where(state)
     valid = (inside & (position >= 0))[:, None, None]
-    at = position.clamp(min=0)
+    at = position.clamp(0, state["table"].shape[1] * case["page"] - 1)  # (rows of no sequence have positions behind all pages: zeros below)
     found = []
     for x, old in zip(_cached(state), (state["out_k"], state["out_v"])):
         found.append(_slices(torch.where(valid, x[s, :, at], torch.zeros((), device="cuda")).to(old.dtype)))
