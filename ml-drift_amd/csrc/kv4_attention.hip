@@ -67,14 +67,28 @@ __device__ __forceinline__ float SumAcrossQuarters(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The lane's number, worked out where it is asked for: kept over a kernel's steps it would cost a register there (spilled for heads of 256).
+__device__ __forceinline__ int LaneHere() {
+  uint32_t all = ~0u;
+  asm volatile("" : "+s"(all));
+  return (int)__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+}
+
 // A row of queries with an infinity or a NaN has no softmax: NaN, unless it sees no position, which is 0 whatever the row holds.  Its scores may
 // be -inf like the ones that masks leave, or NaN behind the masks too: a row whose sum is not above 0 is looked at again, whether any of the
-// positions from .. to - 1, which no mask hides, lies on a page that there is.
-__device__ __forceinline__ bool SeesAny(const Kv4Where& w, const int32_t* table, int from, int to) {
-  if (from < to)
-    for (int page = from >> w.page_shift; page <= (to - 1) >> w.page_shift; ++page)
-      if (table[page] >= 0 && table[page] < w.pages) return true;
-  return false;
+// positions from .. to - 1, which no mask hides, lies on a page that there is.  All lanes take part, 64 pages of begin .. end - 1 (positions, the same
+// in all lanes) at a time.
+__device__ __forceinline__ bool SeesAny(const Kv4Where& w, const int32_t* table, int begin, int end, int from, int to) {
+  const int lane = LaneHere(), pages = end > begin ? ((end - 1) >> w.page_shift) + 1 : 0;
+  const int first = from >> w.page_shift, behind = from < to ? ((to - 1) >> w.page_shift) + 1 : first;
+  bool any = false;
+  for (int page = begin >> w.page_shift; page < pages && __any(!any && first < behind); page += 64) {
+    const int id = page + lane < pages ? table[page + lane] : -1;
+    const uint64_t there = __ballot(id >= 0 && id < w.pages);
+    const int low = max(first - page, 0), high = min(behind - page, 64);
+    if (low < high) any = any || (there << (64 - high) >> (64 - high + low)) != 0;
+  }
+  return any;
 }
 
 // The masks and bases in registers whose values the compiler does not see: as literals each and-or would be two instructions.
@@ -427,7 +441,10 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
       const float2 ml = ml_lds[v][n];
       total += ml.y * (ml.x == best ? 1.0f : __builtin_amdgcn_exp2f((ml.x - best) * p.c));
     }
-    if (total == 0.0f && SeesAny(w, table, max(row_lo, part_begin * kStep), min(row_hi, end * kStep))) total = __builtin_nanf("");
+    if (__any(total == 0.0f)) {
+      const int from = max(row_lo, part_begin * kStep), to = min(row_hi, end * kStep);
+      if (SeesAny(w, table, part_begin * kStep, min(q.held, end * kStep), from, total == 0.0f ? to : from)) total = __builtin_nanf("");
+    }
     const float mine = top == best ? 1.0f : __builtin_amdgcn_exp2f((top - best) * p.c);
     const float factor = mine * (p.parts > 1 ? 1.0f : total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total);
     if (there)
@@ -806,12 +823,11 @@ __global__ __launch_bounds__(D == 256 ? 256 : 512, D == 256 ? 1 : 2) void kv4_at
 
     const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     float total = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    if (!(total > 0.0f)) {
-      int thread = threadIdx.x;  // (worked out again, out of the compiler's sight: kept over the steps, what the row sees would be spilled)
-      asm volatile("" : "+v"(thread));
-      const int same_row = wave_row + (thread & 31), at = q.first + (same_row < rows ? same_row : 0) / p.share;
-      const int from = p.window > 0 ? max(0, at + 1 - p.window) : 0, to = same_row < rows ? (p.causal ? min(q.held, at + 1) : q.held) : 0;
-      total = SeesAny(w, table, max(from, begin * kStep), min(to, end * kStep)) ? __builtin_nanf("") : 0.0f;
+    if (__any(!(total > 0.0f))) {
+      const int same_row = wave_row + LaneHere() % 32, at = q.first + (same_row < rows ? same_row : 0) / p.share;
+      const int from = max(p.window > 0 ? at + 1 - p.window : 0, begin * kStep), to = min(p.causal ? min(q.held, at + 1) : q.held, end * kStep);
+      const bool none = !(total > 0.0f), sees = SeesAny(w, table, begin * kStep, min(q.held, end * kStep), from, none && same_row < rows ? to : from);
+      if (none) total = sees ? __builtin_nanf("") : 0.0f;
     }
     if (is_row) {
       const float factor = p.parts > 1 ? 1.0f : 1.0f / total;

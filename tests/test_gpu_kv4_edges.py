@@ -6,7 +6,7 @@ pytestmark = pytest.mark.gpu
 
 import mldhip as M
 from kv4math import attention
-from test_gpu_kv4 import SHAPES, Device, batch, stream
+from test_gpu_kv4 import SHAPES, Device, batch, check_attention, stream
 
 torch = pytest.importorskip("torch")
 
@@ -162,3 +162,27 @@ def test_attention_of_odd_rows_is_nan_or_nothing(head_dim, group, page, many, pa
     assert np.isnan(got[odd_rows & sees]).all()
     assert (got[odd_rows & ~sees] == 0).all() and (rest[~sees] == 0).all()
     assert np.array_equal(got[~odd_rows], rest[~odd_rows])
+
+
+@pytest.mark.parametrize("many,parts", [(0, 1), (0, 5), (1, 1), (1, 4)])
+@pytest.mark.parametrize("page_there", [0, 63, 64, 130, 162, None])
+def test_attention_of_odd_rows_over_a_table_with_one_page(many, parts, page_there):
+    """Of 163 pages one is there, or none."""
+    rng = np.random.default_rng(7)
+    counts, lengths = [40, 1], [2600, 2600]
+    starts, lengths, table, pages = batch(rng, counts, lengths, 16)
+    for row in table:
+        row[np.arange(len(row)) != (-1 if page_there is None else page_there)] = -3
+    d = Device(1, 64, 32, 16, pages, starts, lengths, table)
+    d.fill(rng)
+    q = rng.standard_normal((d.tokens, 4, 64)).astype(np.float16)
+    odd_rows = rng.random((d.tokens, 4)) < 0.4
+    q[odd_rows, 5] = np.nan
+    with M.tuning(kv4_many=many, kv4_parts=parts):
+        got = d.attend(q, 4)
+    exact, largest, score = attention(np.where(odd_rows[..., None], 0, q), d.host, table, lengths, starts, 64**-0.5, True, 0)
+    sees = (largest[..., 0] > 0) & (np.zeros((1, 4)) == 0)
+    assert sees.any() == (page_there is not None)
+    assert np.isnan(got[odd_rows & sees]).all() and (got[~sees] == 0).all()
+    ordinary = ~odd_rows & sees
+    check_attention(got[ordinary], exact[ordinary], largest[ordinary], score[ordinary])
