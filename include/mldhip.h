@@ -502,7 +502,8 @@ int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int
  * A row that sees no position is 0, one with an infinity or a NaN that sees any is NaN.  Query head h reads key / value head h / (heads / kv_heads).  src objects: 0 "src_q"
  * [heads * head_dim / 4][tokens][4] halfs, 1 "cache", 2 "page_table", 3 "lengths", 4 "starts"; dst 0 "dst_tensor", as src_q (another buffer).
  * fp16 tensors; scores, softmax and sums in fp32, the probabilities rounded to halfs for the second product.
- * max_new_tokens chooses between the kernels for few and for many rows of a sequence; launches with more rows than that are served. */
+ * max_new_tokens chooses between the kernels for few and for many rows of a sequence; launches with more rows than that are served. In how many
+ * parts the positions of a sequence are dealt out follows from pages_per_sequence when the op is created; the parts' workspace is at most 256 MB. */
 typedef struct {
   mldhip_kv4_cache_desc cache;
   int32_t heads; /* a multiple of cache.kv_heads; max_tokens * heads is at most 2^30 */

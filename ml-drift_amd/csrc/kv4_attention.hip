@@ -108,9 +108,10 @@ struct Unpack {
 //                                                              probabilities go from one product to the next in registers
 // Keys and values are dequantized, exactly (kv4.h), so that the scores are fp32 sums of exact products: sums over the codes on their bases
 // would be rounded at the size of 1024 sum |q| and lose the small codes of a group with one channel far from zero.
-// Measured: 4 sequences of 65536 positions, 8 key heads of 128 (285 MB): 56.9 us with the join, 5.0 TB/s where a large copy reaches 4.9.  Shorter
-// caches are bound by vector instructions (about 300 for 32 positions, most of them unpacking: they alone could take heads of 128 in at 10 TB/s,
-// of 64 at 5.4) and by what precedes the first product: lengths, table, codes, one after the other, 3 to 4 us.
+// Measured: 4 sequences of 65536 positions, 8 key heads of 128 (285 MB): 58 us with the join, 4.9 TB/s, what a large copy reaches.  Shorter caches
+// are bound by vector instructions (287 for 32 positions of heads of 128, 184 of 64, most of them unpacking, 8 of them exponentials of four times the
+// cycles: they alone could take heads of 128 in at 8.6 TB/s, of 64 at 6.8) and by what precedes the first product: lengths, table, codes, one
+// after the other, 2 to 4 us.
 template <int D, int GJ>
 struct FewShape {
   static constexpr int P = Kv4Plane(D), kPlanes = D / P, kWords = P / 32, kCell = P / 16;
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
 
     for (int step = begin; step < end; step += WAVES) {
       // The further a wave is in its step, the sooner its instructions go: the waves of a SIMD stay apart, one waits for its bytes while another
-      // has the vector unit (32 sequences up to 4096, 8 heads of 128: 30.7 -> 28.0 us; 4 of 65536: 64.4 -> 60.3).
+      // has the vector unit (32 sequences up to 4096, 8 heads of 128: 28.5 -> 28.1 us; 4 of 65536: 65.3 -> 61.1).
       __builtin_amdgcn_s_setprio(1);
       // scores: score[u][i] = q . k of row n and position 16 u + 4 quad + i
       float score[kTiles][4];
@@ -494,7 +495,7 @@ __global__ __launch_bounds__(64 * WAVES, FewOnSimd(D)) void kv4_attention_few_ke
 // The maximum of a row is left as it is while the scores stay within 2^kSlack of it: the outputs are scaled down rarely.  Probabilities are up
 // to 2^(kManyLift + kSlack) = 2^14 then and keep 11 bits as halfs down to 2^-22 of the largest.
 // Measured: 8192 tokens, 32 heads over 8 of 128 (550 GFLOP): 561 us, 980 TFLOP/s where a large library product reaches 1156.  Vector
-// instructions take 59 % of a SIMD's cycles (exponentials 23, dequantizing 15), products 46 %: with one instruction issued at a time for a wave
+// instructions take 59 % of a SIMD's cycles (exponentials 23, dequantizing 15), products 45 %: with one instruction issued at a time for a wave
 // and two waves on a SIMD the two overlap little.  A fill, the first loads and the outputs of a work-group are 10 us around its steps.
 constexpr float kManyLift = 8.0f, kSlack = 6.0f;  // (in powers of two)
 constexpr int ManyWaves(int head_dim) { return head_dim == 256 ? 4 : 8; }
@@ -884,8 +885,8 @@ struct JoinParams {
 };
 constexpr int kMostParts = 256, kFewParts = 8;
 // Rows of a sequence up to which the kernel for few rows serves it.  It does a tile of 16 rows at a time, the other one up to 256 at once.
-// 8 key heads of 128, few against many, 8 sequences of 2048 positions: 20.4 / 27.4 us at 48 rows, 35.7 / 36.8 at 128; 32 of 4096: 66.8 / 68.0
-// at 32, 90.0 / 90.2 at 48, 117.6 / 90.1 at 64.  8 of 64: 61.1 / 72.3 at 48, 77.0 / 71.8 at 64.  One of 256: 18.6 / 29.2 and 55.8 / 52.5 at 128.
+// Few against many, 8 sequences of 2048 positions / 32 of 4096.  8 key heads of 128: 19.2, 22.8 / 77.8, 82.2 us at 48 rows, 20.5, 25.5 / 101.1, 94.3 at 64.
+// 8 of 64: 14.6, 18.2 / 50.1, 51.7 at 48, 24.6, 22.2 / 126.0, 70.7 at 128.  One of 256: 16.9, 22.4 / 35.0, 38.5 at 64, 18.6, 31.4 / 50.7, 46.9 at 128.
 constexpr int FewRows(int head_dim) { return head_dim == 256 ? 128 : 48; }
 
 // Of a part the weight in a row whose largest maximum is `best`: 0 where it saw nothing, whatever its output holds.
@@ -1091,12 +1092,12 @@ Kv4AttentionPlan PlanKv4Attention(const Kv4AttentionArgs& a) {
     const long long few_keys = a.window > 0 ? std::min<long long>(keys, a.window + most_new) : keys;  // that a tile may see
     const long long groups = row_tiles(many ? std::min<long long>(rows, few_rows) : rows, 16);
     // Work-groups of all the waves that a CU holds where they fill the CUs and each wave has a step: fewer outputs to join, none with as many
-    // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 28.1 us against 29.9 in 3 parts of 4 waves; 16 of up to 2047,
-    // four tokens each, 16 heads of 64: 16.7 against 17.9 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of
-    // 1000 positions, a key head of 256: 11.9 us against 12.8).
+    // tiles as CUs (32 sequences of up to 4096 positions, 8 key heads of 128: 28.2 us against 29.0 in 3 parts of 4 waves; 16 of up to 2047,
+    // four tokens each, 16 heads of 64: 15.8 against 16.4 in 4).  Else work-groups of 4 waves, as many as are on the chip at once (one sequence of
+    // 1000 positions, a key head of 256: 11.1 us in 8 of them, 17.8 in one).
     const int full = 4 * FewOnSimd(a.head_dim), waves = 256 * full;  // of a CU; of the chip
-    // And where one such work-group has a step for each wave: no second kernel (one sequence of 256 positions, 8 heads of 128: 7.3 us against 10.4
-    // from the host, 6.8 against 7.7 in a graph; of 512, heads of 64: 7.9 / 11.0 and 7.2 / 6.8; up to 128 positions are one of 4 waves).
+    // And where one such work-group has a step for each wave: no second kernel (one sequence of 256 positions, 8 heads of 128: 6.9 us against 9.6
+    // from the host, 6.6 against 7.6 in a graph; of 512, heads of 64: 7.2 / 9.9 and 7.1 / 6.7; up to 128 positions are one of 4 waves).
     const bool fills = 256 / groups * groups >= 192 && 256 / groups * 32 * full <= few_keys, one_step = few_keys > 128 && few_keys <= 32 * full;
     plan.few_waves = groups <= 256 && (fills || one_step) ? full : 4;
     plan.few_parts = parts(t.kv4_parts > 0 ? std::min<long long>(t.kv4_parts, (keys + 127) / 128)

@@ -7,9 +7,10 @@
 // codes do not depend on how a division rounds.  Inputs are held to +-57344 and NaN counts as 0: a cached value is always a finite half,
 // and a masked position can never turn a product into NaN.
 //
-// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.63.  Reading 8 sequences of 8192 tokens, 8 heads of 128 (340 MB): 75 us,
-// 4.5 TB/s where a large copy reaches 4.9 (four fifths of the bytes are stores).  5000 fp32 tokens of one head of 256 (12 MB): 8.1 us to append, 6.8 to
-// read, and one token of 64 sequences 3.7 and 2.7: lengths, table and data, one after the other.
+// Memory bounds it: tensors of 2 or 4 bytes a channel against 0.53 .. 0.63.  Reading 8 sequences of 8192 tokens, 8 heads of 128 (340 MB): 69 us,
+// 4.9 TB/s as a large copy (four fifths of the bytes are stores; 75 us under the profiler).  5000 fp32 tokens of one head of 256 (12 MB) are 8.0 us to append,
+// bound by the branches of the corrected quotients between 2-byte stores, and 6.8 to read, where each piece's words are waited for behind the stores of
+// the piece before.  One token of 64 sequences: 3.7 and 2.8, lengths, table and data, one after the other.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -81,7 +82,7 @@ __device__ __forceinline__ void Store4(float4* p, const float v[4]) { *p = make_
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-// Stores past the L2, for results that are larger (8 sequences of 8192 tokens, 8 heads of 128: 83.6 -> 75.4 us).
+// Stores past the L2, for results that are larger (8 sequences of 8192 tokens, 8 heads of 128: 82 -> 70 us; 83.6 -> 75.4 under the profiler).
 __device__ __forceinline__ void Stream4(uint2* p, const float v[4]) {
   uint2 raw;
   Store4(&raw, v);
