@@ -224,6 +224,8 @@ class AttentionBlock:
         tokens).  tokens: rows of the tensors, starts[-1] unless given (padded batches)."""
         torch = self.torch
         page_table, lengths, starts = [np.asarray(a, np.int32) for a in (page_table, lengths, starts)]
+        if page_table.ndim == 1 and len(self.page_table) == 1:
+            page_table = page_table[None]  # (of one sequence)
         for name, a, to in (("page_table", page_table, self.page_table), ("lengths", lengths, self.lengths), ("starts", starts, self.starts)):
             if a.shape != tuple(to.shape):
                 raise ValueError("%s: %s where the block has %s" % (name, a.shape, tuple(to.shape)))

@@ -20,3 +20,9 @@ def test_batches_that_do_not_fit_the_block_are_refused():
         with pytest.raises(ValueError):
             block.set_batch(**dict(dict(page_table=table, lengths=[3, 20, 5], starts=[0, 2, 2, 7], tokens=8), **bad))
         assert block.tokens == 8 and all((a == b).all() for a, b in zip(was, (block.page_table, block.lengths, block.starts, block.positions)))
+
+
+def test_a_block_of_one_sequence_takes_its_pages_as_a_row():
+    block = AttentionBlock(heads=2, kv_heads=1, head_dim=64, hidden=64, max_tokens=4, pages=3, page_size=16, device="cpu")
+    block.set_batch([2, 0, 1], [20], [0, 4])
+    assert block.page_table.tolist() == [[2, 0, 1]] and block.positions.tolist() == [16, 17, 18, 19]
