@@ -437,8 +437,8 @@ int mldhip_conv_int8_create(const mldhip_conv_int8_desc* desc, mldhip_op** op);
  *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * frequency_i, for the pairs of the first rotary_dim channels of a head:
  *   channels (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved is set; frequency_i = base^(-2 i / rotary_dim), or
  *   frequencies[i] (host memory, read by the create call) where that is given.  Channels behind rotary_dim are normed only.
- * fp32 arithmetic, one rounding to the tensors' type.  Whole turns are taken out exactly at every int32 position (frequencies of up to 2^60); what
- * is left of an angle is off by 2^-28 turns at most where tensors are fp32, and by 2^-26 where they are halfs.
+ * fp32 arithmetic, one rounding to the tensors' type.  Angles are reduced in integers, within 2^-32 turns at every int32 position (frequencies of up
+ * to 2^60), before they are rounded to fp32: an eighth of a turn at most for fp32 tensors, half a turn for halfs.
  * src objects: 0 "src_q" [heads * head_dim / 4][tokens][4], 1 "src_k" [kv_heads * head_dim / 4][tokens][4], 2 "positions" int32 [tokens],
  * and with norms 3 "q_norm_weight", 4 "k_norm_weight" [head_dim] of the tensors' type.  dst objects: 0 "dst_q", 1 "dst_k", as the sources;
  * each may be its source's buffer itself.  head_dim and rotary_dim are multiples of 8, head_dim at most 256. */
@@ -499,8 +499,8 @@ int mldhip_kv4_read_create(const mldhip_kv4_cache_desc* cache, int dst_type, int
 
 /* Attention of the rows over what the cache holds of their sequence (their own positions appended before):
  *   out_r = sum_t softmax_t(scale * q_r . k_t) v_t,  t < lengths[s]; causal: t <= position of r; window > 0: t > position of r - window.
- * A row that sees no position is 0, one with an infinity or a NaN that sees any is NaN.  Query head h reads key / value head h / (heads / kv_heads).  src objects: 0 "src_q"
- * [heads * head_dim / 4][tokens][4] halfs, 1 "cache", 2 "page_table", 3 "lengths", 4 "starts"; dst 0 "dst_tensor", as src_q (another buffer).
+ * A row that sees no position is 0, one with an infinity or a NaN that sees any is NaN.  Query head h reads key / value head
+ * h / (heads / kv_heads).  src objects: 0 "src_q" [heads * head_dim / 4][tokens][4] halfs, 1 "cache", 2 "page_table", 3 "lengths", 4 "starts"; dst 0 "dst_tensor", as src_q (another buffer).
  * fp16 tensors; scores, softmax and sums in fp32, the probabilities rounded to halfs for the second product.
  * max_new_tokens chooses between the kernels for few and for many rows of a sequence; launches with more rows than that are served. In how many
  * parts the positions of a sequence are dealt out follows from pages_per_sequence when the op is created; the parts' workspace is at most 256 MB. */
